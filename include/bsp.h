@@ -423,6 +423,139 @@ bsp_status bsp_attn_host(bsp_device* dev, int64_t S, int64_t d, int64_t nnzb, co
                          const int32_t* col_idx, const uint16_t* Q, const uint16_t* K,
                          const uint16_t* V, float scale, uint16_t* O, const bsp_spmm_opts* opts);
 
+/* ---- decoder attention around the block-sparse step ----------------------
+ * Rotary positions, a paged key/value cache held in 8 bits, attention over
+ * whole prompts and attention of single tokens over that cache.  The
+ * reference has no counterpart.
+ *
+ * x[token][head][d] tensors are bf16 (rotary also f32) given as a pointer, the
+ * strides of one token and of one head in elements (d itself is contiguous);
+ * 16-byte aligned pointers, strides that are multiples of 16 bytes.  Tokens of
+ * several sequences are packed one after the other.  Query head h uses
+ * key/value head h / (heads / kv_heads).  Index arrays (positions, starts,
+ * lengths, page tables) live on the device and are read by the kernels, so
+ * nothing here synchronises and every execute can be captured in a graph; an
+ * index outside its table is met by the kernel's own bounds checks, which skip
+ * the access and latch an error that bsp_device_synchronize reports as
+ * BSP_ERR_INVALID_ARG. */
+
+/* Rotary positions.  Pair i < rot/2 of a head is (x[i], x[i + rot/2]) for
+ * BSP_ROPE_HALF and (x[2i], x[2i + 1]) for BSP_ROPE_INTERLEAVED;
+ *   y[a] = x[a] cos - x[b] sin,   y[b] = x[b] cos + x[a] sin
+ * with (cos, sin) of the token's position from the table; the last d - rot
+ * values of a head are copied.  transpose != 0 applies the transposed rotation
+ * (sin negated): the gradient of x from the gradient of y.  y may be x. */
+typedef enum bsp_rope_layout { BSP_ROPE_HALF = 0, BSP_ROPE_INTERLEAVED = 1 } bsp_rope_layout;
+
+/* Frequencies f_i = base^(-2i/rot), changed for contexts longer than trained:
+ *   NONE    f_i
+ *   LINEAR  f_i / factor
+ *   BASE    base replaced by base * factor^(rot / (rot - 2)): the slowest pair
+ *           turns factor times slower, the fastest as before (rot > 2)
+ *   PARTS   f_i k_i + f_i / factor (1 - k_i), k_i = clamp((t_i - slow) /
+ *           (fast - slow), 0, 1), t_i = context f_i / (2 pi) the turns that the
+ *           pair makes in the trained context
+ * magnitude multiplies cos and sin (0 stands for 1). */
+typedef enum bsp_rope_kind {
+  BSP_ROPE_NONE = 0, BSP_ROPE_LINEAR = 1, BSP_ROPE_BASE = 2, BSP_ROPE_PARTS = 3
+} bsp_rope_kind;
+typedef struct bsp_rope_scaling {
+  int32_t kind;
+  double factor;
+  double context;     /* PARTS: trained context in tokens */
+  double slow, fast;  /* PARTS: turns at which the ramp begins and ends */
+  double magnitude;
+} bsp_rope_scaling;
+
+/* table: float [n_pos][rot/2][2] of (cos, sin) on the device, the angle
+ * position * f_i formed and reduced in 64 bits.  scaling NULL: NONE. */
+bsp_status bsp_rope_table(bsp_device* dev, int64_t n_pos, int32_t rot, double base,
+                          const bsp_rope_scaling* scaling, float* table, void* stream);
+/* d % 16 == 0, rot % 16 == 0, 16 <= rot <= d <= 512; type BSP_BF16 or BSP_F32
+ * (x and y); positions: int32 [tokens], each in [0, n_pos). */
+bsp_status bsp_rope(bsp_device* dev, const void* x, int64_t x_token, int64_t x_head, const int32_t* positions,
+                    const float* table, int64_t n_pos, int64_t tokens, int32_t heads, int32_t d, int32_t rot,
+                    bsp_rope_layout layout, int32_t transpose, bsp_dtype type, void* y, int64_t y_token,
+                    int64_t y_head, void* stream);
+
+/* A key/value cache of pages: k and v hold e4m3 codes, code t of head h of
+ * page p at p * page_stride + h * head_stride + t * d (bytes; strides are
+ * multiples of 16); each (page, head) has one scale, a power of two, at
+ * p * kv_heads + h: value = code * scale.  page 16, 32, 64 or 128; d 64 or
+ * 128.  A non-finite value is held as the NaN code. */
+typedef struct bsp_kv_cache {
+  void* k;
+  void* v;
+  float* k_scale;
+  float* v_scale;
+  int64_t n_pages;
+  int64_t page_stride, head_stride;
+  int32_t kv_heads, page, d;
+} bsp_kv_cache;
+
+/* Appends the tokens [starts[s], starts[s + 1]) of each sequence s behind the
+ * before[s] tokens that its pages hold (page_table[s * table_stride + i] holds
+ * positions i * page ...).  With a rotary table, keys are rotated at their
+ * position before they are stored (table NULL: stored as they are).
+ * Optional: q [tokens][heads][d] rotated to q_out, rotated keys to k_out
+ * (NULL skips them; q_out may be q, k_out may be k).
+ * A (page, head) keeps the smallest power of two e that holds its largest
+ * magnitude in e4m3's range (448); when later tokens need a larger one, the
+ * page's earlier codes are rounded to it again (exact but for values that
+ * fall below e4m3's normal range).  Pages of different sequences must differ.
+ * starts: int32 [n_seqs + 1]; before: int32 [n_seqs]; tokens = starts[n_seqs]. */
+bsp_status bsp_kv_append(bsp_device* dev, const bsp_kv_cache* cache, const void* k, int64_t k_token, int64_t k_head,
+                         const void* v, int64_t v_token, int64_t v_head, int64_t tokens, int32_t n_seqs,
+                         const int32_t* starts, const int32_t* before, const int32_t* page_table,
+                         int64_t table_stride, int64_t table_width, const float* table, int64_t n_pos, int32_t rot,
+                         bsp_rope_layout layout, const void* q, int64_t q_token, int64_t q_head, int32_t heads,
+                         void* q_out, int64_t qo_token, int64_t qo_head, void* k_out, int64_t ko_token,
+                         int64_t ko_head, void* stream);
+
+/* Attention over whole prompts (or their later parts), packed:
+ *   O_i = sum_j softmax_j(scale q_i k_j) v_j   within each sequence,
+ * with causal != 0 over the keys j <= i + (kv_len - q_len): the last query sees
+ * every key.  A query that sees no key gets O = 0 and lse = -inf.  lse (may be
+ * NULL): float [tokens][heads], the log of the sum of exp(scale q k).
+ * A plan belongs to one set of lengths (host arrays) and head counts and
+ * serves every layer and step of that batch, on any stream.  d 64 or 128.
+ * Scores, softmax and sums in fp32; probabilities are rounded to bf16 for the
+ * product with V; O is rounded once.  Options: max_ctas, timeout_ms. */
+typedef struct bsp_prompt_plan bsp_prompt_plan;
+
+bsp_status bsp_prompt_plan_create(bsp_device* dev, int32_t n_seqs, const int32_t* q_lens, const int32_t* kv_lens,
+                                  int32_t heads, int32_t kv_heads, int32_t d, int32_t causal,
+                                  const bsp_spmm_opts* opts, bsp_prompt_plan** out);
+bsp_status bsp_prompt_execute(const bsp_prompt_plan* plan, const void* q, int64_t q_token, int64_t q_head,
+                              const void* k, int64_t k_token, int64_t k_head, const void* v, int64_t v_token,
+                              int64_t v_head, float scale, void* o, int64_t o_token, int64_t o_head, float* lse,
+                              void* stream);
+bsp_status bsp_prompt_plan_destroy(bsp_prompt_plan* plan);
+/* info[0] work units, [1] grid, [2] query tokens, [3] key tokens, [4] heads,
+ * [5] kv_heads, [6] d, [7] key tiles over all units, [8] table bytes,
+ * [9] shared memory, [10] TMEM columns, [11] heads packed into a tile's rows. */
+bsp_status bsp_prompt_plan_info(const bsp_prompt_plan* plan, int64_t info[16]);
+
+/* Attention of one new token of each sequence over the cache: q, o
+ * [n_seqs][heads][d] bf16; lens[s] tokens of sequence s are in the cache (the
+ * new one included, if it was appended); lse (may be NULL): float
+ * [n_seqs][heads].  A sequence of length 0 gets O = 0 and lse = -inf.  What the
+ * pages hold behind lens[s] is never used.  The plan is a workspace for up to
+ * max_seqs sequences (any lengths) that one launch uses at a time: run a
+ * plan's launches on one stream.  Options: max_ctas, timeout_ms. */
+typedef struct bsp_decode_plan bsp_decode_plan;
+
+bsp_status bsp_decode_plan_create(bsp_device* dev, int32_t max_seqs, int32_t heads, int32_t kv_heads, int32_t d,
+                                  int32_t page, const bsp_spmm_opts* opts, bsp_decode_plan** out);
+bsp_status bsp_decode_execute(const bsp_decode_plan* plan, const bsp_kv_cache* cache, const void* q, int64_t q_token,
+                              int64_t q_head, int32_t n_seqs, const int32_t* lens, const int32_t* page_table,
+                              int64_t table_stride, int64_t table_width, float scale, void* o, int64_t o_token,
+                              int64_t o_head, float* lse, void* stream);
+bsp_status bsp_decode_plan_destroy(bsp_decode_plan* plan);
+/* info[0] max_seqs, [1] grid, [2] heads, [3] kv_heads, [4] d, [5] page,
+ * [8] workspace bytes, [9] shared memory. */
+bsp_status bsp_decode_plan_info(const bsp_decode_plan* plan, int64_t info[16]);
+
 /* ---- multi-GPU helpers (host logic; the exchange itself is NCCL) --------
  * Contiguous block-row ranges for `parts` GPUs balanced by nonzero-block
  * count (a generalisation of the reference's serpentine balancer,

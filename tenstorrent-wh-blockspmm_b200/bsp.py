@@ -36,6 +36,9 @@ EXPORTS = [
     "bsp_spgemm_plan_destroy", "bsp_spgemm_plan_info", "bsp_spgemm_host", "bsp_spgemm_plan_inspect",
     "bsp_attn_plan_create", "bsp_attn_execute", "bsp_attn_plan_destroy", "bsp_attn_plan_info",
     "bsp_attn_host", "bsp_attn_plan_inspect", "bsp_spmm_plan_traffic", "bsp_spmm_plan_entry_rows",
+    "bsp_rope_table", "bsp_rope", "bsp_kv_append", "bsp_prompt_plan_create", "bsp_prompt_execute",
+    "bsp_prompt_plan_destroy", "bsp_prompt_plan_info", "bsp_decode_plan_create", "bsp_decode_execute",
+    "bsp_decode_plan_destroy", "bsp_decode_plan_info",
 ]
 IPC_HANDLE_BYTES = 64
 
@@ -61,6 +64,23 @@ class SpmmHostJob(ctypes.Structure):
         ("M", ctypes.c_int64), ("K", ctypes.c_int64), ("R", ctypes.c_int32), ("C", ctypes.c_int32),
         ("nnzb", ctypes.c_int64), ("row_ptr", ctypes.c_void_p), ("col_idx", ctypes.c_void_p),
         ("values", ctypes.c_void_p), ("B", ctypes.c_void_p), ("N", ctypes.c_int64), ("C_out", ctypes.c_void_p),
+    ]
+
+
+class RopeScaling(ctypes.Structure):
+    """bsp_rope_scaling: how a rotary table is stretched for long contexts."""
+    _fields_ = [
+        ("kind", ctypes.c_int32), ("factor", ctypes.c_double), ("context", ctypes.c_double),
+        ("slow", ctypes.c_double), ("fast", ctypes.c_double), ("magnitude", ctypes.c_double),
+    ]
+
+
+class KvCacheDesc(ctypes.Structure):
+    """bsp_kv_cache: a paged 8-bit key/value cache (device pointers)."""
+    _fields_ = [
+        ("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("k_scale", ctypes.c_void_p), ("v_scale", ctypes.c_void_p),
+        ("n_pages", ctypes.c_int64), ("page_stride", ctypes.c_int64), ("head_stride", ctypes.c_int64),
+        ("kv_heads", ctypes.c_int32), ("page", ctypes.c_int32), ("d", ctypes.c_int32),
     ]
 
 
@@ -160,6 +180,19 @@ def lib():
         "bsp_buffer_free": (S, [P, P]),
         "bsp_buffer_write": (S, [P, P, P, I64]),
         "bsp_buffer_read": (S, [P, P, P, I64]),
+        "bsp_rope_table": (S, [P, I64, I32, ctypes.c_double, ctypes.POINTER(RopeScaling), P, P]),
+        "bsp_rope": (S, [P, P, I64, I64, P, P, I64, I64, I32, I32, I32, S, I32, S, P, I64, I64, P]),
+        "bsp_kv_append": (S, [P, ctypes.POINTER(KvCacheDesc), P, I64, I64, P, I64, I64, I64, I32, P, P, P, I64, I64,
+                              P, I64, I32, S, P, I64, I64, I32, P, I64, I64, P, I64, I64, P]),
+        "bsp_prompt_plan_create": (S, [P, I32, P, P, I32, I32, I32, I32, ctypes.POINTER(Opts), ctypes.POINTER(P)]),
+        "bsp_prompt_execute": (S, [P, P, I64, I64, P, I64, I64, P, I64, I64, ctypes.c_float, P, I64, I64, P, P]),
+        "bsp_prompt_plan_destroy": (S, [P]),
+        "bsp_prompt_plan_info": (S, [P, ctypes.POINTER(I64)]),
+        "bsp_decode_plan_create": (S, [P, I32, I32, I32, I32, I32, ctypes.POINTER(Opts), ctypes.POINTER(P)]),
+        "bsp_decode_execute": (S, [P, ctypes.POINTER(KvCacheDesc), P, I64, I64, I32, P, P, I64, I64, ctypes.c_float,
+                                   P, I64, I64, P, P]),
+        "bsp_decode_plan_destroy": (S, [P]),
+        "bsp_decode_plan_info": (S, [P, ctypes.POINTER(I64)]),
     }
     for name, (res, args) in sig.items():
         fn = getattr(L, name)
@@ -695,6 +728,299 @@ def inspect_attn_plan(S, d, row_ptr, col_idx, opts=None, sm_count=148, max_smem=
     dd = {k: int(info[i]) for i, k in enumerate(ATTN_INFO_KEYS) if not k.startswith("_")}
     dd.update(unit_table=units[: int(info[0])], chunk_table=chunks[: int(info[2])], cta_begin=cta)
     return dd
+
+
+# ------------------------------------------- attention of a decoder model --
+ROPE_LAYOUTS = {"half": 0, "interleaved": 1}
+ROPE_KINDS = {"none": 0, "linear": 1, "base": 2, "parts": 3}
+
+
+def _refuse(msg):
+    raise BspError(BSP_ERR_INVALID_ARG, msg)
+
+
+def _heads_tensor(x, name, heads=None, d=None, tokens=None, f32=False):
+    """A [tokens, heads, d] operand on the GPU: bf16 (or f32), d contiguous."""
+    import torch
+
+    if not x.is_cuda or x.dim() != 3 or not (x.dtype is torch.bfloat16 or (f32 and x.dtype is torch.float32)):
+        _refuse(f"{name} must be a bf16{' or f32' if f32 else ''} cuda tensor [tokens, heads, d]")
+    n, h, e = x.shape
+    if (heads is not None and h != heads) or (d is not None and e != d) or (tokens is not None and n != tokens):
+        _refuse(f"{name} is {tuple(x.shape)}, expected {(tokens, heads, d)}")
+    if x.stride(2) != 1 and e > 1:
+        _refuse(f"{name}: the values of a head must be contiguous")
+    return x
+
+
+def _index_tensor(x, name, dim=1):
+    import torch
+
+    if not x.is_cuda or x.dtype is not torch.int32 or x.dim() != dim or (x.numel() and x.stride(-1) != 1):
+        _refuse(f"{name} must be an int32 cuda tensor of {dim} dimension(s), contiguous rows")
+    return x
+
+
+def _rope_tensor(table):
+    import torch
+
+    if not table.is_cuda or table.dtype is not torch.float32 or table.dim() != 3 or table.shape[2] != 2 \
+            or not table.is_contiguous():
+        _refuse("a rotary table is a contiguous f32 cuda tensor [positions, rot / 2, 2]")
+    return table
+
+
+def _rope_layout(layout):
+    if layout not in ROPE_LAYOUTS:
+        _refuse(f"rotary layout {layout!r}: one of {sorted(ROPE_LAYOUTS)}")
+    return ROPE_LAYOUTS[layout]
+
+
+def _stride3(x, dim):
+    # a dimension of one entry may carry any stride: it is never stepped over
+    return x.stride(dim) if x.shape[dim] > 1 else 0
+
+
+def rope_table(n_pos, rot, base=10000.0, kind="none", factor=1.0, context=0.0, slow=1.0, fast=32.0, magnitude=1.0,
+               dev: Device = None, stream=None):
+    """Rotary table [n_pos, rot / 2, 2] of (cos, sin) for `rot` rotated values
+    of each head; kind "linear", "base" or "parts" stretches it for contexts
+    longer than trained (bsp_rope_table)."""
+    import torch
+
+    dev = dev or device(torch.cuda.current_device())
+    if kind not in ROPE_KINDS:
+        _refuse(f"scaling {kind!r}: one of {sorted(ROPE_KINDS)}")
+    if n_pos < 1 or rot < 2:
+        _refuse("n_pos and rot must be positive")
+    table = torch.empty((n_pos, rot // 2, 2), dtype=torch.float32, device=torch.device("cuda", dev.ordinal))
+    sc = RopeScaling(ROPE_KINDS[kind], factor, context, slow, fast, magnitude)
+    _check(lib().bsp_rope_table(dev.handle, n_pos, rot, base, ctypes.byref(sc), _ptr(table), _stream_ptr(stream)))
+    return table
+
+
+def rope(x, positions, table, layout="half", transpose=False, out=None, dev: Device = None, stream=None):
+    """Rotary positions of x [tokens, heads, d] (bf16 or f32): pairs
+    (i, i + rot/2) for "half", (2i, 2i + 1) for "interleaved"; the rest of a
+    head is copied.  transpose=True gives the gradient of x from that of the
+    result.  out may be x."""
+    import torch
+
+    _heads_tensor(x, "x", f32=True)
+    _index_tensor(positions, "positions")
+    _rope_tensor(table)
+    tokens, heads, d = x.shape
+    if positions.shape[0] != tokens:
+        _refuse(f"{positions.shape[0]} positions for {tokens} tokens")
+    if out is None:
+        out = torch.empty((tokens, heads, d), dtype=x.dtype, device=x.device)
+    else:
+        _heads_tensor(out, "out", heads, d, tokens, f32=True)
+        if out.dtype is not x.dtype:
+            _refuse("out must have the type of x")
+    if tokens == 0 or heads == 0:
+        return out
+    dev = dev or device(x.device.index or 0)
+    _check(lib().bsp_rope(dev.handle, x.data_ptr(), _stride3(x, 0), _stride3(x, 1), positions.data_ptr(),
+                          table.data_ptr(), table.shape[0], tokens, heads, d, 2 * table.shape[1],
+                          _rope_layout(layout), int(bool(transpose)), F32 if x.dtype is torch.float32 else BF16,
+                          out.data_ptr(), _stride3(out, 0), _stride3(out, 1), _stream_ptr(stream)))
+    return out
+
+
+class KvCache:
+    """A paged key/value cache in e4m3: k, v [pages, kv_heads, page, d] (uint8
+    or float8_e4m3fn), k_scale, v_scale f32 [pages, kv_heads], powers of two;
+    value = code * scale of its (page, head)."""
+
+    def __init__(self, k, v, k_scale, v_scale):
+        import torch
+
+        for x, name in ((k, "k"), (v, "v")):
+            if not x.is_cuda or x.dim() != 4 or x.dtype not in (torch.uint8, torch.float8_e4m3fn):
+                _refuse(f"cache {name} must be a uint8 or float8_e4m3fn cuda tensor [pages, kv_heads, page, d]")
+            if x.shape != k.shape or x.stride() != k.stride() or x.stride(3) != 1 or x.stride(2) != x.shape[3]:
+                _refuse("cache k and v must have the same shape and strides, the tokens of a page contiguous")
+        for x, name in ((k_scale, "k_scale"), (v_scale, "v_scale")):
+            if not x.is_cuda or x.dtype is not torch.float32 or x.shape != k.shape[:2] or not x.is_contiguous():
+                _refuse(f"cache {name} must be a contiguous f32 cuda tensor [pages, kv_heads]")
+        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
+        n, h, page, d = k.shape
+        # strides of single-entry dimensions are never stepped over: give them a valid value
+        hs = k.stride(1) if h > 1 else page * d
+        ps = k.stride(0) if n > 1 else h * hs
+        self.desc = KvCacheDesc(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), n, ps, hs, h,
+                                page, d)
+        self._ref = ctypes.byref(self.desc)
+
+    @staticmethod
+    def empty(n_pages, kv_heads, page, d, device_index=0):
+        """A cache of n_pages zeroed pages."""
+        import torch
+
+        dv = torch.device("cuda", device_index)
+        k, v = (torch.zeros((n_pages, kv_heads, page, d), dtype=torch.uint8, device=dv) for _ in range(2))
+        ks, vs = (torch.ones((n_pages, kv_heads), dtype=torch.float32, device=dv) for _ in range(2))
+        return KvCache(k, v, ks, vs)
+
+
+def kv_append(cache: KvCache, k, v, starts, before, pages, table=None, layout="half", q=None, q_out=None, k_out=None,
+              dev: Device = None, stream=None):
+    """Append the tokens starts[s] .. starts[s + 1] of k and v [tokens,
+    kv_heads, d] behind the before[s] tokens that sequence s has in the cache;
+    pages[s, i] is the page of its positions i * page ....  With a rotary table
+    keys are rotated on the way; q [tokens, heads, d] is rotated to q_out and
+    the rotated keys go to k_out where these are given (bsp_kv_append)."""
+    c = cache.desc
+    tokens = k.shape[0]
+    _heads_tensor(k, "k", c.kv_heads, c.d)
+    _heads_tensor(v, "v", c.kv_heads, c.d, tokens)
+    _index_tensor(starts, "starts")
+    _index_tensor(before, "before")
+    _index_tensor(pages, "pages", 2)
+    n = before.shape[0]
+    if starts.shape[0] != n + 1 or pages.shape[0] != n:
+        _refuse(f"{n} sequences need {n + 1} starts and {n} rows of pages")
+    rot = n_pos = tab = 0
+    if table is not None:
+        _rope_tensor(table)
+        n_pos, rot, tab = table.shape[0], 2 * table.shape[1], table.data_ptr()
+    if (q is None) != (q_out is None):
+        _refuse("q and q_out come together")
+    qa, qs, qt = (0, 0, 0), (0, 0, 0), 0
+    if q is not None:
+        qt = q.shape[1]
+        _heads_tensor(q, "q", None, c.d, tokens)
+        _heads_tensor(q_out, "q_out", qt, c.d, tokens)
+        qa = (q.data_ptr(), _stride3(q, 0), _stride3(q, 1))
+        qs = (q_out.data_ptr(), _stride3(q_out, 0), _stride3(q_out, 1))
+    ka = (0, 0, 0)
+    if k_out is not None:
+        _heads_tensor(k_out, "k_out", c.kv_heads, c.d, tokens)
+        ka = (k_out.data_ptr(), _stride3(k_out, 0), _stride3(k_out, 1))
+    if tokens == 0 or n == 0:
+        return cache
+    dev = dev or device(k.device.index or 0)
+    _check(lib().bsp_kv_append(dev.handle, cache._ref, k.data_ptr(), _stride3(k, 0), _stride3(k, 1), v.data_ptr(),
+                               _stride3(v, 0), _stride3(v, 1), tokens, n, starts.data_ptr(), before.data_ptr(),
+                               pages.data_ptr(), _stride3(pages, 0), pages.shape[1], tab or None, n_pos, rot,
+                               _rope_layout(layout), qa[0] or None, qa[1], qa[2], qt, qs[0] or None, qs[1], qs[2],
+                               ka[0] or None, ka[1], ka[2], _stream_ptr(stream)))
+    return cache
+
+
+def _lse_tensor(lse, tokens, heads):
+    import torch
+
+    if lse is None:
+        return None
+    if not lse.is_cuda or lse.dtype is not torch.float32 or tuple(lse.shape) != (tokens, heads) \
+            or not lse.is_contiguous():
+        _refuse(f"lse must be a contiguous f32 cuda tensor {(tokens, heads)}")
+    return lse.data_ptr()
+
+
+PROMPT_INFO_KEYS = ["units", "ctas", "q_tokens", "kv_tokens", "heads", "kv_heads", "d", "tiles", "plan_bytes",
+                    "smem_bytes", "tmem_cols", "packed_heads"]
+
+
+class PromptPlan:
+    """Attention over whole prompts packed one after the other: q_lens[s]
+    queries and kv_lens[s] keys of sequence s (host lists); causal: query i
+    sees the keys up to i + (kv_len - q_len)."""
+
+    def __init__(self, dev: Device, q_lens, kv_lens, heads, kv_heads, d, causal=True, opts=None):
+        ql = np.ascontiguousarray(q_lens, dtype=np.int32)
+        kl = np.ascontiguousarray(kv_lens, dtype=np.int32)
+        if ql.ndim != 1 or ql.shape != kl.shape:
+            _refuse("q_lens and kv_lens must be lists of one length")
+        self.handle = None
+        self.dev, self.heads, self.kv_heads, self.d = dev, heads, kv_heads, d
+        self.q_tokens, self.kv_tokens = int(ql.sum(dtype=np.int64)), int(kl.sum(dtype=np.int64))
+        h = ctypes.c_void_p()
+        o = opts if opts is not None else Opts()
+        _check(lib().bsp_prompt_plan_create(dev.handle, ql.size, _ptr(ql), _ptr(kl), heads, kv_heads, d,
+                                            int(bool(causal)), ctypes.byref(o), ctypes.byref(h)))
+        self.handle = h
+        self.scale = 1.0 / float(np.sqrt(d))
+
+    def info(self) -> dict:
+        arr = (ctypes.c_int64 * 16)()
+        _check(lib().bsp_prompt_plan_info(self.handle, arr))
+        return {k: int(arr[i]) for i, k in enumerate(PROMPT_INFO_KEYS)}
+
+    def execute(self, q, k, v, o, scale=None, lse=None, stream=None):
+        """q, o: bf16 cuda [q_tokens, heads, d]; k, v [kv_tokens, kv_heads, d];
+        lse (optional): f32 [q_tokens, heads]."""
+        _heads_tensor(q, "q", self.heads, self.d, self.q_tokens)
+        _heads_tensor(o, "o", self.heads, self.d, self.q_tokens)
+        _heads_tensor(k, "k", self.kv_heads, self.d, self.kv_tokens)
+        _heads_tensor(v, "v", self.kv_heads, self.d, self.kv_tokens)
+        _check(lib().bsp_prompt_execute(
+            self.handle, q.data_ptr(), _stride3(q, 0), _stride3(q, 1), k.data_ptr(), _stride3(k, 0), _stride3(k, 1),
+            v.data_ptr(), _stride3(v, 0), _stride3(v, 1), self.scale if scale is None else float(scale), o.data_ptr(),
+            _stride3(o, 0), _stride3(o, 1), _lse_tensor(lse, self.q_tokens, self.heads), _stream_ptr(stream)))
+
+    def close(self):
+        if self.handle:
+            lib().bsp_prompt_plan_destroy(self.handle)
+            self.handle = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+
+DECODE_INFO_KEYS = ["max_seqs", "ctas", "heads", "kv_heads", "d", "page", "_6", "_7", "workspace_bytes", "smem_bytes"]
+
+
+class DecodePlan:
+    """Attention of one token of each of up to max_seqs sequences over a
+    KvCache; the plan is the workspace, lengths are given to execute."""
+
+    def __init__(self, dev: Device, max_seqs, heads, kv_heads, d, page, opts=None):
+        self.handle = None
+        self.dev, self.max_seqs, self.heads, self.kv_heads, self.d = dev, max_seqs, heads, kv_heads, d
+        h = ctypes.c_void_p()
+        o = opts if opts is not None else Opts()
+        _check(lib().bsp_decode_plan_create(dev.handle, max_seqs, heads, kv_heads, d, page, ctypes.byref(o),
+                                            ctypes.byref(h)))
+        self.handle = h
+        self.scale = 1.0 / float(np.sqrt(d))
+
+    def info(self) -> dict:
+        arr = (ctypes.c_int64 * 16)()
+        _check(lib().bsp_decode_plan_info(self.handle, arr))
+        return {k: int(arr[i]) for i, k in enumerate(DECODE_INFO_KEYS) if not k.startswith("_")}
+
+    def execute(self, cache: KvCache, q, lens, pages, o, scale=None, lse=None, stream=None):
+        """q, o: bf16 cuda [sequences, heads, d]; lens: int32 tokens in the
+        cache; pages: int32 [sequences, width]; lse (optional): f32
+        [sequences, heads]."""
+        n = q.shape[0]
+        _heads_tensor(q, "q", self.heads, self.d)
+        _heads_tensor(o, "o", self.heads, self.d, n)
+        _index_tensor(lens, "lens")
+        _index_tensor(pages, "pages", 2)
+        if lens.shape[0] != n or pages.shape[0] != n:
+            _refuse(f"{n} queries need {n} lengths and {n} rows of pages")
+        _check(lib().bsp_decode_execute(
+            self.handle, cache._ref, q.data_ptr(), _stride3(q, 0), _stride3(q, 1), n, lens.data_ptr(),
+            pages.data_ptr(), _stride3(pages, 0), pages.shape[1], self.scale if scale is None else float(scale),
+            o.data_ptr(), _stride3(o, 0), _stride3(o, 1), _lse_tensor(lse, n, self.heads), _stream_ptr(stream)))
+
+    def close(self):
+        if self.handle:
+            lib().bsp_decode_plan_destroy(self.handle)
+            self.handle = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
 
 
 # ----------------------------------------------------------------- helpers --

@@ -17,6 +17,16 @@ constexpr int kTileN = 128;        // dense columns per MMA (MMA M dimension)
 constexpr int kTmemCols = 512;     // TMEM columns per SM
 constexpr int kSmemBudget = 227 * 1024;
 
+// ---- status word bits the kernels latch ------------------------------------
+enum : unsigned int {
+  ST_TIMEOUT_PRODUCER = 1u << 0,
+  ST_TIMEOUT_MMA = 1u << 1,
+  ST_TIMEOUT_EPILOGUE = 1u << 2,
+  ST_TIMEOUT_DRAIN = 1u << 3,
+  ST_BAD_PLAN = 1u << 4,
+  ST_BAD_INDEX = 1u << 5,  // an index array (position, start, length, page) pointed outside its table
+};
+
 // ---- SpMM schedule ----------------------------------------------------------
 // One unit = a group of `nrows` consecutive block-rows x a sub-row slab of
 // height Rs x `nt` consecutive 128-column tiles of C.  Its steps (one per
@@ -445,6 +455,18 @@ struct bsp_sddmm_plan {
 };
 
 namespace bsp {
+struct OnDevice {  // make `ordinal` current for a call, put the caller's device back after
+  int prev = -1;
+  explicit OnDevice(int ordinal) {
+    if (cudaGetDevice(&prev) != cudaSuccess) prev = -1;
+    if (prev != ordinal) cudaSetDevice(ordinal);
+  }
+  ~OnDevice() {
+    int cur = -1;
+    if (prev >= 0 && cudaGetDevice(&cur) == cudaSuccess && cur != prev) cudaSetDevice(prev);
+  }
+};
+
 // error plumbing (capi.cpp)
 bsp_status set_error(bsp_status s, const std::string& msg);
 bsp_status cuda_check(cudaError_t e, const char* what);

@@ -80,13 +80,6 @@ struct WaitCtl {
   uint64_t timeout_ns;
 };
 
-enum : unsigned int {
-  ST_TIMEOUT_PRODUCER = 1u << 0,
-  ST_TIMEOUT_MMA = 1u << 1,
-  ST_TIMEOUT_EPILOGUE = 1u << 2,
-  ST_TIMEOUT_DRAIN = 1u << 3,
-  ST_BAD_PLAN = 1u << 4,
-};
 
 // Slow path of a bounded wait: poll until the phase completes, another role
 // has aborted, or ctl.timeout_ns has passed (then latch `who` into the global

@@ -317,6 +317,9 @@ bsp_status bsp_device_synchronize(bsp_device* dev) {
   if (bits) {
     cudaMemset(dev->d_status, 0, 4);
     char msg[128];
+    if (!(bits & ~ST_BAD_INDEX))
+      return set_error(BSP_ERR_INVALID_ARG,
+                       "a kernel met an index outside its table (position, start, length or page); the access was skipped");
     snprintf(msg, sizeof(msg), "a kernel wait timed out (status bits 0x%x)", bits);
     return set_error(BSP_ERR_TIMEOUT, msg);
   }
@@ -324,20 +327,6 @@ bsp_status bsp_device_synchronize(bsp_device* dev) {
 }
 
 // ------------------------------------------------ device storage ----
-namespace {
-struct OnDevice {  // make `ordinal` current for a call, put the caller's device back after
-  int prev = -1;
-  explicit OnDevice(int ordinal) {
-    if (cudaGetDevice(&prev) != cudaSuccess) prev = -1;
-    if (prev != ordinal) cudaSetDevice(ordinal);
-  }
-  ~OnDevice() {
-    int cur = -1;
-    if (prev >= 0 && cudaGetDevice(&cur) == cudaSuccess && cur != prev) cudaSetDevice(prev);
-  }
-};
-}  // namespace
-
 bsp_status bsp_buffer_alloc(bsp_device* dev, int64_t bytes, void** ptr) {
   if (!dev || !ptr || bytes < 0) return set_error(BSP_ERR_INVALID_ARG, "bad arguments");
   *ptr = nullptr;

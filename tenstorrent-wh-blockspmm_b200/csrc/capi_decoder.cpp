@@ -1,0 +1,340 @@
+// C ABI of the decoder-attention operators (declared in include/bsp.h).
+#include <math.h>
+
+#include <algorithm>
+#include <cstring>
+#include <new>
+
+#include "decoder.h"
+
+using namespace bsp;
+
+namespace {
+
+constexpr int64_t kMaxTokens = 0x7FFFFFFF;
+
+bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
+
+// A [tokens][heads][d] operand of `size`-byte elements: 16-byte vectors are
+// loaded from every head of every token.
+bsp_status check_heads(const char* name, const void* p, int64_t token, int64_t head, int size) {
+  if (!p) return set_error(BSP_ERR_INVALID_ARG, std::string(name) + " is null");
+  if (!aligned16(p) || (token * size) % 16 || (head * size) % 16)
+    return set_error(BSP_ERR_INVALID_ARG, std::string(name) + " must be 16-byte aligned with strides of 16-byte multiples");
+  if (token < 0 || head < 0) return set_error(BSP_ERR_INVALID_ARG, std::string(name) + ": negative stride");
+  return BSP_OK;
+}
+
+bsp_status check_cache(const bsp_kv_cache* c) {
+  if (!c || !c->k || !c->v || !c->k_scale || !c->v_scale) return set_error(BSP_ERR_INVALID_ARG, "null cache");
+  if (c->page != 16 && c->page != 32 && c->page != 64 && c->page != 128)
+    return set_error(BSP_ERR_INVALID_ARG, "a cache page holds 16, 32, 64 or 128 tokens");
+  if (c->d != 64 && c->d != 128) return set_error(BSP_ERR_INVALID_ARG, "head size must be 64 or 128");
+  if (c->kv_heads < 1 || c->n_pages < 1 || c->n_pages > kMaxTokens)
+    return set_error(BSP_ERR_INVALID_ARG, "bad cache dimensions");
+  const int64_t block = static_cast<int64_t>(c->page) * c->d;
+  if (c->page_stride % 16 || c->head_stride % 16 || c->page_stride < block || c->head_stride < block)
+    return set_error(BSP_ERR_INVALID_ARG, "cache strides must be multiples of 16 bytes that hold a page of one head");
+  if (!aligned16(c->k) || !aligned16(c->v))
+    return set_error(BSP_ERR_INVALID_ARG, "cache pointers must be 16-byte aligned");
+  return BSP_OK;
+}
+
+bsp_status check_rot(int32_t d, int32_t rot, int32_t layout) {
+  if (rot < 16 || rot % 16 || rot > d) return set_error(BSP_ERR_INVALID_ARG, "rot must be a multiple of 16 in [16, d]");
+  if (layout != BSP_ROPE_HALF && layout != BSP_ROPE_INTERLEAVED)
+    return set_error(BSP_ERR_INVALID_ARG, "unknown rotary layout");
+  return BSP_OK;
+}
+
+bsp_status check_attention_heads(int32_t heads, int32_t kv_heads, int32_t d) {
+  if (heads < 1 || kv_heads < 1 || heads % kv_heads)
+    return set_error(BSP_ERR_INVALID_ARG, "heads must be a positive multiple of kv_heads");
+  if (d != 64 && d != 128) return set_error(BSP_ERR_INVALID_ARG, "head size must be 64 or 128");
+  return BSP_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+bsp_status bsp_rope_table(bsp_device* dev, int64_t n_pos, int32_t rot, double base, const bsp_rope_scaling* scaling,
+                          float* table, void* stream) {
+  if (!dev || !table) return set_error(BSP_ERR_INVALID_ARG, "null argument");
+  if (!aligned16(table)) return set_error(BSP_ERR_INVALID_ARG, "the table must be 16-byte aligned");
+  if (n_pos < 1 || n_pos > kMaxTokens) return set_error(BSP_ERR_INVALID_ARG, "n_pos out of range");
+  bsp_status s = check_rot(512, rot, BSP_ROPE_HALF);
+  if (s != BSP_OK) return s;
+  if (!(base > 0) || !std::isfinite(base)) return set_error(BSP_ERR_INVALID_ARG, "base must be positive");
+  bsp_rope_scaling sc{};
+  if (scaling) sc = *scaling;
+  if (sc.kind < BSP_ROPE_NONE || sc.kind > BSP_ROPE_PARTS) return set_error(BSP_ERR_INVALID_ARG, "unknown scaling kind");
+  if (sc.kind != BSP_ROPE_NONE && (!(sc.factor > 0) || !std::isfinite(sc.factor)))
+    return set_error(BSP_ERR_INVALID_ARG, "the scaling factor must be positive");
+  if (sc.kind == BSP_ROPE_PARTS && (!(sc.context > 0) || !(sc.fast > sc.slow)))
+    return set_error(BSP_ERR_INVALID_ARG, "by parts: context > 0 and fast > slow");
+  if (!std::isfinite(sc.magnitude) || sc.magnitude < 0) return set_error(BSP_ERR_INVALID_ARG, "bad magnitude");
+  if (sc.magnitude == 0) sc.magnitude = 1;
+  OnDevice on(dev->ordinal);
+  return launch_rope_table(dev, n_pos, rot, base, sc, table, static_cast<cudaStream_t>(stream));
+}
+
+bsp_status bsp_rope(bsp_device* dev, const void* x, int64_t x_token, int64_t x_head, const int32_t* positions,
+                    const float* table, int64_t n_pos, int64_t tokens, int32_t heads, int32_t d, int32_t rot,
+                    bsp_rope_layout layout, int32_t transpose, bsp_dtype type, void* y, int64_t y_token,
+                    int64_t y_head, void* stream) {
+  if (!dev) return set_error(BSP_ERR_INVALID_ARG, "null device");
+  if (type != BSP_BF16 && type != BSP_F32) return set_error(BSP_ERR_INVALID_ARG, "type must be BSP_BF16 or BSP_F32");
+  if (tokens < 0 || heads < 1 || tokens > kMaxTokens / heads || n_pos < 0)
+    return set_error(BSP_ERR_INVALID_ARG, "bad dimensions");
+  if (d < 16 || d % 16 || d > 512) return set_error(BSP_ERR_INVALID_ARG, "d must be a multiple of 16, at most 512");
+  bsp_status s = check_rot(d, rot, layout);
+  if (s != BSP_OK) return s;
+  if (tokens == 0) return BSP_OK;
+  const int size = type == BSP_F32 ? 4 : 2;
+  if ((s = check_heads("x", x, x_token, x_head, size)) != BSP_OK) return s;
+  if ((s = check_heads("y", y, y_token, y_head, size)) != BSP_OK) return s;
+  if (!positions || !table || !aligned16(table)) return set_error(BSP_ERR_INVALID_ARG, "positions or table missing");
+  RopeParams p{};
+  p.x = {x, x_token, x_head};
+  p.y = {y, y_token, y_head};
+  p.positions = positions;
+  p.table = reinterpret_cast<const float2*>(table);
+  p.n_pos = n_pos;
+  p.tokens = tokens;
+  p.heads = heads;
+  p.d = d;
+  p.rot = rot;
+  p.interleaved = layout == BSP_ROPE_INTERLEAVED;
+  p.sign = transpose ? -1.f : 1.f;
+  p.status = dev->d_status;
+  OnDevice on(dev->ordinal);
+  return launch_rope(p, type, static_cast<cudaStream_t>(stream));
+}
+
+bsp_status bsp_kv_append(bsp_device* dev, const bsp_kv_cache* cache, const void* k, int64_t k_token, int64_t k_head,
+                         const void* v, int64_t v_token, int64_t v_head, int64_t tokens, int32_t n_seqs,
+                         const int32_t* starts, const int32_t* before, const int32_t* page_table,
+                         int64_t table_stride, int64_t table_width, const float* table, int64_t n_pos, int32_t rot,
+                         bsp_rope_layout layout, const void* q, int64_t q_token, int64_t q_head, int32_t heads,
+                         void* q_out, int64_t qo_token, int64_t qo_head, void* k_out, int64_t ko_token,
+                         int64_t ko_head, void* stream) {
+  if (!dev) return set_error(BSP_ERR_INVALID_ARG, "null device");
+  bsp_status s = check_cache(cache);
+  if (s != BSP_OK) return s;
+  if (tokens < 0 || tokens > kMaxTokens || n_seqs < 0 || table_width < 0 || table_stride < 0 || n_pos < 0)
+    return set_error(BSP_ERR_INVALID_ARG, "bad dimensions");
+  if (table) {
+    if ((s = check_rot(cache->d, rot, layout)) != BSP_OK) return s;
+    if (!aligned16(table)) return set_error(BSP_ERR_INVALID_ARG, "the table must be 16-byte aligned");
+  } else if (q || k_out) {
+    return set_error(BSP_ERR_INVALID_ARG, "q and k_out are rotated outputs: they need a rotary table");
+  }
+  if (tokens == 0 || n_seqs == 0) return BSP_OK;
+  if ((s = check_heads("k", k, k_token, k_head, 2)) != BSP_OK) return s;
+  if ((s = check_heads("v", v, v_token, v_head, 2)) != BSP_OK) return s;
+  if (q) {
+    if (heads < 1) return set_error(BSP_ERR_INVALID_ARG, "bad number of query heads");
+    if ((s = check_heads("q", q, q_token, q_head, 2)) != BSP_OK) return s;
+    if ((s = check_heads("q_out", q_out, qo_token, qo_head, 2)) != BSP_OK) return s;
+  }
+  if (2 * static_cast<int64_t>(cache->kv_heads) + (q ? heads : 0) > 65535)
+    return set_error(BSP_ERR_UNSUPPORTED, "more than 65535 heads");
+  if (k_out && (s = check_heads("k_out", k_out, ko_token, ko_head, 2)) != BSP_OK) return s;
+  if (!starts || !before || !page_table) return set_error(BSP_ERR_INVALID_ARG, "null index array");
+  AppendParams p{};
+  p.q = {q, q_token, q_head};
+  p.k = {k, k_token, k_head};
+  p.v = {v, v_token, v_head};
+  p.q_out = {q_out, qo_token, qo_head};
+  p.k_out = {k_out, ko_token, ko_head};
+  p.cache = *cache;
+  p.starts = starts;
+  p.before = before;
+  p.page_table = page_table;
+  p.table_stride = table_stride;
+  p.table_width = table_width;
+  p.table = reinterpret_cast<const float2*>(table);
+  p.n_pos = n_pos;
+  p.tokens = tokens;
+  p.n_seqs = n_seqs;
+  p.heads = heads;
+  p.rot = rot;
+  p.interleaved = layout == BSP_ROPE_INTERLEAVED;
+  p.status = dev->d_status;
+  OnDevice on(dev->ordinal);
+  return launch_append(p, static_cast<cudaStream_t>(stream));
+}
+
+bsp_status bsp_prompt_plan_create(bsp_device* dev, int32_t n_seqs, const int32_t* q_lens, const int32_t* kv_lens,
+                                  int32_t heads, int32_t kv_heads, int32_t d, int32_t causal,
+                                  const bsp_spmm_opts* opts, bsp_prompt_plan** out) {
+  if (!out) return set_error(BSP_ERR_INVALID_ARG, "null argument");
+  *out = nullptr;
+  if (!dev) return set_error(BSP_ERR_INVALID_ARG, "null device");
+  if (n_seqs < 0 || (n_seqs > 0 && (!q_lens || !kv_lens))) return set_error(BSP_ERR_INVALID_ARG, "bad lengths");
+  bsp_status s = check_attention_heads(heads, kv_heads, d);
+  if (s != BSP_OK) return s;
+  (void)opts;
+  bsp_prompt_plan* p = new (std::nothrow) bsp_prompt_plan();
+  if (!p) return set_error(BSP_ERR_ALLOC, "host allocation failed");
+  p->dev = dev;
+  p->n_seqs = n_seqs;
+  p->heads = heads;
+  p->kv_heads = kv_heads;
+  p->d = d;
+  p->causal = causal != 0;
+  try {
+    for (int32_t i = 0; i < n_seqs; ++i) {
+      if (q_lens[i] < 0 || kv_lens[i] < 0) s = set_error(BSP_ERR_INVALID_ARG, "negative length");
+      if (p->q_tokens + q_lens[i] > kMaxTokens || p->kv_tokens + kv_lens[i] > kMaxTokens)
+        s = set_error(BSP_ERR_INVALID_ARG, "too many tokens");
+      if (s != BSP_OK) break;
+      p->h_seqs.push_back({static_cast<int32_t>(p->q_tokens), q_lens[i], static_cast<int32_t>(p->kv_tokens), kv_lens[i]});
+      p->q_tokens += q_lens[i];
+      p->kv_tokens += kv_lens[i];
+    }
+  } catch (const std::bad_alloc&) {
+    s = set_error(BSP_ERR_ALLOC, "host allocation failed");
+  }
+  if (s == BSP_OK && p->q_tokens > 0) {
+    OnDevice on(dev->ordinal);
+    p->blob_bytes = p->h_seqs.size() * sizeof(PromptSeq);
+    if (cudaMalloc(&p->d_blob, p->blob_bytes) != cudaSuccess) s = set_error(BSP_ERR_ALLOC, "cudaMalloc of the plan tables failed");
+    if (s == BSP_OK)
+      s = cuda_check(cudaMemcpy(p->d_blob, p->h_seqs.data(), p->blob_bytes, cudaMemcpyHostToDevice), "upload plan tables");
+    p->d_seqs = static_cast<PromptSeq*>(p->d_blob);
+  }
+  if (s != BSP_OK) {
+    bsp_prompt_plan_destroy(p);
+    return s;
+  }
+  *out = p;
+  return BSP_OK;
+}
+
+bsp_status bsp_prompt_execute(const bsp_prompt_plan* plan, const void* q, int64_t q_token, int64_t q_head,
+                              const void* k, int64_t k_token, int64_t k_head, const void* v, int64_t v_token,
+                              int64_t v_head, float scale, void* o, int64_t o_token, int64_t o_head, float* lse,
+                              void* stream) {
+  if (!plan) return set_error(BSP_ERR_INVALID_ARG, "null plan");
+  if (plan->q_tokens == 0) return BSP_OK;
+  bsp_status s = check_heads("q", q, q_token, q_head, 2);
+  if (s == BSP_OK) s = check_heads("o", o, o_token, o_head, 2);
+  if (s == BSP_OK && plan->kv_tokens > 0) {
+    s = check_heads("k", k, k_token, k_head, 2);
+    if (s == BSP_OK) s = check_heads("v", v, v_token, v_head, 2);
+  }
+  if (s != BSP_OK) return s;
+  PromptParams p{};
+  p.q = {q, q_token, q_head};
+  p.k = {k, k_token, k_head};
+  p.v = {v, v_token, v_head};
+  p.o = {o, o_token, o_head};
+  p.lse = lse;
+  p.seqs = plan->d_seqs;
+  p.n_seqs = plan->n_seqs;
+  p.heads = plan->heads;
+  p.kv_heads = plan->kv_heads;
+  p.d = plan->d;
+  p.causal = plan->causal;
+  p.tokens = static_cast<int32_t>(plan->q_tokens);
+  p.scale = scale;
+  OnDevice on(plan->dev->ordinal);
+  return launch_prompt(plan, p, static_cast<cudaStream_t>(stream));
+}
+
+bsp_status bsp_prompt_plan_destroy(bsp_prompt_plan* plan) {
+  if (!plan) return BSP_OK;
+  if (plan->d_blob) cudaFree(plan->d_blob);
+  delete plan;
+  return BSP_OK;
+}
+
+bsp_status bsp_prompt_plan_info(const bsp_prompt_plan* p, int64_t info[16]) {
+  if (!p || !info) return set_error(BSP_ERR_INVALID_ARG, "null argument");
+  memset(info, 0, sizeof(int64_t) * 16);
+  info[0] = p->n_units;
+  info[1] = p->grid;
+  info[2] = p->q_tokens;
+  info[3] = p->kv_tokens;
+  info[4] = p->heads;
+  info[5] = p->kv_heads;
+  info[6] = p->d;
+  info[8] = static_cast<int64_t>(p->blob_bytes);
+  return BSP_OK;
+}
+
+bsp_status bsp_decode_plan_create(bsp_device* dev, int32_t max_seqs, int32_t heads, int32_t kv_heads, int32_t d,
+                                  int32_t page, const bsp_spmm_opts* opts, bsp_decode_plan** out) {
+  if (!out) return set_error(BSP_ERR_INVALID_ARG, "null argument");
+  *out = nullptr;
+  if (!dev) return set_error(BSP_ERR_INVALID_ARG, "null device");
+  if (max_seqs < 0) return set_error(BSP_ERR_INVALID_ARG, "bad max_seqs");
+  bsp_status s = check_attention_heads(heads, kv_heads, d);
+  if (s != BSP_OK) return s;
+  if (page != 16 && page != 32 && page != 64 && page != 128)
+    return set_error(BSP_ERR_INVALID_ARG, "a cache page holds 16, 32, 64 or 128 tokens");
+  (void)opts;
+  bsp_decode_plan* p = new (std::nothrow) bsp_decode_plan();
+  if (!p) return set_error(BSP_ERR_ALLOC, "host allocation failed");
+  p->dev = dev;
+  p->max_seqs = max_seqs;
+  p->heads = heads;
+  p->kv_heads = kv_heads;
+  p->d = d;
+  p->page = page;
+  *out = p;
+  return BSP_OK;
+}
+
+bsp_status bsp_decode_execute(const bsp_decode_plan* plan, const bsp_kv_cache* cache, const void* q, int64_t q_token,
+                              int64_t q_head, int32_t n_seqs, const int32_t* lens, const int32_t* page_table,
+                              int64_t table_stride, int64_t table_width, float scale, void* o, int64_t o_token,
+                              int64_t o_head, float* lse, void* stream) {
+  if (!plan) return set_error(BSP_ERR_INVALID_ARG, "null plan");
+  bsp_status s = check_cache(cache);
+  if (s != BSP_OK) return s;
+  if (cache->kv_heads != plan->kv_heads || cache->d != plan->d || cache->page != plan->page)
+    return set_error(BSP_ERR_INVALID_ARG, "the cache differs from the plan's heads, head size or page");
+  if (n_seqs < 0 || n_seqs > plan->max_seqs) return set_error(BSP_ERR_INVALID_ARG, "more sequences than the plan holds");
+  if (table_width < 0 || table_width > kMaxTokens || table_stride < 0)
+    return set_error(BSP_ERR_INVALID_ARG, "bad page table");
+  if (n_seqs == 0) return BSP_OK;
+  if ((s = check_heads("q", q, q_token, q_head, 2)) != BSP_OK) return s;
+  if ((s = check_heads("o", o, o_token, o_head, 2)) != BSP_OK) return s;
+  if (!lens || !page_table) return set_error(BSP_ERR_INVALID_ARG, "null index array");
+  DecodeParams p{};
+  p.q = {q, q_token, q_head};
+  p.o = {o, o_token, o_head};
+  p.lse = lse;
+  p.cache = *cache;
+  p.lens = lens;
+  p.page_table = page_table;
+  p.table_stride = table_stride;
+  p.table_width = table_width;
+  p.n_seqs = n_seqs;
+  p.heads = plan->heads;
+  p.scale = scale;
+  p.status = plan->dev->d_status;
+  OnDevice on(plan->dev->ordinal);
+  return launch_decode(plan, p, static_cast<cudaStream_t>(stream));
+}
+
+bsp_status bsp_decode_plan_destroy(bsp_decode_plan* plan) {
+  delete plan;
+  return BSP_OK;
+}
+
+bsp_status bsp_decode_plan_info(const bsp_decode_plan* p, int64_t info[16]) {
+  if (!p || !info) return set_error(BSP_ERR_INVALID_ARG, "null argument");
+  memset(info, 0, sizeof(int64_t) * 16);
+  info[0] = p->max_seqs;
+  info[2] = p->heads;
+  info[3] = p->kv_heads;
+  info[4] = p->d;
+  info[5] = p->page;
+  return BSP_OK;
+}
+
+}  // extern "C"
