@@ -3,8 +3,10 @@
 
 #include <algorithm>
 #include <cstring>
+#include <exception>
 #include <new>
 
+#include "bsp_testing.h"
 #include "decoder.h"
 
 using namespace bsp;
@@ -185,25 +187,27 @@ bsp_status bsp_prompt_plan_create(bsp_device* dev, int32_t n_seqs, const int32_t
   p->d = d;
   p->causal = causal != 0;
   try {
-    for (int32_t i = 0; i < n_seqs; ++i) {
-      if (q_lens[i] < 0 || kv_lens[i] < 0) s = set_error(BSP_ERR_INVALID_ARG, "negative length");
-      if (p->q_tokens + q_lens[i] > kMaxTokens || p->kv_tokens + kv_lens[i] > kMaxTokens)
-        s = set_error(BSP_ERR_INVALID_ARG, "too many tokens");
-      if (s != BSP_OK) break;
-      p->h_seqs.push_back({static_cast<int32_t>(p->q_tokens), q_lens[i], static_cast<int32_t>(p->kv_tokens), kv_lens[i]});
-      p->q_tokens += q_lens[i];
-      p->kv_tokens += kv_lens[i];
-    }
-  } catch (const std::bad_alloc&) {
+    s = plan_prompt_host(p, q_lens, kv_lens, dev->sm_count, opts);
+  } catch (const std::exception&) {
     s = set_error(BSP_ERR_ALLOC, "host allocation failed");
   }
-  if (s == BSP_OK && p->q_tokens > 0) {
+  p->smem_bytes = prompt_smem_bytes(d);
+  if (s == BSP_OK && p->n_units > 0) {
     OnDevice on(dev->ordinal);
-    p->blob_bytes = p->h_seqs.size() * sizeof(PromptSeq);
-    if (cudaMalloc(&p->d_blob, p->blob_bytes) != cudaSuccess) s = set_error(BSP_ERR_ALLOC, "cudaMalloc of the plan tables failed");
-    if (s == BSP_OK)
-      s = cuda_check(cudaMemcpy(p->d_blob, p->h_seqs.data(), p->blob_bytes, cudaMemcpyHostToDevice), "upload plan tables");
-    p->d_seqs = static_cast<PromptSeq*>(p->d_blob);
+    const size_t ub = p->h_units.size() * sizeof(PromptUnit);
+    p->blob_bytes = ub + p->h_cta_begin.size() * sizeof(int32_t);
+    if (cudaMalloc(&p->d_blob, p->blob_bytes) != cudaSuccess) {
+      p->d_blob = nullptr;
+      s = set_error(BSP_ERR_ALLOC, "cudaMalloc of the plan tables failed");
+    } else {
+      p->d_units = static_cast<PromptUnit*>(p->d_blob);
+      p->d_cta_begin = reinterpret_cast<int32_t*>(static_cast<uint8_t*>(p->d_blob) + ub);
+      s = cuda_check(cudaMemcpy(p->d_units, p->h_units.data(), ub, cudaMemcpyHostToDevice), "upload plan tables");
+      if (s == BSP_OK)
+        s = cuda_check(cudaMemcpy(p->d_cta_begin, p->h_cta_begin.data(), p->h_cta_begin.size() * sizeof(int32_t),
+                                  cudaMemcpyHostToDevice),
+                       "upload plan tables");
+    }
   }
   if (s != BSP_OK) {
     bsp_prompt_plan_destroy(p);
@@ -218,6 +222,7 @@ bsp_status bsp_prompt_execute(const bsp_prompt_plan* plan, const void* q, int64_
                               int64_t v_head, float scale, void* o, int64_t o_token, int64_t o_head, float* lse,
                               void* stream) {
   if (!plan) return set_error(BSP_ERR_INVALID_ARG, "null plan");
+  if (!(scale > 0) || !std::isfinite(scale)) return set_error(BSP_ERR_INVALID_ARG, "scale must be positive");
   if (plan->q_tokens == 0) return BSP_OK;
   bsp_status s = check_heads("q", q, q_token, q_head, 2);
   if (s == BSP_OK) s = check_heads("o", o, o_token, o_head, 2);
@@ -232,21 +237,26 @@ bsp_status bsp_prompt_execute(const bsp_prompt_plan* plan, const void* q, int64_
   p.v = {v, v_token, v_head};
   p.o = {o, o_token, o_head};
   p.lse = lse;
-  p.seqs = plan->d_seqs;
-  p.n_seqs = plan->n_seqs;
+  p.units = plan->d_units;
+  p.cta_begin = plan->d_cta_begin;
   p.heads = plan->heads;
-  p.kv_heads = plan->kv_heads;
-  p.d = plan->d;
+  p.group = plan->heads / plan->kv_heads;
+  p.packed = plan->packed;
+  p.tile_tokens = plan->tile_tokens;
   p.causal = plan->causal;
-  p.tokens = static_cast<int32_t>(plan->q_tokens);
-  p.scale = scale;
+  p.scale_log2 = scale * 1.4426950408889634f;
+  p.status = plan->dev->d_status;
+  p.timeout_ns = plan->timeout_ns;
   OnDevice on(plan->dev->ordinal);
   return launch_prompt(plan, p, static_cast<cudaStream_t>(stream));
 }
 
 bsp_status bsp_prompt_plan_destroy(bsp_prompt_plan* plan) {
   if (!plan) return BSP_OK;
-  if (plan->d_blob) cudaFree(plan->d_blob);
+  if (plan->d_blob) {
+    OnDevice on(plan->dev->ordinal);
+    cudaFree(plan->d_blob);
+  }
   delete plan;
   return BSP_OK;
 }
@@ -261,7 +271,36 @@ bsp_status bsp_prompt_plan_info(const bsp_prompt_plan* p, int64_t info[16]) {
   info[4] = p->heads;
   info[5] = p->kv_heads;
   info[6] = p->d;
+  info[7] = p->n_tiles;
   info[8] = static_cast<int64_t>(p->blob_bytes);
+  info[9] = p->smem_bytes;
+  info[10] = 512;
+  info[11] = p->packed;
+  return BSP_OK;
+}
+
+bsp_status bsp_prompt_plan_inspect(int32_t n_seqs, const int32_t* q_lens, const int32_t* kv_lens, int32_t heads,
+                                   int32_t kv_heads, int32_t d, int32_t causal, const bsp_spmm_opts* opts,
+                                   int32_t sm_count, int64_t info[16], int32_t* units_out, int32_t* cta_begin_out) {
+  if (n_seqs < 0 || (n_seqs > 0 && (!q_lens || !kv_lens)) || !info || sm_count < 1)
+    return set_error(BSP_ERR_INVALID_ARG, "bad arguments");
+  bsp_status s = check_attention_heads(heads, kv_heads, d);
+  if (s != BSP_OK) return s;
+  bsp_prompt_plan p;
+  p.n_seqs = n_seqs;
+  p.heads = heads;
+  p.kv_heads = kv_heads;
+  p.d = d;
+  p.causal = causal != 0;
+  try {
+    s = plan_prompt_host(&p, q_lens, kv_lens, sm_count, opts);
+  } catch (const std::exception&) {
+    s = set_error(BSP_ERR_ALLOC, "host allocation failed");
+  }
+  if (s != BSP_OK) return s;
+  bsp_prompt_plan_info(&p, info);
+  if (units_out && !p.h_units.empty()) memcpy(units_out, p.h_units.data(), p.h_units.size() * sizeof(PromptUnit));
+  if (cta_begin_out) memcpy(cta_begin_out, p.h_cta_begin.data(), p.h_cta_begin.size() * sizeof(int32_t));
   return BSP_OK;
 }
 
@@ -298,6 +337,7 @@ bsp_status bsp_decode_execute(const bsp_decode_plan* plan, const bsp_kv_cache* c
   if (cache->kv_heads != plan->kv_heads || cache->d != plan->d || cache->page != plan->page)
     return set_error(BSP_ERR_INVALID_ARG, "the cache differs from the plan's heads, head size or page");
   if (n_seqs < 0 || n_seqs > plan->max_seqs) return set_error(BSP_ERR_INVALID_ARG, "more sequences than the plan holds");
+  if (!(scale > 0) || !std::isfinite(scale)) return set_error(BSP_ERR_INVALID_ARG, "scale must be positive");
   if (table_width < 0 || table_width > kMaxTokens || table_stride < 0)
     return set_error(BSP_ERR_INVALID_ARG, "bad page table");
   if (n_seqs == 0) return BSP_OK;

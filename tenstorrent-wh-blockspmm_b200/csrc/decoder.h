@@ -56,19 +56,32 @@ struct DecodeParams {
   unsigned int* status;
 };
 
-struct PromptSeq {
-  int32_t q0, q_len;    // query tokens [q0, q0 + q_len)
-  int32_t kv0, kv_len;
+// A unit of prompt attention: one or two tiles (tile_tokens queries x packed
+// heads each) of consecutive queries of one sequence.
+struct PromptUnit {
+  int32_t q0, q_end;     // first query token (packed index); end of the sequence's tokens
+  int32_t kv0, kv_len;   // the sequence's keys
+  int32_t sees;          // keys that query q0 attends to (causal; may be <= 0)
+  int32_t head0;         // first query head
+  int32_t n[2];          // steps of 128 keys of tile a and b (0: the tile sees no key)
+  int32_t two;           // the unit has a tile b
+  int32_t pad[3];
 };
+static_assert(sizeof(PromptUnit) == 48, "unit layout");
 
 struct PromptParams {
+  CUtensorMap tm_q, tm_k, tm_v;   // [token][head][d], boxes {64, packed, tile_tokens} and {64, 1, 128}
   HeadsView q, k, v;
   HeadsOut o;
   float* lse;
-  const PromptSeq* seqs;
-  int32_t n_seqs, heads, kv_heads, d, causal;
-  int32_t tokens;
-  float scale;
+  const PromptUnit* units;
+  const int32_t* cta_begin;       // [grid + 1]
+  int32_t heads, group;           // group: query heads of one key/value head
+  int32_t packed, tile_tokens;
+  int32_t causal;
+  float scale_log2;
+  unsigned int* status;
+  uint64_t timeout_ns;
 };
 
 }  // namespace bsp
@@ -77,12 +90,16 @@ struct bsp_prompt_plan {
   bsp_device* dev = nullptr;
   int32_t n_seqs = 0, heads = 0, kv_heads = 0, d = 0, causal = 0;
   int64_t q_tokens = 0, kv_tokens = 0;
-  int32_t grid = 0;
-  int64_t n_units = 0;
-  void* d_blob = nullptr;
+  int32_t packed = 1, tile_tokens = 128;
+  int32_t grid = 0, smem_bytes = 0;
+  int64_t n_units = 0, n_tiles = 0;
+  uint64_t timeout_ns = 0;
+  void* d_blob = nullptr;  // units | cta_begin
   size_t blob_bytes = 0;
-  bsp::PromptSeq* d_seqs = nullptr;
-  std::vector<bsp::PromptSeq> h_seqs;
+  bsp::PromptUnit* d_units = nullptr;
+  int32_t* d_cta_begin = nullptr;
+  std::vector<bsp::PromptUnit> h_units;
+  std::vector<int32_t> h_cta_begin;
 };
 
 struct bsp_decode_plan {
@@ -96,5 +113,8 @@ bsp_status launch_rope_table(bsp_device* dev, int64_t n_pos, int32_t rot, double
 bsp_status launch_rope(const RopeParams& p, bsp_dtype type, cudaStream_t stream);
 bsp_status launch_append(const AppendParams& p, cudaStream_t stream);
 bsp_status launch_decode(const bsp_decode_plan* plan, const DecodeParams& p, cudaStream_t stream);
-bsp_status launch_prompt(const bsp_prompt_plan* plan, const PromptParams& p, cudaStream_t stream);
+bsp_status plan_prompt_host(bsp_prompt_plan* p, const int32_t* q_lens, const int32_t* kv_lens, int sm_count,
+                            const bsp_spmm_opts* opts);
+bsp_status launch_prompt(const bsp_prompt_plan* plan, PromptParams& p, cudaStream_t stream);
+int prompt_smem_bytes(int d);
 }  // namespace bsp

@@ -21,6 +21,7 @@
 #include <thread>
 
 #include "bsp_internal.h"
+#include "decoder.h"
 
 namespace bsp {
 
@@ -2428,6 +2429,85 @@ void spmm_plan_traffic(const bsp_spmm_plan& p, int64_t out[4]) {
           out[2] += 1;
         }
   }
+}
+
+// ------------------------------------------------------- prompt attention ----
+// Units are one or two tiles of 128 rows (128 / packed queries x packed heads).
+// Two tiles read each key once for both and keep the tensor cores busy while
+// one of them is in its softmax; with so few that half the CTAs would stay
+// idle, units of one tile use twice as many.  Units go, heaviest first, to
+// the CTA with the least work so far.
+bsp_status plan_prompt_host(bsp_prompt_plan* p, const int32_t* q_lens, const int32_t* kv_lens, int sm_count,
+                            const bsp_spmm_opts* opts) {
+  const int32_t group = p->heads / p->kv_heads;
+  p->packed = 1;
+  while (group % (2 * p->packed) == 0 && p->packed < 32) p->packed *= 2;
+  p->tile_tokens = 128 / p->packed;
+  const int64_t bands = p->heads / p->packed;  // row bands of a query block
+  p->timeout_ns = static_cast<uint64_t>(opts && opts->timeout_ms > 0 ? opts->timeout_ms : 2000) * 1000000ull;
+  int64_t pairs = 0;
+  for (int32_t s = 0; s < p->n_seqs; ++s) {
+    if (q_lens[s] < 0 || kv_lens[s] < 0) return set_error(BSP_ERR_INVALID_ARG, "negative length");
+    p->q_tokens += q_lens[s];
+    p->kv_tokens += kv_lens[s];
+    if (p->q_tokens > INT32_MAX - 256 || p->kv_tokens > INT32_MAX - 256)
+      return set_error(BSP_ERR_INVALID_ARG, "too many tokens");
+    pairs += (static_cast<int64_t>(q_lens[s]) + 2 * p->tile_tokens - 1) / (2 * p->tile_tokens) * bands;
+  }
+  int ctas = opts && opts->max_ctas > 0 ? std::min(opts->max_ctas, sm_count) : sm_count;
+  const int32_t tiles = 2 * pairs <= ctas ? 1 : 2;
+  if (pairs > (int64_t(1) << 28)) return set_error(BSP_ERR_UNSUPPORTED, "too many work units");
+  std::vector<PromptUnit> units;
+  units.reserve(static_cast<size_t>(pairs * 2));
+  int64_t q0 = 0, kv0 = 0;
+  for (int32_t s = 0; s < p->n_seqs; ++s) {
+    const int32_t step = tiles * p->tile_tokens;
+    for (int64_t a = 0; a < q_lens[s]; a += step) {
+      PromptUnit u{};
+      u.q0 = static_cast<int32_t>(q0 + a);
+      u.q_end = static_cast<int32_t>(q0 + q_lens[s]);
+      u.kv0 = static_cast<int32_t>(kv0);
+      u.kv_len = kv_lens[s];
+      u.sees = static_cast<int32_t>(kv_lens[s] - q_lens[s] + a + 1);
+      u.two = tiles == 2 && a + p->tile_tokens < q_lens[s];
+      for (int t = 0; t <= u.two; ++t) {
+        // keys of the tile's last query
+        const int64_t last = std::min<int64_t>(a + (t + 1) * p->tile_tokens, q_lens[s]) - 1;
+        const int64_t sees = p->causal ? std::min<int64_t>(kv_lens[s], kv_lens[s] - q_lens[s] + last + 1) : kv_lens[s];
+        u.n[t] = sees > 0 ? static_cast<int32_t>((sees + 127) / 128) : 0;
+        p->n_tiles += u.n[t] * bands;
+      }
+      for (int64_t b = 0; b < bands; ++b) {
+        u.head0 = static_cast<int32_t>(b * p->packed);
+        units.push_back(u);
+      }
+    }
+    q0 += q_lens[s];
+    kv0 += kv_lens[s];
+  }
+  // a unit costs its tile steps and about two more for its start and its epilogue
+  auto cost = [](const PromptUnit& u) { return int64_t(u.n[0]) + u.n[1] + 2; };
+  std::stable_sort(units.begin(), units.end(),
+                   [&](const PromptUnit& x, const PromptUnit& y) { return cost(x) > cost(y); });
+  ctas = static_cast<int>(std::min<int64_t>(ctas, static_cast<int64_t>(units.size())));
+  std::priority_queue<std::pair<int64_t, int>, std::vector<std::pair<int64_t, int>>, std::greater<>> least;
+  for (int c = 0; c < ctas; ++c) least.push({0, c});
+  std::vector<std::vector<int32_t>> mine(static_cast<size_t>(std::max(ctas, 1)));
+  for (size_t i = 0; i < units.size(); ++i) {
+    const auto [load, c] = least.top();
+    least.pop();
+    mine[static_cast<size_t>(c)].push_back(static_cast<int32_t>(i));
+    least.push({load + cost(units[i]), c});
+  }
+  p->h_units.reserve(units.size());
+  p->h_cta_begin.assign(1, 0);
+  for (int c = 0; c < ctas; ++c) {
+    for (int32_t i : mine[static_cast<size_t>(c)]) p->h_units.push_back(units[static_cast<size_t>(i)]);
+    p->h_cta_begin.push_back(static_cast<int32_t>(p->h_units.size()));
+  }
+  p->n_units = static_cast<int64_t>(units.size());
+  p->grid = ctas;
+  return BSP_OK;
 }
 
 }  // namespace bsp

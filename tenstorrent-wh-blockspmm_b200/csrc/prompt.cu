@@ -1,50 +1,441 @@
-// Attention over whole prompts, packed sequences of different lengths:
+// Attention over whole prompts on the tcgen05 tensor cores, packed sequences
+// of different lengths, several query heads to a key/value head:
 //   O_i = sum_j softmax_j(scale q_i k_j) v_j,  j <= i + (kv_len - q_len).
-// A warp takes one (query, head) and walks its keys with a running maximum and
-// sum.
+//
+// Rows.  A tile is 128 rows = 128 / P queries x P query heads of one key/value
+// head (P: the largest power of two that divides heads / kv_heads), so that a
+// short sequence still fills a tile and a causal tile wastes little on its
+// diagonal.  One TMA box {64 values, P heads, 128 / P queries} brings it in
+// that order.  A unit is one or two such tiles of consecutive queries; both
+// read the same keys.
+//
+// Steps.  128 keys a step.  Per tile and step
+//   S = Q K^T            128 x 128 x d    fp32 in TMEM
+//   P = exp2(S c - m)    one thread a row; c = scale log2 e; the running maximum
+//                        m moves only when it grows by more than 8 (2^8), and
+//                        only then O and the row sum l are rescaled; P goes back
+//                        to TMEM as bf16 pairs, over S
+//   O += P V             128 x d x 128, A = P read from TMEM
+// and at the end O / l, m ln 2 + ln l.  With two tiles the tensor cores work on
+// one while the softmax of the other runs: the MMA warp issues
+//   S_a(0) S_b(0) | O_a(0) S_a(1) | O_b(0) S_b(1) | O_a(1) S_a(2) | ...
+// S_t(j + 1) is issued behind O_t(j), so P(j) has been read when S(j + 1)
+// overwrites it, and a thread that sees S_t(j) complete knows O_t(j - 1) to be
+// complete and may rescale it.
+//
+// TMEM (512 columns): S_a 0, S_b 128 (P in their first 64), O_a 256, O_b 384.
+// Shared memory: Q of both tiles, then a ring of K and V slots in the order
+// K0 V0 K1 V1 ...
+//
+// Warps (320 threads, one CTA per SM): 0-3 softmax of tile a, 4-7 of tile b
+// (TMEM lane quarter = warp & 3), 8 MMA, 9 TMA.  Every wait is bounded.
 #include <cuda_bf16.h>
 
+#include "bsp_ptx.cuh"
 #include "decoder.h"
 
 namespace bsp {
+using namespace dev;
+
 namespace {
 
+constexpr int kPrThreads = 320;
+constexpr int kPrMmaWarp = 8, kPrTmaWarp = 9;
+constexpr uint32_t kPrAtom = 128 * 128;  // 128 rows x 128 bytes (64 values)
+constexpr float kPrRescale = 8.f;        // log2 of the growth that forces a rescale
+constexpr int kPrMaxSlots = 8;
+
+__host__ __device__ constexpr uint32_t pr_tile(int d) { return 128u * 2u * static_cast<uint32_t>(d); }
+__host__ __device__ constexpr int pr_slots(int d) { return d == 128 ? 5 : 8; }
+
+struct PrHeader {
+  uint64_t q_full, q_empty;
+  uint64_t kv_full[kPrMaxSlots], kv_empty[kPrMaxSlots];
+  uint64_t s_full[2], p_full[2], o_full[2], o_empty[2];
+  uint64_t drain;
+  uint32_t tmem_base;
+  int abort_flag;
+};
+static_assert(sizeof(PrHeader) <= 1024, "header must fit its 1 KiB slot");
+
+__device__ __forceinline__ uint32_t baddr(const uint64_t* b) { return smem_u32(b); }
+
+__device__ __forceinline__ bool wait_all(const uint64_t* bar, uint32_t parity, const WaitCtl& ctl, uint32_t what) {
+  return __all_sync(0xffffffffu, mbar_wait_bounded(baddr(bar), parity, ctl, what));
+}
+
+// A wait for copies or MMAs in flight that does not give up when another role
+// did: shared memory and TMEM may not be left while they are written.
+__device__ __noinline__ bool drain_wait(uint32_t bar, uint32_t parity, const WaitCtl& ctl) {
+  int zero = 0;
+  WaitCtl c2{&zero, ctl.status, ctl.timeout_ns};
+  return mbar_wait_bounded(bar, parity, c2, ST_TIMEOUT_DRAIN);
+}
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
 template <int kD>
-__global__ void __launch_bounds__(128) prompt_kernel(const PromptParams p) {
-  constexpr int kPer = kD / 32;
-  const int token = blockIdx.x * 4 + (threadIdx.x >> 5), head = blockIdx.y, lane = threadIdx.x & 31;
-  if (token >= p.tokens) return;
-  int s = 0;
-  while (s + 1 < p.n_seqs && p.seqs[s + 1].q0 <= token) ++s;
-  const PromptSeq sq = p.seqs[s];
-  const int kh = head / (p.heads / p.kv_heads);
-  const int n = p.causal ? min(sq.kv_len, max(0, token - sq.q0 + sq.kv_len - sq.q_len + 1)) : sq.kv_len;
-  const __nv_bfloat16* q = static_cast<const __nv_bfloat16*>(p.q.p) + token * p.q.token + head * p.q.head;
-  const __nv_bfloat16* kp = static_cast<const __nv_bfloat16*>(p.k.p) + sq.kv0 * p.k.token + kh * p.k.head;
-  const __nv_bfloat16* vp = static_cast<const __nv_bfloat16*>(p.v.p) + sq.kv0 * p.v.token + kh * p.v.head;
-  float qr[kPer], acc[kPer], m = -INFINITY, l = 0.f;
-  for (int i = 0; i < kPer; ++i) qr[i] = __bfloat162float(q[lane * kPer + i]), acc[i] = 0.f;
-  for (int j = 0; j < n; ++j) {
-    float x = 0.f;
-    for (int i = 0; i < kPer; ++i) x += qr[i] * __bfloat162float(kp[j * p.k.token + lane * kPer + i]);
-    for (int k = 16; k; k >>= 1) x += __shfl_xor_sync(0xFFFFFFFFu, x, k);
-    x *= p.scale;
-    const float mn = fmaxf(m, x), c = m == mn ? 1.f : expf(m - mn), w = expf(x - mn);
-    l = l * c + w;
-    for (int i = 0; i < kPer; ++i) acc[i] = acc[i] * c + w * __bfloat162float(vp[j * p.v.token + lane * kPer + i]);
-    m = mn;
+__device__ __forceinline__ void pr_tma(const PromptParams& p, PrHeader* hdr, uint32_t q_smem, uint32_t ring, int u0,
+                                      int u1, const WaitCtl& ctl, int lane) {
+  constexpr int kHalves = kD / 64, kSlots = pr_slots(kD);
+  constexpr uint32_t kTile = pr_tile(kD);
+  int64_t slot_n = 0;
+  int units = 0;
+  uint32_t armed = 0, armed_parity = 0;
+  bool q_armed = false, ok = true;
+  auto load = [&](const CUtensorMap* tm, int kvh, int token) -> bool {
+    const int sl = static_cast<int>(slot_n % kSlots);
+    const uint32_t ph = static_cast<uint32_t>((slot_n / kSlots) & 1);
+    ++slot_n;
+    if (!wait_all(&hdr->kv_empty[sl], ph ^ 1u, ctl, ST_TIMEOUT_PRODUCER)) return false;
+    const uint32_t bar = baddr(&hdr->kv_full[sl]);
+    mbar_arrive_expect_tx_pred(bar, kTile, lane == 0);
+    tma_load_3d_pred(ring + sl * kTile + lane * kPrAtom, tm, 64 * lane, kvh, token, bar, lane < kHalves);
+    armed |= 1u << sl;
+    armed_parity = (armed_parity & ~(1u << sl)) | (ph << sl);
+    return true;
+  };
+#pragma unroll 1
+  for (int u = u0; u < u1 && ok; ++u) {
+    const PromptUnit un = p.units[u];
+    const int n = max(un.n[0], un.n[1]);
+    if (n == 0) continue;
+    ok = wait_all(&hdr->q_empty, (units & 1) ^ 1u, ctl, ST_TIMEOUT_PRODUCER);
+    if (!ok) break;
+    ++units;
+    q_armed = true;
+    const int tiles = un.n[1] > 0 ? 2 : 1;
+    mbar_arrive_expect_tx_pred(baddr(&hdr->q_full), tiles * kTile, lane == 0);
+    tma_load_3d_pred(q_smem + lane * kPrAtom, &p.tm_q, 64 * (lane % kHalves), un.head0,
+                     un.q0 + (lane / kHalves) * p.tile_tokens, baddr(&hdr->q_full), lane < tiles * kHalves);
+    const int kvh = un.head0 / p.group;
+#pragma unroll 1
+    for (int j = 0; j < n && ok; ++j) {
+      ok = load(&p.tm_k, kvh, un.kv0 + 128 * j);
+      if (ok) ok = load(&p.tm_v, kvh, un.kv0 + 128 * j);
+    }
   }
-  __nv_bfloat16* o = static_cast<__nv_bfloat16*>(p.o.p) + token * p.o.token + head * p.o.head;
-  for (int i = 0; i < kPer; ++i) o[lane * kPer + i] = __float2bfloat16(n == 0 ? 0.f : acc[i] / l);
-  if (lane == 0 && p.lse) p.lse[static_cast<int64_t>(token) * p.heads + head] = m + logf(l);
+  if (lane == 0) {
+    if (q_armed) drain_wait(baddr(&hdr->q_full), (units - 1) & 1, ctl);
+    for (int s = 0; s < kSlots; ++s)
+      if (armed & (1u << s)) drain_wait(baddr(&hdr->kv_full[s]), (armed_parity >> s) & 1u, ctl);
+  }
+  __syncwarp();
+}
+
+template <int kD>
+__device__ __forceinline__ void pr_mma(const PromptParams& p, PrHeader* hdr, uint8_t* ring_ptr, uint32_t q_smem,
+                                      uint32_t ring, uint32_t tmem, int u0, int u1, const WaitCtl& ctl, int lane) {
+  constexpr int kSlots = pr_slots(kD);
+  constexpr uint32_t kTile = pr_tile(kD), kAtom16 = kPrAtom >> 4;
+  const uint32_t is0 = lane == 0 ? 1u : 0u;
+  const uint32_t idesc_s = idesc_bf16_f32(128, 128, 0, 0), idesc_o = idesc_bf16_f32(128, kD, 0, 1);
+  const uint64_t qd = smem_desc(q_smem, 16u, 1024u, 2u);
+  const uint64_t kd = smem_desc(ring, 16u, 1024u, 2u);
+  const uint64_t vd = smem_desc(ring, kPrAtom, 1024u, 2u);  // MN-major: LBO = next 64 columns of d
+  int64_t slot_n = 0;  // ring position of K0 of the unit
+  uint32_t units = 0, steps[2] = {0, 0}, outs[2] = {0, 0};
+  bool ok = true;
+  auto full = [&](int64_t k) {
+    return wait_all(&hdr->kv_full[k % kSlots], static_cast<uint32_t>((k / kSlots) & 1), ctl, ST_TIMEOUT_MMA);
+  };
+  auto scores = [&](int t, int64_t k) {
+    const uint64_t a = qd + t * (kTile >> 4), b = kd + (k % kSlots) * (kTile >> 4);
+#pragma unroll
+    for (int i = 0; i < kD / 16; ++i)
+      mma_bf16_pred(tmem + 128u * t, a + (i >> 2) * kAtom16 + (i & 3) * 2u, b + (i >> 2) * kAtom16 + (i & 3) * 2u,
+                    idesc_s, i > 0, is0);
+    mma_commit_pred(baddr(&hdr->s_full[t]), is0);
+  };
+#pragma unroll 1
+  for (int u = u0; u < u1 && ok; ++u) {
+    const PromptUnit un = p.units[u];
+    const int n = max(un.n[0], un.n[1]);
+    if (n == 0) continue;
+    ok = wait_all(&hdr->q_full, units & 1, ctl, ST_TIMEOUT_MMA) && full(slot_n);
+    if (!ok) break;
+    ++units;
+    tc_fence_after();
+    for (int t = 0; t < 2; ++t)
+      if (un.n[t] > 0) scores(t, slot_n);
+    mma_commit_pred(baddr(&hdr->kv_empty[slot_n % kSlots]), is0);
+    if (n == 1) mma_commit_pred(baddr(&hdr->q_empty), is0);
+#pragma unroll 1
+    for (int j = 0; j < n && ok; ++j) {
+      const int64_t kv = slot_n + 2 * j + 1, kn = slot_n + 2 * j + 2;
+      ok = full(kv);
+      if (!ok) break;
+      // Rows of V behind the sequence's end belong to its neighbour; their
+      // weight is 0, but 0 times an infinity or NaN there is not: clear them.
+      const int rows = un.kv_len - 128 * j;
+      if (rows < 128) {
+        uint8_t* v = ring_ptr + (kv % kSlots) * kTile;
+        for (int i = rows * 8 + lane; i < 128 * 8; i += 32)
+          for (int h = 0; h < kD / 64; ++h)
+            *reinterpret_cast<uint4*>(v + h * kPrAtom + i * 16) = make_uint4(0, 0, 0, 0);
+        fence_proxy_async_smem();
+        __syncwarp();
+      }
+      const int last = j < un.n[1] ? 1 : 0;        // last tile that uses V of this step
+      const int last_next = j + 1 < un.n[1] ? 1 : 0;
+      if (j + 1 < n) ok = full(kn);
+      for (int t = 0; t < 2 && ok; ++t) {
+        if (j >= un.n[t]) continue;
+        if (j == 0) {
+          ok = wait_all(&hdr->o_empty[t], (outs[t] & 1) ^ 1u, ctl, ST_TIMEOUT_MMA);
+          ++outs[t];
+        }
+        ok = ok && wait_all(&hdr->p_full[t], steps[t] & 1, ctl, ST_TIMEOUT_MMA);
+        if (!ok) break;
+        ++steps[t];
+        tc_fence_after();
+        const uint64_t b = vd + (kv % kSlots) * (kTile >> 4);
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          mma_bf16_ts_pred(tmem + 256u + 128u * t, tmem + 128u * t + 8u * i, b + i * 128u, idesc_o, j > 0 || i > 0, is0);
+        if (j == un.n[t] - 1) mma_commit_pred(baddr(&hdr->o_full[t]), is0);
+        if (t == last) mma_commit_pred(baddr(&hdr->kv_empty[kv % kSlots]), is0);
+        if (j + 1 < un.n[t]) {
+          scores(t, kn);
+          if (t == last_next) {
+            mma_commit_pred(baddr(&hdr->kv_empty[kn % kSlots]), is0);
+            if (j + 2 == n) mma_commit_pred(baddr(&hdr->q_empty), is0);
+          }
+        }
+      }
+    }
+    slot_n += 2 * n;
+  }
+  if (lane == 0) {
+    mma_commit(baddr(&hdr->drain));
+    drain_wait(baddr(&hdr->drain), 0, ctl);
+  }
+  __syncwarp();
+}
+
+// Store 32 bytes of a row.
+__device__ __forceinline__ void store32(uint16_t* dst, const uint32_t (&o)[32], int at, float f) {
+  uint32_t w[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+    w[i] = pack2(__uint_as_float(o[at + 2 * i]) * f, __uint_as_float(o[at + 2 * i + 1]) * f);
+  *reinterpret_cast<uint4*>(dst) = make_uint4(w[0], w[1], w[2], w[3]);
+  *reinterpret_cast<uint4*>(dst + 8) = make_uint4(w[4], w[5], w[6], w[7]);
+}
+
+template <int kD>
+__device__ __forceinline__ void pr_softmax(const PromptParams& p, PrHeader* hdr, uint32_t tmem, int u0, int u1,
+                                          const WaitCtl& ctl, int warp, int lane) {
+  const int t = warp >> 2, row = 32 * (warp & 3) + lane;
+  const uint32_t lanes = tmem + (static_cast<uint32_t>(32 * (warp & 3)) << 16);
+  const uint32_t t_s = lanes + 128u * t, t_o = lanes + 256u + 128u * t;
+  const int dt = t * p.tile_tokens + row / p.packed, dh = row % p.packed;
+  uint32_t steps = 0, outs = 0;
+#pragma unroll 1
+  for (int u = u0; u < u1; ++u) {
+    const PromptUnit un = p.units[u];
+    const int n = un.n[t];
+    const int64_t token = static_cast<int64_t>(un.q0) + dt;
+    const bool valid = token < un.q_end && (t == 0 || un.two);
+    uint16_t* orow = static_cast<uint16_t*>(p.o.p) + token * p.o.token + (un.head0 + dh) * p.o.head;
+    float* lrow = p.lse ? p.lse + token * p.heads + un.head0 + dh : nullptr;
+    if (n == 0) {
+      if (valid) {
+        for (int c = 0; c < kD / 8; ++c) reinterpret_cast<uint4*>(orow)[c] = make_uint4(0, 0, 0, 0);
+        if (lrow) *lrow = -INFINITY;
+      }
+      continue;
+    }
+    const int sees = p.causal ? min(un.kv_len, un.sees + dt) : un.kv_len;  // keys this row attends to
+    float m = -INFINITY, l = 0.f;
+#pragma unroll 1
+    for (int j = 0; j < n; ++j) {
+      if (!wait_all(&hdr->s_full[t], steps & 1, ctl, ST_TIMEOUT_EPILOGUE)) return;
+      ++steps;
+      tc_fence_after();
+      uint32_t v[4][32];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) tmem_ld_32x32b_x32(t_s + 32u * c, v[c]);
+      tmem_ld_wait();
+      const int limit = sees - 128 * j;
+      if (__any_sync(0xffffffffu, limit < 128)) {
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+#pragma unroll
+          for (int i = 0; i < 32; ++i)
+            if (32 * c + i >= limit) v[c][i] = 0xFF800000u;
+      }
+      float x0 = -INFINITY, x1 = -INFINITY, x2 = -INFINITY, x3 = -INFINITY;
+#pragma unroll
+      for (int i = 0; i < 32; ++i) {
+        x0 = fmaxf(x0, __uint_as_float(v[0][i]));
+        x1 = fmaxf(x1, __uint_as_float(v[1][i]));
+        x2 = fmaxf(x2, __uint_as_float(v[2][i]));
+        x3 = fmaxf(x3, __uint_as_float(v[3][i]));
+      }
+      const float mx = fmaxf(fmaxf(x0, x1), fmaxf(x2, x3)) * p.scale_log2;
+      const bool need = mx > m + kPrRescale;
+      if (__any_sync(0xffffffffu, need)) {
+        const float mn = need ? mx : m;
+        const float alpha = need ? (m == -INFINITY ? 0.f : ex2(m - mn)) : 1.f;
+        if (j > 0) {
+#pragma unroll 1
+          for (int c = 0; c < kD / 32; ++c) {
+            uint32_t o[32];
+            tmem_ld_32x32b_x32(t_o + 32u * c, o);
+            tmem_ld_wait();
+#pragma unroll
+            for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+            tmem_st_32x32b_x32(t_o + 32u * c, o);
+          }
+        }
+        l *= alpha;
+        m = mn;
+      }
+      // Exponents S c - m in one fused step.  For |m| above 2^24 the rounding of
+      // m itself would show in them: there the product is rounded like m first.
+      float c = p.scale_log2, mm = m == -INFINITY ? 0.f : m;
+      if (__any_sync(0xffffffffu, fabsf(mm) > 16777216.f)) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+#pragma unroll
+          for (int i = 0; i < 32; ++i)
+            v[k][i] = __float_as_uint(__fsub_rn(__fmul_rn(__uint_as_float(v[k][i]), c), mm));
+        c = 1.f;
+        mm = 0.f;
+      }
+      float l0 = 0.f, l1 = 0.f;
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        uint32_t w[32];
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {
+          const float a = ex2(fmaf(__uint_as_float(v[2 * k + i / 16][2 * (i % 16)]), c, -mm));
+          const float b = ex2(fmaf(__uint_as_float(v[2 * k + i / 16][2 * (i % 16) + 1]), c, -mm));
+          l0 += a;
+          l1 += b;
+          w[i] = pack2(a, b);
+        }
+        tmem_st_32x32b_x32(t_s + 32u * k, w);
+      }
+      l += l0 + l1;
+      tmem_st_wait();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(baddr(&hdr->p_full[t]));
+    }
+    if (!wait_all(&hdr->o_full[t], outs & 1, ctl, ST_TIMEOUT_EPILOGUE)) return;
+    ++outs;
+    tc_fence_after();
+    const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);  // a NaN sum stays one
+#pragma unroll 1
+    for (int c = 0; c < kD / 32; ++c) {
+      uint32_t o[32];
+      tmem_ld_32x32b_x32(t_o + 32u * c, o);
+      tmem_ld_wait();
+      if (valid) {
+        store32(orow + 32 * c, o, 0, inv);
+        store32(orow + 32 * c + 16, o, 16, inv);
+      }
+    }
+    if (valid && lrow) *lrow = l == 0.f ? -INFINITY : m * 0.6931471805599453f + logf(l);
+    tc_fence_before();
+    __syncwarp();
+    if (lane == 0) mbar_arrive(baddr(&hdr->o_empty[t]));
+  }
+}
+
+template <int kD>
+__global__ void __launch_bounds__(kPrThreads, 1) prompt_tcgen05(const __grid_constant__ PromptParams p) {
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  const uint32_t raw = smem_u32(smem_raw);
+  const uint32_t base = (raw + 1023u) & ~1023u;
+  uint8_t* gbase = smem_raw + (base - raw);
+  PrHeader* hdr = reinterpret_cast<PrHeader*>(gbase);
+  const uint32_t q_smem = base + 1024u, ring = q_smem + 2u * pr_tile(kD);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int u0 = p.cta_begin[blockIdx.x], u1 = p.cta_begin[blockIdx.x + 1];
+  if (threadIdx.x == 0) {
+    mbar_init(baddr(&hdr->q_full), 1);
+    mbar_init(baddr(&hdr->q_empty), 1);
+    for (int s = 0; s < pr_slots(kD); ++s) {
+      mbar_init(baddr(&hdr->kv_full[s]), 1);
+      mbar_init(baddr(&hdr->kv_empty[s]), 1);
+    }
+    for (int t = 0; t < 2; ++t) {
+      mbar_init(baddr(&hdr->s_full[t]), 1);
+      mbar_init(baddr(&hdr->p_full[t]), 4);
+      mbar_init(baddr(&hdr->o_full[t]), 1);
+      mbar_init(baddr(&hdr->o_empty[t]), 4);
+    }
+    mbar_init(baddr(&hdr->drain), 1);
+    hdr->abort_flag = 0;
+    fence_mbar_init();
+    tma_prefetch_desc(&p.tm_q);
+    tma_prefetch_desc(&p.tm_k);
+    tma_prefetch_desc(&p.tm_v);
+  }
+  if (warp == kPrMmaWarp) {
+    tmem_alloc(smem_u32(&hdr->tmem_base), 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = hdr->tmem_base;
+  const WaitCtl ctl{&hdr->abort_flag, p.status, p.timeout_ns};
+  if (warp == kPrMmaWarp)
+    pr_mma<kD>(p, hdr, gbase + 1024 + 2 * pr_tile(kD), q_smem, ring, tmem, u0, u1, ctl, lane);
+  else if (warp == kPrTmaWarp)
+    pr_tma<kD>(p, hdr, q_smem, ring, u0, u1, ctl, lane);
+  else
+    pr_softmax<kD>(p, hdr, tmem, u0, u1, ctl, warp, lane);
+  tc_fence_before();
+  __syncthreads();
+  if (warp == kPrMmaWarp) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+// Tensor map of a [tokens][heads][d] operand, box {64, box_heads, box_tokens}.
+// A dimension of one entry is never stepped over: its stride is any valid one.
+bsp_status encode_heads(bsp_device* dev, CUtensorMap* tm, const HeadsView& x, int64_t tokens, int heads, int d,
+                        uint32_t box_heads, uint32_t box_tokens) {
+  const uint64_t dims[3] = {static_cast<uint64_t>(d), static_cast<uint64_t>(heads), static_cast<uint64_t>(tokens)};
+  const uint64_t strides[2] = {static_cast<uint64_t>(heads > 1 ? x.head : d) * 2,
+                               static_cast<uint64_t>(tokens > 1 ? x.token : static_cast<int64_t>(heads) * d) * 2};
+  const uint32_t box[3] = {64, box_heads, box_tokens};
+  return encode_nd(dev, tm, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, x.p, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
 }  // namespace
 
-bsp_status launch_prompt(const bsp_prompt_plan* plan, const PromptParams& p, cudaStream_t stream) {
-  const dim3 grid((p.tokens + 3) / 4, p.heads);
-  if (plan->d == 64) prompt_kernel<64><<<grid, 128, 0, stream>>>(p);
-  else prompt_kernel<128><<<grid, 128, 0, stream>>>(p);
+int prompt_smem_bytes(int d) { return static_cast<int>(2048u + (2u + pr_slots(d)) * pr_tile(d)); }
+
+bsp_status launch_prompt(const bsp_prompt_plan* plan, PromptParams& p, cudaStream_t stream) {
+  bsp_device* dev = plan->dev;
+  bsp_status st = encode_heads(dev, &p.tm_q, p.q, plan->q_tokens, plan->heads, plan->d, plan->packed,
+                               plan->tile_tokens);
+  p.tm_k = p.tm_v = p.tm_q;  // without any key nothing loads through these
+  if (st == BSP_OK && plan->kv_tokens > 0) {
+    st = encode_heads(dev, &p.tm_k, p.k, plan->kv_tokens, plan->kv_heads, plan->d, 1, 128);
+    if (st == BSP_OK) st = encode_heads(dev, &p.tm_v, p.v, plan->kv_tokens, plan->kv_heads, plan->d, 1, 128);
+  }
+  if (st != BSP_OK) return st;
+  const auto kernel = plan->d == 64 ? prompt_tcgen05<64> : prompt_tcgen05<128>;
+  st = cuda_check(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, plan->smem_bytes),
+                  "cudaFuncSetAttribute(prompt)");
+  if (st != BSP_OK) return st;
+  kernel<<<plan->grid, kPrThreads, plan->smem_bytes, stream>>>(p);
   return cuda_check(cudaGetLastError(), "prompt attention launch");
 }
 
