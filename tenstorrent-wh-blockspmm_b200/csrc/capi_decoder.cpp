@@ -314,7 +314,6 @@ bsp_status bsp_decode_plan_create(bsp_device* dev, int32_t max_seqs, int32_t hea
   if (s != BSP_OK) return s;
   if (page != 16 && page != 32 && page != 64 && page != 128)
     return set_error(BSP_ERR_INVALID_ARG, "a cache page holds 16, 32, 64 or 128 tokens");
-  (void)opts;
   bsp_decode_plan* p = new (std::nothrow) bsp_decode_plan();
   if (!p) return set_error(BSP_ERR_ALLOC, "host allocation failed");
   p->dev = dev;
@@ -323,6 +322,26 @@ bsp_status bsp_decode_plan_create(bsp_device* dev, int32_t max_seqs, int32_t hea
   p->kv_heads = kv_heads;
   p->d = d;
   p->page = page;
+  p->grid = decode_ctas(dev);
+  if (opts && opts->max_ctas > 0) p->grid = std::min(p->grid, opts->max_ctas);
+  p->smem_bytes = decode_smem_bytes(d, heads / kv_heads);
+  p->timeout_ns = static_cast<uint64_t>(opts && opts->timeout_ms > 0 ? opts->timeout_ms : 2000) * 1000000ull;
+  OnDevice on(dev->ordinal);
+  const size_t counters = (sizeof(int32_t) * p->grid + 255) / 256 * 256;
+  p->blob_bytes = counters + sizeof(float) * decode_work_floats(p->grid, d);
+  if (cudaMalloc(&p->d_blob, p->blob_bytes) != cudaSuccess) {
+    delete p;
+    return set_error(BSP_ERR_ALLOC, "cudaMalloc of the decode workspace failed");
+  }
+  p->d_counters = static_cast<int32_t*>(p->d_blob);
+  p->d_work = reinterpret_cast<float*>(static_cast<uint8_t*>(p->d_blob) + counters);
+  s = cuda_check(cudaMemset(p->d_counters, 0, counters), "clear the decode counters");
+  // the clearing ran on the legacy stream: executes may come on any other
+  if (s == BSP_OK) s = cuda_check(cudaStreamSynchronize(nullptr), "clear the decode counters");
+  if (s != BSP_OK) {
+    bsp_decode_plan_destroy(p);
+    return s;
+  }
   *out = p;
   return BSP_OK;
 }
@@ -355,13 +374,24 @@ bsp_status bsp_decode_execute(const bsp_decode_plan* plan, const bsp_kv_cache* c
   p.table_width = table_width;
   p.n_seqs = n_seqs;
   p.heads = plan->heads;
-  p.scale = scale;
+  p.group = plan->heads / plan->kv_heads;
+  p.chunks = (p.group + 15) / 16;
+  p.streams = plan->kv_heads * p.chunks;
+  p.scale_log2 = scale * 1.4426950408889634f;
+  p.work = plan->d_work;
+  p.counters = plan->d_counters;
   p.status = plan->dev->d_status;
+  p.timeout_ns = plan->timeout_ns;
   OnDevice on(plan->dev->ordinal);
   return launch_decode(plan, p, static_cast<cudaStream_t>(stream));
 }
 
 bsp_status bsp_decode_plan_destroy(bsp_decode_plan* plan) {
+  if (!plan) return BSP_OK;
+  if (plan->d_blob) {
+    OnDevice on(plan->dev->ordinal);
+    cudaFree(plan->d_blob);
+  }
   delete plan;
   return BSP_OK;
 }
@@ -370,10 +400,13 @@ bsp_status bsp_decode_plan_info(const bsp_decode_plan* p, int64_t info[16]) {
   if (!p || !info) return set_error(BSP_ERR_INVALID_ARG, "null argument");
   memset(info, 0, sizeof(int64_t) * 16);
   info[0] = p->max_seqs;
+  info[1] = p->grid;
   info[2] = p->heads;
   info[3] = p->kv_heads;
   info[4] = p->d;
   info[5] = p->page;
+  info[8] = static_cast<int64_t>(p->blob_bytes);
+  info[9] = p->smem_bytes;
   return BSP_OK;
 }
 

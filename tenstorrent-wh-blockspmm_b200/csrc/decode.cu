@@ -1,77 +1,613 @@
 // Attention of one token of each sequence over the paged 8-bit cache:
-//   o = sum_t softmax_t(scale q k_t) v_t,  k_t = code * page scale.
-// A block takes one (sequence, query head); each warp walks every fourth token
-// with a running maximum and sum, and the warps' results are joined at the end.
+//   o = sum_t softmax_t(scale q k_t) v_t,  k_t = code * 2^a, v_t = code * 2^b
+// with a and b of the token's page.
+//
+// Memory-bound: 2 d bytes of codes per token and key/value head are read once,
+// for all the query heads that share it.
+//
+// Work.  A row is one sequence x one key/value head x up to 16 of its query
+// heads; a tile is 64 tokens of a row.  The tiles of all rows form one list,
+// and each CTA takes an equal stretch of it, whatever the lengths (read from
+// the device).  A row that crosses a stretch's end is cut: its parts leave
+// (m, l, O) in the workspace, and the CTA that finishes last joins them, in
+// the order of the parts (the result does not depend on who is last).
+//
+// Tile.  K and V codes of 64 tokens come by TMA, one box per page (or 64
+// tokens of it) and operand, swizzled so that ldmatrix reads without bank
+// conflicts.  Each of four warps takes 16 tokens with its own running maximum:
+//   S^T [16 tokens x 8 heads]  = K Q^T    m16n8k16, A = K, B = Q
+//   P'  = 2^(S c + b - m)                 c = scale log2 e 2^a: the value scale
+//                                         2^b goes into the exponent, so codes
+//                                         of V enter the product as they are;
+//                                         l sums P' 2^-b
+//   O^T [d x 8 heads]         += V^T P'   A = V (ldmatrix.trans), B = P'
+// e4m3 codes are exact in fp16.  Q is scaled to [1, 2) by a power of two per
+// head before it is rounded to fp16 (bf16's 8 bits fit; what falls below
+// 2^-14 of the head's largest value loses bits that the sum cannot show).
+// P' <= 2^8 is rounded to fp16 (2^-11); sums are in fp32.
+//
+// Warps (160 threads, two CTAs per SM): 0-3 as above, 4 issues the copies; it
+// holds the page numbers and scales of the next tiles in its lanes, so their
+// loads are off the path.  Every wait is bounded; a CTA that gave up still
+// counts its parts, so the counters stay right for the next launch.
 #include <cuda_bf16.h>
-#include <cuda_fp8.h>
+#include <cuda_fp16.h>
 
+#include "bsp_ptx.cuh"
 #include "decoder.h"
 
 namespace bsp {
+using namespace dev;
+
 namespace {
 
-__device__ __forceinline__ float code_value(uint32_t c) {
-  const __half_raw h = __nv_cvt_fp8_to_halfraw(static_cast<__nv_fp8_storage_t>(c), __NV_E4M3);
-  return __half2float(*reinterpret_cast<const __half*>(&h));
+constexpr int kDcThreads = 160;
+constexpr int kDcTile = 64;          // tokens
+constexpr int kDcTmaWarp = 4;
+constexpr int kDcMaxStages = 12;
+constexpr float kDcRescale = 8.f;    // log2 of the growth that moves the maximum
+
+struct DcHeader {
+  uint64_t full[kDcMaxStages], empty[kDcMaxStages];
+  int64_t tiles, base;  // tiles of all rows; first tile of sequence `seq`
+  int32_t seq;
+  int32_t ctas;         // CTAs that take part
+  int32_t last;         // this CTA joins the row
+  int abort_flag;
+  float scales[kDcMaxStages][8];  // per stage: 2^a of four slices of 16 tokens, then 2^b
+};
+static_assert(sizeof(DcHeader) <= 1024, "header must fit its 1 KiB slot");
+
+// Shared memory from the 1 KiB-aligned base: header, stages (K then V), then
+// the warps' results: O [4][heads][d], m [4][heads], l [4][heads].
+// As many stages as let two CTAs share an SM's 228 KB (1 KB of each is the
+// system's).
+__host__ __device__ constexpr int dc_stage_bytes(int d) { return 2 * kDcTile * d; }
+__host__ __device__ constexpr int dc_result_bytes(int d, int heads) { return 16 * heads * (d + 2); }
+__host__ __device__ constexpr int dc_stages(int d, int heads) {
+  const int n = (113 * 1024 - 2048 - dc_result_bytes(d, heads)) / dc_stage_bytes(d);
+  return n < kDcMaxStages ? n : kDcMaxStages;
+}
+__host__ __device__ constexpr int dc_smem(int d, int heads) {
+  return 2048 + dc_stages(d, heads) * dc_stage_bytes(d) + dc_result_bytes(d, heads);
 }
 
-template <int kD>
-__global__ void __launch_bounds__(128) decode_kernel(const DecodeParams p) {
-  constexpr int kPer = kD / 32;
-  const int seq = blockIdx.x, head = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int hk = p.cache.kv_heads, kh = head / (p.heads / hk), page = p.cache.page;
-  int64_t len = __ldg(p.lens + seq);
-  if (len < 0 || len > p.table_width * page) {
-    if (threadIdx.x == 0) atomicOr(p.status, ST_BAD_INDEX);
-    len = 0;
+__device__ __forceinline__ uint32_t baddr(const uint64_t* b) { return smem_u32(b); }
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ void ldmatrix4(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+__device__ __forceinline__ void ldmatrix4t(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+// two e4m3 codes (16 bits) to two fp16, exactly
+__device__ __forceinline__ void codes_to_half(uint32_t w, uint32_t& lo, uint32_t& hi) {
+  asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\t"
+      "cvt.rn.f16x2.e4m3x2 %0, a;\n\tcvt.rn.f16x2.e4m3x2 %1, b;\n\t}"
+      : "=r"(lo), "=r"(hi)
+      : "r"(w));
+}
+__device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                         uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// transpose of an 8 x 8 matrix of 16-bit values held by the warp
+__device__ __forceinline__ uint32_t transpose8(uint32_t v) {
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
+}
+__device__ __forceinline__ uint32_t half_pair(float a, float b) {
+  const __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ uint32_t bf16_two(float a, float b) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ void consumers_sync() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
+
+__device__ __forceinline__ void tma_load_4d_pred(uint32_t smem_dst, const void* tmap, int32_t x, int32_t y, int32_t z,
+                                                 int32_t w, uint32_t bar, uint32_t issue) {
+  asm volatile(
+      "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %7, 0;\n\t"
+      "@q cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%2, %3, %4, %5}], [%6];\n\t}" ::"r"(smem_dst),
+      "l"(reinterpret_cast<uint64_t>(tmap)), "r"(x), "r"(y), "r"(z), "r"(w), "r"(bar), "r"(issue)
+      : "memory");
+}
+
+// Tokens of sequence s that count: 0 where the length is not one that the page
+// table holds.
+__device__ __forceinline__ int dc_len(const DecodeParams& p, int s) {
+  const int len = __ldg(p.lens + s);
+  return len < 0 || len > p.table_width * p.cache.page ? 0 : len;
+}
+__device__ __forceinline__ int dc_tiles(const DecodeParams& p, int s) { return (dc_len(p, s) + kDcTile - 1) / kDcTile; }
+
+// A CTA's way through its stretch [g, g1) of the list of tiles.
+struct Walk {
+  int64_t g, g1, base;
+  int seq, tiles;  // of the current sequence
+};
+struct Piece {
+  int seq, stream, tile0, n, tiles;  // tiles [tile0, tile0 + n) of the row's `tiles`
+  int64_t row0;                      // the row's first tile in the list
+};
+__device__ __forceinline__ bool next_piece(const DecodeParams& p, Walk& w, Piece& pc) {
+  if (w.g >= w.g1) return false;
+  while (w.g >= w.base + static_cast<int64_t>(w.tiles) * p.streams) {
+    w.base += static_cast<int64_t>(w.tiles) * p.streams;
+    if (++w.seq >= p.n_seqs) return false;
+    w.tiles = dc_tiles(p, w.seq);
   }
-  const __nv_bfloat16* q = static_cast<const __nv_bfloat16*>(p.q.p) + seq * p.q.token + head * p.q.head;
-  float qr[kPer], acc[kPer], m = -INFINITY, l = 0.f;
-  for (int i = 0; i < kPer; ++i) qr[i] = __bfloat162float(q[lane * kPer + i]), acc[i] = 0.f;
-  for (int64_t t = warp; t < len; t += 4) {
-    const int32_t id = __ldg(p.page_table + seq * p.table_stride + t / page);
-    if (id < 0 || id >= p.cache.n_pages) {
-      if (lane == 0) atomicOr(p.status, ST_BAD_INDEX);
-      continue;
+  const int64_t rel = w.g - w.base;
+  pc.seq = w.seq;
+  pc.tiles = w.tiles;
+  pc.stream = static_cast<int>(rel / w.tiles);
+  pc.tile0 = static_cast<int>(rel - static_cast<int64_t>(pc.stream) * w.tiles);
+  pc.n = static_cast<int>(min(static_cast<int64_t>(w.tiles - pc.tile0), w.g1 - w.g));
+  pc.row0 = w.base + static_cast<int64_t>(pc.stream) * w.tiles;
+  w.g += pc.n;
+  return true;
+}
+
+template <int kD, int kStages>
+__device__ __forceinline__ void dc_produce(const DecodeParams& p, DcHeader* hdr, uint32_t ring, Walk w,
+                                          const WaitCtl& ctl, int lane) {
+  constexpr uint32_t kHalf = kDcTile * kD;
+  const int page = p.cache.page, shift = __ffs(page) - 1;  // a power of two
+  const int box = min(page, kDcTile), boxes = kDcTile / box;  // per tile and operand
+  const int kind = lane >> 4, at = (lane & 15) / boxes, sub = (lane & 15) % boxes;
+  const int per_batch = 16 / boxes;
+  const float* scale = kind ? p.cache.v_scale : p.cache.k_scale;
+  const CUtensorMap* tm = kind ? &p.tm_v : &p.tm_k;
+  int64_t it = 0;
+  uint32_t armed = 0, armed_parity = 0;
+  bool ok = true;
+  Piece pc;
+  while (ok && next_piece(p, w, pc)) {
+    const int len = dc_len(p, pc.seq), kvh = pc.stream / p.chunks;
+    const int32_t* pages = p.page_table + pc.seq * p.table_stride;
+    // lane's box of the batch that starts at tile b: its page and scale
+    auto page_of = [&](int b) -> int32_t {
+      const int64_t token = static_cast<int64_t>(pc.tile0 + b + at) * kDcTile + sub * box;
+      return b + at < pc.n && token < len ? __ldg(pages + (token >> shift)) : -2;  // -2: no box
+    };
+    auto checked = [&](int32_t id) -> int32_t {
+      if (id == -2 || (id >= 0 && id < p.cache.n_pages)) return id;
+      atomicOr(p.status, ST_BAD_INDEX);
+      return -1;  // read as zeros
+    };
+    auto scale_of = [&](int32_t id) {
+      return id >= 0 ? __ldg(scale + static_cast<int64_t>(id) * p.cache.kv_heads + kvh) : 1.f;
+    };
+    int32_t id = checked(page_of(0)), id_next = page_of(per_batch);
+    float sc = scale_of(id);
+#pragma unroll 1
+    for (int b = 0; b < pc.n && ok; b += per_batch) {
+      const int32_t idn = checked(id_next);
+      id_next = page_of(b + 2 * per_batch);
+      const float sc_next = scale_of(idn);
+      const int n = min(per_batch, pc.n - b);
+#pragma unroll 1
+      for (int k = 0; k < n; ++k, ++it) {
+        const int st = static_cast<int>(it % kStages);
+        const uint32_t ph = static_cast<uint32_t>((it / kStages) & 1);
+        ok = __all_sync(0xffffffffu, mbar_wait_bounded(baddr(&hdr->empty[st]), ph ^ 1u, ctl, ST_TIMEOUT_PRODUCER));
+        if (!ok) break;
+        const bool mine = at == k && id != -2;
+        if (at == k)
+          for (int i = 0; i < 4 / boxes; ++i) hdr->scales[st][4 * kind + sub * (4 / boxes) + i] = sc;
+        const uint32_t bytes = static_cast<uint32_t>(__popc(__ballot_sync(0xffffffffu, mine))) * box * kD;
+        __syncwarp();  // the scales are written before lane 0 arrives
+        const uint32_t bar = baddr(&hdr->full[st]);
+        mbar_arrive_expect_tx_pred(bar, bytes, lane == 0);
+        const int in_page = ((pc.tile0 + b + k) * kDcTile) & (page - 1);
+        tma_load_4d_pred(ring + st * dc_stage_bytes(kD) + kind * kHalf + sub * box * kD, tm, 0,
+                         in_page, kvh, id >= 0 ? id : static_cast<int32_t>(p.cache.n_pages),
+                         bar, mine);
+        armed |= 1u << st;
+        armed_parity = (armed_parity & ~(1u << st)) | (ph << st);
+      }
+      id = idn;
+      sc = sc_next;
     }
-    const int64_t at = id * p.cache.page_stride + kh * p.cache.head_stride + (t % page) * kD + lane * kPer;
-    const float ks = p.cache.k_scale[static_cast<int64_t>(id) * hk + kh];
-    const float vs = p.cache.v_scale[static_cast<int64_t>(id) * hk + kh];
-    float s = 0.f;
-    for (int i = 0; i < kPer; ++i) s += qr[i] * code_value(static_cast<const uint8_t*>(p.cache.k)[at + i]);
-    for (int k = 16; k; k >>= 1) s += __shfl_xor_sync(0xFFFFFFFFu, s, k);
-    s *= ks * p.scale;
-    const float mn = fmaxf(m, s), c = m == mn ? 1.f : expf(m - mn), w = expf(s - mn);
-    l = l * c + w;
-    for (int i = 0; i < kPer; ++i)
-      acc[i] = acc[i] * c + w * vs * code_value(static_cast<const uint8_t*>(p.cache.v)[at + i]);
-    m = mn;
   }
-  __shared__ float sm[4], sl[4], so[4][kD];
-  for (int i = 0; i < kPer; ++i) so[warp][lane * kPer + i] = acc[i];
-  if (lane == 0) sm[warp] = m, sl[warp] = l;
+  if (lane == 0) {  // no copy may be in flight when the CTA leaves
+    int zero = 0;
+    const WaitCtl c2{&zero, ctl.status, ctl.timeout_ns};
+    for (int s = 0; s < kStages; ++s)
+      if (armed & (1u << s)) mbar_wait_bounded(baddr(&hdr->full[s]), (armed_parity >> s) & 1u, c2, ST_TIMEOUT_DRAIN);
+  }
+  __syncwarp();
+}
+
+template <int kD, int kNt>
+__device__ __forceinline__ void dc_consume(const DecodeParams& p, DcHeader* hdr, uint32_t ring, float* red, Walk w,
+                                          const WaitCtl& ctl, int warp, int lane) {
+  constexpr int kChunks = kD / 16, kHeads = 8 * kNt, kStages = dc_stages(kD, kHeads);
+  constexpr uint32_t kHalf = kDcTile * kD;
+  const int g = lane >> 2, t = lane & 3;
+  // ldmatrix addresses inside a 16-token slice: lane's row and 16-byte chunk.
+  // K: matrices (tokens 0-7, 8-15) x (chunk c, c + 1); V the same.
+  const int row = (lane & 7) + ((lane >> 3) & 1) * 8, cadd = lane >> 4;
+  const int srow = 16 * warp + row;
+  const int swz = kD == 128 ? (srow & 7) : ((srow >> 1) & 3);
+  const uint32_t row_at = static_cast<uint32_t>(srow) * kD;
+  float* red_o = red;                            // [4][kHeads][kD]
+  float* red_m = red + 4 * kHeads * kD;          // [4][kHeads]
+  float* red_l = red_m + 4 * kHeads;
+  int64_t it = 0;
+  bool ok = true;
+  Piece pc;
+  while (next_piece(p, w, pc)) {
+    const int len = dc_len(p, pc.seq);
+    const int kvh = pc.stream / p.chunks, h0 = kvh * p.group + (pc.stream % p.chunks) * 16;
+    const int nh = min(16, p.group - (pc.stream % p.chunks) * 16);
+    uint32_t q[kNt][kChunks][2];
+    float qs[kNt][2];  // scale log2 e times the power of two taken out of q, of heads 2 t, 2 t + 1
+#pragma unroll
+    for (int n = 0; n < kNt; ++n) {
+      float v[kChunks][4], top = 0.f;
+      const bool have = 8 * n + g < nh;
+      const uint16_t* src = static_cast<const uint16_t*>(p.q.p) + pc.seq * p.q.token + (h0 + 8 * n + g) * p.q.head;
+#pragma unroll
+      for (int c = 0; c < kChunks; ++c) {
+        const uint2 x = have ? *reinterpret_cast<const uint2*>(src + 16 * c + 4 * t) : make_uint2(0, 0);
+        v[c][0] = __uint_as_float(x.x << 16);
+        v[c][1] = __uint_as_float(x.x & 0xFFFF0000u);
+        v[c][2] = __uint_as_float(x.y << 16);
+        v[c][3] = __uint_as_float(x.y & 0xFFFF0000u);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) top = fmaxf(top, fabsf(v[c][i]));
+      }
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      // 2^e with e the exponent of the largest value, kept where 2^-e is a normal number
+      const uint32_t e = min(max(__float_as_uint(top) >> 23, 1u), 253u);
+      const float down = __uint_as_float((254u - e) << 23), up = __uint_as_float(e << 23);
+#pragma unroll
+      for (int c = 0; c < kChunks; ++c) {
+        q[n][c][0] = half_pair(v[c][0] * down, v[c][1] * down);
+        q[n][c][1] = half_pair(v[c][2] * down, v[c][3] * down);
+      }
+      // head g's factor sits in the lanes 4 g ..; this lane needs heads 2 t, 2 t + 1
+      qs[n][0] = __shfl_sync(0xffffffffu, up, 8 * t) * p.scale_log2;
+      qs[n][1] = __shfl_sync(0xffffffffu, up, 8 * t + 4) * p.scale_log2;
+    }
+    float o[kNt][kChunks][4], m[kNt][2], l[kNt][2];
+#pragma unroll
+    for (int n = 0; n < kNt; ++n) {
+      m[n][0] = m[n][1] = -INFINITY;
+      l[n][0] = l[n][1] = 0.f;
+#pragma unroll
+      for (int c = 0; c < kChunks; ++c) o[n][c][0] = o[n][c][1] = o[n][c][2] = o[n][c][3] = 0.f;
+    }
+#pragma unroll 1
+    for (int k = 0; k < pc.n && ok; ++k, ++it) {
+      const int st = static_cast<int>(it % kStages);
+      ok = __all_sync(0xffffffffu, mbar_wait_bounded(baddr(&hdr->full[st]), static_cast<uint32_t>((it / kStages) & 1),
+                                                     ctl, ST_TIMEOUT_EPILOGUE));
+      if (!ok) break;
+      const int left = len - (pc.tile0 + k) * kDcTile - 16 * warp;  // tokens of this warp's slice
+      if (left > 0) {
+        const uint32_t kb = ring + st * dc_stage_bytes(kD) + row_at, vb = kb + kHalf;
+        const float ks = hdr->scales[st][warp], vs = hdr->scales[st][4 + warp];
+        float s[kNt][4];
+#pragma unroll
+        for (int n = 0; n < kNt; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
+#pragma unroll
+        for (int c = 0; c < kChunks; c += 2) {
+          uint32_t r[4];  // (tokens 0-7, chunk c), (8-15, c), (0-7, c + 1), (8-15, c + 1)
+          ldmatrix4(kb + static_cast<uint32_t>(((c + cadd) ^ swz) << 4), r);
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            uint32_t a0, a1, a2, a3;
+            codes_to_half(r[2 * i], a0, a2);
+            codes_to_half(r[2 * i + 1], a1, a3);
+#pragma unroll
+            for (int n = 0; n < kNt; ++n) mma16816(s[n], a0, a1, a2, a3, q[n][c + i][0], q[n][c + i][1]);
+          }
+        }
+        // s[n]: tokens g and g + 8 (rows) of heads 2 t, 2 t + 1 (columns)
+        const float eb = static_cast<float>(static_cast<int>(__float_as_uint(vs) >> 23) - 127), vs_inv = 1.f / vs;
+        const bool in0 = g < left, in1 = g + 8 < left;
+        bool grow = false;
+        float mx[kNt][2];
+#pragma unroll
+        for (int n = 0; n < kNt; ++n) {
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const float f = qs[n][h] * ks;
+            s[n][h] = in0 ? fmaf(s[n][h], f, eb) : -INFINITY;
+            s[n][2 + h] = in1 ? fmaf(s[n][2 + h], f, eb) : -INFINITY;
+            float x = fmaxf(s[n][h], s[n][2 + h]);
+            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
+            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
+            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
+            mx[n][h] = x;
+            grow |= x > m[n][h] + kDcRescale;
+          }
+        }
+        if (__any_sync(0xffffffffu, grow)) {
+#pragma unroll
+          for (int n = 0; n < kNt; ++n) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const float mn = fmaxf(m[n][h], mx[n][h]);
+              const float f = m[n][h] == -INFINITY ? 0.f : ex2(m[n][h] - mn);
+              m[n][h] = mn;
+              l[n][h] *= f;
+#pragma unroll
+              for (int c = 0; c < kChunks; ++c) {
+                o[n][c][h] *= f;
+                o[n][c][2 + h] *= f;
+              }
+            }
+          }
+        }
+        uint32_t pb[kNt][2];
+#pragma unroll
+        for (int n = 0; n < kNt; ++n) {
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const float mm = m[n][h] == -INFINITY ? 0.f : m[n][h];
+            s[n][h] = ex2(s[n][h] - mm);
+            s[n][2 + h] = ex2(s[n][2 + h] - mm);
+            l[n][h] += (s[n][h] + s[n][2 + h]) * vs_inv;
+          }
+          pb[n][0] = transpose8(half_pair(s[n][0], s[n][1]));  // B: tokens 2 t, 2 t + 1 of head g
+          pb[n][1] = transpose8(half_pair(s[n][2], s[n][3]));  // tokens 2 t + 8, 2 t + 9
+        }
+        // Codes behind the last token are whatever the page held: clear them
+        // (0 times a NaN code would not be 0).
+        const bool tail = left < 16;
+        uint32_t keep0 = ~0u, keep1 = ~0u;
+        if (tail) {
+          keep0 = (2 * t < left ? 0xFFFFu : 0u) | (2 * t + 1 < left ? 0xFFFF0000u : 0u);
+          keep1 = (2 * t + 8 < left ? 0xFFFFu : 0u) | (2 * t + 9 < left ? 0xFFFF0000u : 0u);
+        }
+#pragma unroll
+        for (int c = 0; c < kChunks; c += 2) {
+          uint32_t r[4];
+          ldmatrix4t(vb + static_cast<uint32_t>(((c + cadd) ^ swz) << 4), r);
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            // register: codes (token 2 t, d 2 g), (2 t, 2 g + 1), (2 t + 1, 2 g), (2 t + 1, 2 g + 1)
+            uint32_t a0, a1, a2, a3;  // rows 0-7 of A: even d, rows 8-15: odd d
+            codes_to_half(__byte_perm(r[2 * i], 0, 0x3120), a0, a1);
+            codes_to_half(__byte_perm(r[2 * i + 1], 0, 0x3120), a2, a3);
+            if (tail) a0 &= keep0, a1 &= keep0, a2 &= keep1, a3 &= keep1;
+#pragma unroll
+            for (int n = 0; n < kNt; ++n) mma16816(o[n][c + i], a0, a1, a2, a3, pb[n][0], pb[n][1]);
+          }
+        }
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(baddr(&hdr->empty[st]));
+    }
+    // ---- the four warps' results of this piece
+    consumers_sync();  // the last piece's have been read
+#pragma unroll
+    for (int n = 0; n < kNt; ++n) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        float x = l[n][h];
+        x += __shfl_xor_sync(0xffffffffu, x, 4);
+        x += __shfl_xor_sync(0xffffffffu, x, 8);
+        x += __shfl_xor_sync(0xffffffffu, x, 16);
+        const int head = 8 * n + 2 * t + h;
+        if (g == 0) {
+          red_m[warp * kHeads + head] = m[n][h];
+          red_l[warp * kHeads + head] = x;
+        }
+        float* dst = red_o + (warp * kHeads + head) * kD + 2 * g;
+#pragma unroll
+        for (int c = 0; c < kChunks; ++c) *reinterpret_cast<float2*>(dst + 16 * c) = make_float2(o[n][c][h], o[n][c][2 + h]);
+      }
+    }
+    consumers_sync();
+    const int tid = 32 * warp + lane;
+    const bool whole = pc.n == pc.tiles;
+    const int64_t slot_floats = 16 * (kD + 2);
+    float* ws = p.work + (2 * static_cast<int64_t>(blockIdx.x) + (pc.tile0 == 0 ? 1 : 0)) * slot_floats;
+    for (int i = tid; i < nh * (kD / 4); i += 128) {
+      const int head = i / (kD / 4), col = i % (kD / 4);
+      float M = red_m[head];
+      for (int k = 1; k < 4; ++k) M = fmaxf(M, red_m[k * kHeads + head]);
+      float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+      float L = 0.f;
+      for (int k = 0; k < 4; ++k) {
+        const float mk = red_m[k * kHeads + head];
+        // a warp without tokens has m = -inf and l = 0; one that met only NaN has l = NaN
+        const float f = mk == -INFINITY ? 1.f : ex2(mk - M);
+        const float4 v = reinterpret_cast<const float4*>(red_o + (k * kHeads + head) * kD)[col];
+        a.x += f * v.x, a.y += f * v.y, a.z += f * v.z, a.w += f * v.w;
+        L += f * red_l[k * kHeads + head];
+      }
+      if (whole) {
+        const float inv = 1.f / L;
+        uint16_t* dst = static_cast<uint16_t*>(p.o.p) + pc.seq * p.o.token + (h0 + head) * p.o.head + 4 * col;
+        *reinterpret_cast<uint2*>(dst) = make_uint2(bf16_two(a.x * inv, a.y * inv), bf16_two(a.z * inv, a.w * inv));
+        if (col == 0 && p.lse)
+          p.lse[static_cast<int64_t>(pc.seq) * p.heads + h0 + head] = (M + log2f(L)) * 0.6931471805599453f;
+      } else {
+        __stcg(reinterpret_cast<float4*>(ws + head * kD) + col, a);
+        if (col == 0) {
+          __stcg(ws + 16 * kD + head, M);
+          __stcg(ws + 16 * kD + 16 + head, L);
+        }
+      }
+    }
+    if (whole) continue;
+    // ---- a part of a row: the last of its CTAs joins the parts
+    const int64_t tiles = hdr->tiles;
+    const int first = static_cast<int>(((pc.row0 + 1) * hdr->ctas - 1) / tiles);
+    const int last = static_cast<int>(((pc.row0 + pc.tiles) * hdr->ctas - 1) / tiles);
+    const int parts = last - first + 1;
+    __threadfence();
+    consumers_sync();
+    if (tid == 0) hdr->last = atomicAdd(p.counters + first, 1) == parts - 1 ? 1 : 0;
+    consumers_sync();
+    if (!hdr->last) continue;
+    __threadfence();
+    const float* first_ws = p.work + (2 * static_cast<int64_t>(first) + 1) * slot_floats;
+    auto part_ws = [&](int k) { return k == 0 ? first_ws : p.work + 2 * static_cast<int64_t>(first + k) * slot_floats; };
+    for (int i = tid; i < nh * (kD / 4); i += 128) {
+      const int head = i / (kD / 4), col = i % (kD / 4);
+      float M = -INFINITY;
+      for (int k = 0; k < parts; ++k) M = fmaxf(M, __ldcg(part_ws(k) + 16 * kD + head));
+      float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+      float L = 0.f;
+#pragma unroll 4
+      for (int k = 0; k < parts; ++k) {
+        const float* src = part_ws(k);
+        const float mk = __ldcg(src + 16 * kD + head);
+        const float f = mk == -INFINITY ? 1.f : ex2(mk - M);
+        const float4 v = __ldcg(reinterpret_cast<const float4*>(src + head * kD) + col);
+        a.x += f * v.x, a.y += f * v.y, a.z += f * v.z, a.w += f * v.w;
+        L += f * __ldcg(src + 16 * kD + 16 + head);
+      }
+      const float inv = 1.f / L;
+      uint16_t* dst = static_cast<uint16_t*>(p.o.p) + pc.seq * p.o.token + (h0 + head) * p.o.head + 4 * col;
+      *reinterpret_cast<uint2*>(dst) = make_uint2(bf16_two(a.x * inv, a.y * inv), bf16_two(a.z * inv, a.w * inv));
+      if (col == 0 && p.lse)
+        p.lse[static_cast<int64_t>(pc.seq) * p.heads + h0 + head] = (M + log2f(L)) * 0.6931471805599453f;
+    }
+    if (tid == 0) p.counters[first] = 0;  // ready for the next launch
+  }
+}
+
+template <int kD, int kNt>
+__global__ void __launch_bounds__(kDcThreads) decode_kernel(const __grid_constant__ DecodeParams p) {
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  const uint32_t raw = smem_u32(smem_raw), base = (raw + 1023u) & ~1023u;
+  uint8_t* gbase = smem_raw + (base - raw);
+  DcHeader* hdr = reinterpret_cast<DcHeader*>(gbase);
+  const uint32_t ring = base + 1024u;
+  constexpr int kStages = dc_stages(kD, 8 * kNt);
+  float* red = reinterpret_cast<float*>(gbase + 1024 + kStages * dc_stage_bytes(kD));
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (warp == 0 && lane == 0) {
+    for (int s = 0; s < kStages; ++s) {
+      mbar_init(baddr(&hdr->full[s]), 1);
+      mbar_init(baddr(&hdr->empty[s]), 4);
+    }
+    hdr->abort_flag = 0;
+    fence_mbar_init();
+  }
+  if (warp == kDcTmaWarp) {
+    if (lane < 2) tma_prefetch_desc(lane ? &p.tm_v : &p.tm_k);
+    // tiles of all rows, then the sequence in which this CTA's stretch begins
+    int64_t total = 0;
+    for (int s = lane; s < p.n_seqs; s += 32) {
+      const int len = __ldg(p.lens + s);
+      if (blockIdx.x == 0 && (len < 0 || len > p.table_width * p.cache.page)) atomicOr(p.status, ST_BAD_INDEX);
+      total += dc_tiles(p, s);
+    }
+    for (int k = 16; k; k >>= 1) total += __shfl_xor_sync(0xffffffffu, total, k);
+    total *= p.streams;
+    // at least two tiles to a CTA and at most 64 parts to a row on average: past
+    // that the joining costs more than the reading
+    const int64_t rows = static_cast<int64_t>(p.n_seqs) * p.streams;
+    const int ctas = static_cast<int>(min(static_cast<int64_t>(gridDim.x), min((total + 1) / 2, 64 * rows)));
+    const int64_t g0 = ctas > 0 ? blockIdx.x * total / ctas : 0;
+    int64_t at = 0;
+    int seq = 0;
+    bool found = false;
+    for (int s0 = 0; s0 < p.n_seqs && !found; s0 += 32) {
+      const int64_t mine = s0 + lane < p.n_seqs ? static_cast<int64_t>(dc_tiles(p, s0 + lane)) * p.streams : 0;
+      int64_t upto = mine;
+      for (int k = 1; k < 32; k <<= 1) {
+        const int64_t x = __shfl_up_sync(0xffffffffu, upto, k);
+        if (lane >= k) upto += x;
+      }
+      const unsigned past = __ballot_sync(0xffffffffu, at + upto > g0);
+      found = past != 0;
+      const int src = found ? __ffs(past) - 1 : 31;
+      const int64_t incl = __shfl_sync(0xffffffffu, upto, src), own = __shfl_sync(0xffffffffu, mine, src);
+      seq = s0 + src;
+      at += found ? incl - own : incl;
+    }
+    if (lane == 0) {
+      hdr->tiles = total;
+      hdr->ctas = ctas;
+      hdr->seq = seq;
+      hdr->base = at;
+    }
+  }
   __syncthreads();
-  const float M = fmaxf(fmaxf(sm[0], sm[1]), fmaxf(sm[2], sm[3]));
-  float L = 0.f, w[4];
-  for (int k = 0; k < 4; ++k) {
-    w[k] = sl[k] == 0.f ? 0.f : expf(sm[k] - M);
-    L += w[k] * sl[k];
+  // sequences without a token: O = 0, lse = -inf
+  for (int s = blockIdx.x; s < p.n_seqs; s += gridDim.x) {
+    if (dc_len(p, s) > 0) continue;
+    for (int i = threadIdx.x; i < p.heads * (kD / 8); i += kDcThreads) {
+      const int head = i / (kD / 8), col = i % (kD / 8);
+      uint16_t* dst = static_cast<uint16_t*>(p.o.p) + s * p.o.token + head * p.o.head;
+      reinterpret_cast<uint4*>(dst)[col] = make_uint4(0, 0, 0, 0);
+      if (col == 0 && p.lse) p.lse[static_cast<int64_t>(s) * p.heads + head] = -INFINITY;
+    }
   }
-  __nv_bfloat16* o = static_cast<__nv_bfloat16*>(p.o.p) + seq * p.o.token + head * p.o.head;
-  if (threadIdx.x < kD) {
-    float v = 0.f;
-    for (int k = 0; k < 4; ++k) v += w[k] * so[k][threadIdx.x];
-    o[threadIdx.x] = __float2bfloat16(L == 0.f ? 0.f : v / L);
-  }
-  if (threadIdx.x == 0 && p.lse) p.lse[static_cast<int64_t>(seq) * p.heads + head] = M + logf(L);
+  if (static_cast<int>(blockIdx.x) >= hdr->ctas) return;
+  Walk w;
+  w.g = blockIdx.x * hdr->tiles / hdr->ctas;
+  w.g1 = (blockIdx.x + 1) * hdr->tiles / hdr->ctas;
+  w.base = hdr->base;
+  w.seq = hdr->seq;
+  w.tiles = dc_tiles(p, w.seq);
+  const WaitCtl ctl{&hdr->abort_flag, p.status, p.timeout_ns};
+  if (warp == kDcTmaWarp) dc_produce<kD, kStages>(p, hdr, ring, w, ctl, lane);
+  else dc_consume<kD, kNt>(p, hdr, ring, red, w, ctl, warp, lane);
+}
+
+bsp_status encode_codes(bsp_device* dev, CUtensorMap* tm, const bsp_kv_cache& c, const void* codes) {
+  const uint64_t dims[4] = {static_cast<uint64_t>(c.d), static_cast<uint64_t>(c.page),
+                            static_cast<uint64_t>(c.kv_heads), static_cast<uint64_t>(c.n_pages)};
+  const uint64_t strides[3] = {static_cast<uint64_t>(c.d), static_cast<uint64_t>(c.head_stride),
+                               static_cast<uint64_t>(c.page_stride)};
+  const uint32_t box[4] = {static_cast<uint32_t>(c.d), static_cast<uint32_t>(std::min(c.page, kDcTile)), 1, 1};
+  return encode_nd(dev, tm, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, codes, dims, strides, box,
+                   c.d == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B);
+}
+
+using DecodeKernel = void (*)(DecodeParams);
+DecodeKernel pick(int d, int group) {
+  if (d == 64) return group > 8 ? decode_kernel<64, 2> : decode_kernel<64, 1>;
+  return group > 8 ? decode_kernel<128, 2> : decode_kernel<128, 1>;
 }
 
 }  // namespace
 
-bsp_status launch_decode(const bsp_decode_plan* plan, const DecodeParams& p, cudaStream_t stream) {
-  const dim3 grid(p.n_seqs, p.heads);
-  if (plan->d == 64) decode_kernel<64><<<grid, 128, 0, stream>>>(p);
-  else decode_kernel<128><<<grid, 128, 0, stream>>>(p);
+int64_t decode_work_floats(int32_t ctas, int32_t d) { return 2 * static_cast<int64_t>(ctas) * 16 * (d + 2); }
+
+// Two CTAs fit an SM (shared memory).
+int32_t decode_ctas(const bsp_device* dev) { return 2 * dev->sm_count; }
+
+int decode_smem_bytes(int d, int group) { return dc_smem(d, group > 8 ? 16 : 8); }
+
+bsp_status launch_decode(const bsp_decode_plan* plan, DecodeParams& p, cudaStream_t stream) {
+  bsp_status st = encode_codes(plan->dev, &p.tm_k, p.cache, p.cache.k);
+  if (st == BSP_OK) st = encode_codes(plan->dev, &p.tm_v, p.cache, p.cache.v);
+  if (st != BSP_OK) return st;
+  const DecodeKernel kernel = pick(plan->d, p.group);
+  st = cuda_check(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, plan->smem_bytes),
+                  "cudaFuncSetAttribute(decode)");
+  if (st != BSP_OK) return st;
+  kernel<<<plan->grid, kDcThreads, plan->smem_bytes, stream>>>(p);
   return cuda_check(cudaGetLastError(), "decode attention launch");
 }
 

@@ -44,6 +44,7 @@ struct AppendParams {
 };
 
 struct DecodeParams {
+  CUtensorMap tm_k, tm_v;     // codes: [page][head][token][d], boxes of up to 64 tokens of one page and head
   HeadsView q;
   HeadsOut o;
   float* lse;
@@ -52,8 +53,14 @@ struct DecodeParams {
   const int32_t* page_table;
   int64_t table_stride, table_width;
   int32_t n_seqs, heads;
-  float scale;
+  int32_t group;              // query heads of one key/value head
+  int32_t chunks;             // rows of up to 16 query heads per key/value head
+  int32_t streams;            // rows per sequence: kv_heads * chunks
+  float scale_log2;
+  float* work;                // two slots per CTA: O [16][d], m [16], l [16] of a row's part
+  int32_t* counters;          // one per CTA: finished parts of the row that begins in it, 0 between launches
   unsigned int* status;
+  uint64_t timeout_ns;
 };
 
 // A unit of prompt attention: one or two tiles (tile_tokens queries x packed
@@ -105,6 +112,12 @@ struct bsp_prompt_plan {
 struct bsp_decode_plan {
   bsp_device* dev = nullptr;
   int32_t max_seqs = 0, heads = 0, kv_heads = 0, d = 0, page = 0;
+  int32_t grid = 0, smem_bytes = 0;
+  uint64_t timeout_ns = 0;
+  void* d_blob = nullptr;  // counters | partial results
+  size_t blob_bytes = 0;
+  int32_t* d_counters = nullptr;
+  float* d_work = nullptr;
 };
 
 namespace bsp {
@@ -112,7 +125,10 @@ bsp_status launch_rope_table(bsp_device* dev, int64_t n_pos, int32_t rot, double
                              float* table, cudaStream_t stream);
 bsp_status launch_rope(const RopeParams& p, bsp_dtype type, cudaStream_t stream);
 bsp_status launch_append(const AppendParams& p, cudaStream_t stream);
-bsp_status launch_decode(const bsp_decode_plan* plan, const DecodeParams& p, cudaStream_t stream);
+bsp_status launch_decode(const bsp_decode_plan* plan, DecodeParams& p, cudaStream_t stream);
+int32_t decode_ctas(const bsp_device* dev);
+int64_t decode_work_floats(int32_t ctas, int32_t d);
+int decode_smem_bytes(int d, int group);
 bsp_status plan_prompt_host(bsp_prompt_plan* p, const int32_t* q_lens, const int32_t* kv_lens, int sm_count,
                             const bsp_spmm_opts* opts);
 bsp_status launch_prompt(const bsp_prompt_plan* plan, PromptParams& p, cudaStream_t stream);
