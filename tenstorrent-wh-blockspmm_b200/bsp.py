@@ -37,7 +37,7 @@ EXPORTS = [
     "bsp_attn_plan_create", "bsp_attn_execute", "bsp_attn_plan_destroy", "bsp_attn_plan_info",
     "bsp_attn_host", "bsp_attn_plan_inspect", "bsp_spmm_plan_traffic", "bsp_spmm_plan_entry_rows",
     "bsp_rope_table", "bsp_rope", "bsp_kv_append", "bsp_prompt_plan_create", "bsp_prompt_execute",
-    "bsp_prompt_plan_destroy", "bsp_prompt_plan_info", "bsp_decode_plan_create", "bsp_decode_execute",
+    "bsp_prompt_plan_destroy", "bsp_prompt_plan_info", "bsp_prompt_plan_inspect", "bsp_decode_plan_create", "bsp_decode_execute",
     "bsp_decode_plan_destroy", "bsp_decode_plan_info",
 ]
 IPC_HANDLE_BYTES = 64
@@ -188,6 +188,7 @@ def lib():
         "bsp_prompt_execute": (S, [P, P, I64, I64, P, I64, I64, P, I64, I64, ctypes.c_float, P, I64, I64, P, P]),
         "bsp_prompt_plan_destroy": (S, [P]),
         "bsp_prompt_plan_info": (S, [P, ctypes.POINTER(I64)]),
+        "bsp_prompt_plan_inspect": (S, [I32, P, P, I32, I32, I32, I32, ctypes.POINTER(Opts), I32, P, P, P]),
         "bsp_decode_plan_create": (S, [P, I32, I32, I32, I32, I32, ctypes.POINTER(Opts), ctypes.POINTER(P)]),
         "bsp_decode_execute": (S, [P, ctypes.POINTER(KvCacheDesc), P, I64, I64, I32, P, P, I64, I64, ctypes.c_float,
                                    P, I64, I64, P, P]),
@@ -748,7 +749,7 @@ def _heads_tensor(x, name, heads=None, d=None, tokens=None, f32=False):
     n, h, e = x.shape
     if (heads is not None and h != heads) or (d is not None and e != d) or (tokens is not None and n != tokens):
         _refuse(f"{name} is {tuple(x.shape)}, expected {(tokens, heads, d)}")
-    if x.stride(2) != 1 and e > 1:
+    if x.stride(2) != 1 and e > 1 and n > 0:
         _refuse(f"{name}: the values of a head must be contiguous")
     return x
 
@@ -971,6 +972,24 @@ class PromptPlan:
             self.close()
         except Exception:
             pass
+
+
+def inspect_prompt_plan(q_lens, kv_lens, heads, kv_heads, d, causal=True, opts=None, sm_count=148):
+    """Run the prompt attention planner on the host only (no GPU)."""
+    ql = np.ascontiguousarray(q_lens, dtype=np.int32)
+    kl = np.ascontiguousarray(kv_lens, dtype=np.int32)
+    if ql.ndim != 1 or ql.shape != kl.shape:
+        _refuse("q_lens and kv_lens must be lists of one length")
+    info = np.zeros(16, np.int64)
+    o = opts if opts is not None else Opts()
+    args = (ql.size, _ptr(ql), _ptr(kl), heads, kv_heads, d, int(bool(causal)), ctypes.byref(o), sm_count, _ptr(info))
+    _check(lib().bsp_prompt_plan_inspect(*args, None, None))
+    units = np.zeros((max(int(info[0]), 1), 12), np.int32)
+    cta = np.zeros(int(info[1]) + 1, np.int32)
+    _check(lib().bsp_prompt_plan_inspect(*args, _ptr(units), _ptr(cta)))
+    dd = {k: int(info[i]) for i, k in enumerate(PROMPT_INFO_KEYS)}
+    dd.update(unit_table=units[: int(info[0])], cta_begin=cta)
+    return dd
 
 
 DECODE_INFO_KEYS = ["max_seqs", "ctas", "heads", "kv_heads", "d", "page", "_6", "_7", "workspace_bytes", "smem_bytes"]
