@@ -736,50 +736,75 @@ ROPE_LAYOUTS = {"half": 0, "interleaved": 1}
 ROPE_KINDS = {"none": 0, "linear": 1, "base": 2, "parts": 3}
 
 
+class _Torch:
+    """The names of torch that every call below needs, looked up once: a call
+    costs a few microseconds, and `import torch` in each helper or a Stream
+    object for the stream's number would be most of it."""
+    bf16 = f32 = i32 = raw_stream = None
+
+    @classmethod
+    def load(cls):
+        import torch
+
+        cls.bf16, cls.f32, cls.i32 = torch.bfloat16, torch.float32, torch.int32
+        raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+        cls.raw_stream = raw or (lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
+def _stream_of(stream, dev: Device):
+    """Stream number: the given stream, or the current one of dev's GPU."""
+    if stream is None:
+        if _Torch.raw_stream is None:
+            _Torch.load()
+        return _Torch.raw_stream(dev.ordinal)
+    return stream.cuda_stream if hasattr(stream, "cuda_stream") else int(stream)
+
+
 def _refuse(msg):
     raise BspError(BSP_ERR_INVALID_ARG, msg)
 
 
-def _heads_tensor(x, name, heads=None, d=None, tokens=None, f32=False):
-    """A [tokens, heads, d] operand on the GPU: bf16 (or f32), d contiguous."""
-    import torch
-
-    if not x.is_cuda or x.dim() != 3 or not (x.dtype is torch.bfloat16 or (f32 and x.dtype is torch.float32)):
-        _refuse(f"{name} must be a bf16{' or f32' if f32 else ''} cuda tensor [tokens, heads, d]")
-    n, h, e = x.shape
-    if (heads is not None and h != heads) or (d is not None and e != d) or (tokens is not None and n != tokens):
+def _heads_tensor(x, name, tokens, heads, d, dtype=None):
+    """Pointer, token stride and head stride of a [tokens, heads, d] operand on
+    the GPU, d contiguous; bf16 unless another type is asked for.  A dimension
+    of one entry is never stepped over: its stride counts as 0."""
+    if _Torch.bf16 is None:
+        _Torch.load()
+    if not x.is_cuda or x.dtype is not (dtype or _Torch.bf16):
+        _refuse(f"{name} must be a {dtype or _Torch.bf16} cuda tensor, not {x.dtype} on {x.device}")
+    if x.shape != (tokens, heads, d):
         _refuse(f"{name} is {tuple(x.shape)}, expected {(tokens, heads, d)}")
-    if x.stride(2) != 1 and e > 1 and n > 0:
+    st, sh, sd = x.stride()
+    if sd != 1 and d > 1 and tokens > 0:
         _refuse(f"{name}: the values of a head must be contiguous")
-    return x
+    return x.data_ptr(), st if tokens > 1 else 0, sh if heads > 1 else 0
 
 
-def _index_tensor(x, name, dim=1):
-    import torch
-
-    if not x.is_cuda or x.dtype is not torch.int32 or x.dim() != dim or (x.numel() and x.stride(-1) != 1):
-        _refuse(f"{name} must be an int32 cuda tensor of {dim} dimension(s), contiguous rows")
-    return x
+def _index_tensor(x, name, *shape):
+    """Pointer of an int32 tensor on the GPU, contiguous rows; None: any size."""
+    if _Torch.i32 is None:
+        _Torch.load()
+    if not x.is_cuda or x.dtype is not _Torch.i32 or x.dim() != len(shape) or (x.stride(-1) != 1 and x.numel() > 1):
+        _refuse(f"{name} must be an int32 cuda tensor of {len(shape)} dimension(s), contiguous rows")
+    for have, want in zip(x.shape, shape):
+        if want is not None and have != want:
+            _refuse(f"{name} is {tuple(x.shape)}, expected {shape}")
+    return x.data_ptr()
 
 
 def _rope_tensor(table):
-    import torch
-
-    if not table.is_cuda or table.dtype is not torch.float32 or table.dim() != 3 or table.shape[2] != 2 \
+    if _Torch.f32 is None:
+        _Torch.load()
+    if not table.is_cuda or table.dtype is not _Torch.f32 or table.dim() != 3 or table.shape[2] != 2 \
             or not table.is_contiguous():
         _refuse("a rotary table is a contiguous f32 cuda tensor [positions, rot / 2, 2]")
-    return table
+    return table.data_ptr()
 
 
 def _rope_layout(layout):
     if layout not in ROPE_LAYOUTS:
         _refuse(f"rotary layout {layout!r}: one of {sorted(ROPE_LAYOUTS)}")
     return ROPE_LAYOUTS[layout]
-
-
-def _stride3(x, dim):
-    # a dimension of one entry may carry any stride: it is never stepped over
-    return x.stride(dim) if x.shape[dim] > 1 else 0
 
 
 def rope_table(n_pos, rot, base=10000.0, kind="none", factor=1.0, context=0.0, slow=1.0, fast=32.0, magnitude=1.0,
@@ -796,7 +821,7 @@ def rope_table(n_pos, rot, base=10000.0, kind="none", factor=1.0, context=0.0, s
         _refuse("n_pos and rot must be positive")
     table = torch.empty((n_pos, rot // 2, 2), dtype=torch.float32, device=torch.device("cuda", dev.ordinal))
     sc = RopeScaling(ROPE_KINDS[kind], factor, context, slow, fast, magnitude)
-    _check(lib().bsp_rope_table(dev.handle, n_pos, rot, base, ctypes.byref(sc), _ptr(table), _stream_ptr(stream)))
+    _check(lib().bsp_rope_table(dev.handle, n_pos, rot, base, ctypes.byref(sc), _ptr(table), _stream_of(stream, dev)))
     return table
 
 
@@ -805,27 +830,27 @@ def rope(x, positions, table, layout="half", transpose=False, out=None, dev: Dev
     (i, i + rot/2) for "half", (2i, 2i + 1) for "interleaved"; the rest of a
     head is copied.  transpose=True gives the gradient of x from that of the
     result.  out may be x."""
-    import torch
-
-    _heads_tensor(x, "x", f32=True)
-    _index_tensor(positions, "positions")
-    _rope_tensor(table)
+    if x.dim() != 3:
+        _refuse("x must be [tokens, heads, d]")
     tokens, heads, d = x.shape
-    if positions.shape[0] != tokens:
-        _refuse(f"{positions.shape[0]} positions for {tokens} tokens")
+    if _Torch.bf16 is None:
+        _Torch.load()
+    dtype = x.dtype if x.dtype is _Torch.f32 else _Torch.bf16
+    xp, xt, xh = _heads_tensor(x, "x", tokens, heads, d, dtype)
+    pp = _index_tensor(positions, "positions", tokens)
+    tp = _rope_tensor(table)
     if out is None:
+        import torch
+
         out = torch.empty((tokens, heads, d), dtype=x.dtype, device=x.device)
-    else:
-        _heads_tensor(out, "out", heads, d, tokens, f32=True)
-        if out.dtype is not x.dtype:
-            _refuse("out must have the type of x")
+    yp, yt, yh = _heads_tensor(out, "out", tokens, heads, d, dtype)
     if tokens == 0 or heads == 0:
         return out
     dev = dev or device(x.device.index or 0)
-    _check(lib().bsp_rope(dev.handle, x.data_ptr(), _stride3(x, 0), _stride3(x, 1), positions.data_ptr(),
-                          table.data_ptr(), table.shape[0], tokens, heads, d, 2 * table.shape[1],
-                          _rope_layout(layout), int(bool(transpose)), F32 if x.dtype is torch.float32 else BF16,
-                          out.data_ptr(), _stride3(out, 0), _stride3(out, 1), _stream_ptr(stream)))
+    n_pos, half, _ = table.shape
+    _check(lib().bsp_rope(dev.handle, xp, xt, xh, pp, tp, n_pos, tokens, heads, d, 2 * half, _rope_layout(layout),
+                          1 if transpose else 0, F32 if dtype is _Torch.f32 else BF16, yp, yt, yh,
+                          _stream_of(stream, dev)))
     return out
 
 
@@ -852,7 +877,8 @@ class KvCache:
         ps = k.stride(0) if n > 1 else h * hs
         self.desc = KvCacheDesc(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), n, ps, hs, h,
                                 page, d)
-        self._ref = ctypes.byref(self.desc)
+        self.ref = ctypes.byref(self.desc)
+        self.kv_heads, self.page, self.d = h, page, d
 
     @staticmethod
     def empty(n_pages, kv_heads, page, d, device_index=0):
@@ -872,51 +898,44 @@ def kv_append(cache: KvCache, k, v, starts, before, pages, table=None, layout="h
     pages[s, i] is the page of its positions i * page ....  With a rotary table
     keys are rotated on the way; q [tokens, heads, d] is rotated to q_out and
     the rotated keys go to k_out where these are given (bsp_kv_append)."""
-    c = cache.desc
+    hk, d = cache.kv_heads, cache.d
     tokens = k.shape[0]
-    _heads_tensor(k, "k", c.kv_heads, c.d)
-    _heads_tensor(v, "v", c.kv_heads, c.d, tokens)
-    _index_tensor(starts, "starts")
-    _index_tensor(before, "before")
-    _index_tensor(pages, "pages", 2)
+    kp, kt, kh = _heads_tensor(k, "k", tokens, hk, d)
+    vp, vt, vh = _heads_tensor(v, "v", tokens, hk, d)
     n = before.shape[0]
-    if starts.shape[0] != n + 1 or pages.shape[0] != n:
-        _refuse(f"{n} sequences need {n + 1} starts and {n} rows of pages")
-    rot = n_pos = tab = 0
+    sp = _index_tensor(starts, "starts", n + 1)
+    bp = _index_tensor(before, "before", n)
+    gp = _index_tensor(pages, "pages", n, None)
+    width = pages.shape[1]
+    rot = n_pos = 0
+    tp = None
     if table is not None:
-        _rope_tensor(table)
-        n_pos, rot, tab = table.shape[0], 2 * table.shape[1], table.data_ptr()
+        tp = _rope_tensor(table)
+        n_pos, rot = table.shape[0], 2 * table.shape[1]
     if (q is None) != (q_out is None):
         _refuse("q and q_out come together")
-    qa, qs, qt = (0, 0, 0), (0, 0, 0), 0
+    qp = qt = qh = op = ot = oh = yp = yt = yh = None
+    heads = 0
     if q is not None:
-        qt = q.shape[1]
-        _heads_tensor(q, "q", None, c.d, tokens)
-        _heads_tensor(q_out, "q_out", qt, c.d, tokens)
-        qa = (q.data_ptr(), _stride3(q, 0), _stride3(q, 1))
-        qs = (q_out.data_ptr(), _stride3(q_out, 0), _stride3(q_out, 1))
-    ka = (0, 0, 0)
+        heads = q.shape[1]
+        qp, qt, qh = _heads_tensor(q, "q", tokens, heads, d)
+        op, ot, oh = _heads_tensor(q_out, "q_out", tokens, heads, d)
     if k_out is not None:
-        _heads_tensor(k_out, "k_out", c.kv_heads, c.d, tokens)
-        ka = (k_out.data_ptr(), _stride3(k_out, 0), _stride3(k_out, 1))
+        yp, yt, yh = _heads_tensor(k_out, "k_out", tokens, hk, d)
     if tokens == 0 or n == 0:
         return cache
     dev = dev or device(k.device.index or 0)
-    _check(lib().bsp_kv_append(dev.handle, cache._ref, k.data_ptr(), _stride3(k, 0), _stride3(k, 1), v.data_ptr(),
-                               _stride3(v, 0), _stride3(v, 1), tokens, n, starts.data_ptr(), before.data_ptr(),
-                               pages.data_ptr(), _stride3(pages, 0), pages.shape[1], tab or None, n_pos, rot,
-                               _rope_layout(layout), qa[0] or None, qa[1], qa[2], qt, qs[0] or None, qs[1], qs[2],
-                               ka[0] or None, ka[1], ka[2], _stream_ptr(stream)))
+    _check(lib().bsp_kv_append(dev.handle, cache.ref, kp, kt, kh, vp, vt, vh, tokens, n, sp, bp, gp,
+                               pages.stride(0) if n > 1 else 0, width, tp, n_pos, rot, _rope_layout(layout), qp,
+                               qt or 0, qh or 0, heads, op, ot or 0, oh or 0, yp, yt or 0, yh or 0,
+                               _stream_of(stream, dev)))
     return cache
 
 
 def _lse_tensor(lse, tokens, heads):
-    import torch
-
     if lse is None:
         return None
-    if not lse.is_cuda or lse.dtype is not torch.float32 or tuple(lse.shape) != (tokens, heads) \
-            or not lse.is_contiguous():
+    if not lse.is_cuda or lse.dtype is not _Torch.f32 or lse.shape != (tokens, heads) or not lse.is_contiguous():
         _refuse(f"lse must be a contiguous f32 cuda tensor {(tokens, heads)}")
     return lse.data_ptr()
 
@@ -953,14 +972,13 @@ class PromptPlan:
     def execute(self, q, k, v, o, scale=None, lse=None, stream=None):
         """q, o: bf16 cuda [q_tokens, heads, d]; k, v [kv_tokens, kv_heads, d];
         lse (optional): f32 [q_tokens, heads]."""
-        _heads_tensor(q, "q", self.heads, self.d, self.q_tokens)
-        _heads_tensor(o, "o", self.heads, self.d, self.q_tokens)
-        _heads_tensor(k, "k", self.kv_heads, self.d, self.kv_tokens)
-        _heads_tensor(v, "v", self.kv_heads, self.d, self.kv_tokens)
-        _check(lib().bsp_prompt_execute(
-            self.handle, q.data_ptr(), _stride3(q, 0), _stride3(q, 1), k.data_ptr(), _stride3(k, 0), _stride3(k, 1),
-            v.data_ptr(), _stride3(v, 0), _stride3(v, 1), self.scale if scale is None else float(scale), o.data_ptr(),
-            _stride3(o, 0), _stride3(o, 1), _lse_tensor(lse, self.q_tokens, self.heads), _stream_ptr(stream)))
+        n, m, d = self.q_tokens, self.kv_tokens, self.d
+        qa = _heads_tensor(q, "q", n, self.heads, d)
+        ka = _heads_tensor(k, "k", m, self.kv_heads, d)
+        va = _heads_tensor(v, "v", m, self.kv_heads, d)
+        oa = _heads_tensor(o, "o", n, self.heads, d)
+        _check(lib().bsp_prompt_execute(self.handle, *qa, *ka, *va, self.scale if scale is None else scale, *oa,
+                                        _lse_tensor(lse, n, self.heads), _stream_of(stream, self.dev)))
 
     def close(self):
         if self.handle:
@@ -1019,16 +1037,13 @@ class DecodePlan:
         cache; pages: int32 [sequences, width]; lse (optional): f32
         [sequences, heads]."""
         n = q.shape[0]
-        _heads_tensor(q, "q", self.heads, self.d)
-        _heads_tensor(o, "o", self.heads, self.d, n)
-        _index_tensor(lens, "lens")
-        _index_tensor(pages, "pages", 2)
-        if lens.shape[0] != n or pages.shape[0] != n:
-            _refuse(f"{n} queries need {n} lengths and {n} rows of pages")
-        _check(lib().bsp_decode_execute(
-            self.handle, cache._ref, q.data_ptr(), _stride3(q, 0), _stride3(q, 1), n, lens.data_ptr(),
-            pages.data_ptr(), _stride3(pages, 0), pages.shape[1], self.scale if scale is None else float(scale),
-            o.data_ptr(), _stride3(o, 0), _stride3(o, 1), _lse_tensor(lse, n, self.heads), _stream_ptr(stream)))
+        qa = _heads_tensor(q, "q", n, self.heads, self.d)
+        oa = _heads_tensor(o, "o", n, self.heads, self.d)
+        lp = _index_tensor(lens, "lens", n)
+        gp = _index_tensor(pages, "pages", n, None)
+        _check(lib().bsp_decode_execute(self.handle, cache.ref, *qa, n, lp, gp, pages.stride(0) if n > 1 else 0,
+                                        pages.shape[1], self.scale if scale is None else scale, *oa,
+                                        _lse_tensor(lse, n, self.heads), _stream_of(stream, self.dev)))
 
     def close(self):
         if self.handle:

@@ -207,6 +207,7 @@ bsp_status bsp_prompt_plan_create(bsp_device* dev, int32_t n_seqs, const int32_t
         s = cuda_check(cudaMemcpy(p->d_cta_begin, p->h_cta_begin.data(), p->h_cta_begin.size() * sizeof(int32_t),
                                   cudaMemcpyHostToDevice),
                        "upload plan tables");
+      if (s == BSP_OK) s = prepare_prompt(p);
     }
   }
   if (s != BSP_OK) {
@@ -336,6 +337,7 @@ bsp_status bsp_decode_plan_create(bsp_device* dev, int32_t max_seqs, int32_t hea
   p->d_counters = static_cast<int32_t*>(p->d_blob);
   p->d_work = reinterpret_cast<float*>(static_cast<uint8_t*>(p->d_blob) + counters);
   s = cuda_check(cudaMemset(p->d_counters, 0, counters), "clear the decode counters");
+  if (s == BSP_OK) s = prepare_decode(p);
   // the clearing ran on the legacy stream: executes may come on any other
   if (s == BSP_OK) s = cuda_check(cudaStreamSynchronize(nullptr), "clear the decode counters");
   if (s != BSP_OK) {

@@ -599,15 +599,17 @@ int32_t decode_ctas(const bsp_device* dev) { return 2 * dev->sm_count; }
 
 int decode_smem_bytes(int d, int group) { return dc_smem(d, group > 8 ? 16 : 8); }
 
+bsp_status prepare_decode(const bsp_decode_plan* plan) {
+  return cuda_check(cudaFuncSetAttribute(pick(plan->d, plan->heads / plan->kv_heads),
+                                         cudaFuncAttributeMaxDynamicSharedMemorySize, plan->smem_bytes),
+                    "cudaFuncSetAttribute(decode)");
+}
+
 bsp_status launch_decode(const bsp_decode_plan* plan, DecodeParams& p, cudaStream_t stream) {
   bsp_status st = encode_codes(plan->dev, &p.tm_k, p.cache, p.cache.k);
   if (st == BSP_OK) st = encode_codes(plan->dev, &p.tm_v, p.cache, p.cache.v);
   if (st != BSP_OK) return st;
-  const DecodeKernel kernel = pick(plan->d, p.group);
-  st = cuda_check(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, plan->smem_bytes),
-                  "cudaFuncSetAttribute(decode)");
-  if (st != BSP_OK) return st;
-  kernel<<<plan->grid, kDcThreads, plan->smem_bytes, stream>>>(p);
+  pick(plan->d, p.group)<<<plan->grid, kDcThreads, plan->smem_bytes, stream>>>(p);
   return cuda_check(cudaGetLastError(), "decode attention launch");
 }
 

@@ -125,6 +125,9 @@ bsp_status launch_rope_table(bsp_device* dev, int64_t n_pos, int32_t rot, double
                              float* table, cudaStream_t stream);
 bsp_status launch_rope(const RopeParams& p, bsp_dtype type, cudaStream_t stream);
 bsp_status launch_append(const AppendParams& p, cudaStream_t stream);
+// one-time settings of the kernel that a plan launches
+bsp_status prepare_prompt(const bsp_prompt_plan* plan);
+bsp_status prepare_decode(const bsp_decode_plan* plan);
 bsp_status launch_decode(const bsp_decode_plan* plan, DecodeParams& p, cudaStream_t stream);
 int32_t decode_ctas(const bsp_device* dev);
 int64_t decode_work_floats(int32_t ctas, int32_t d);

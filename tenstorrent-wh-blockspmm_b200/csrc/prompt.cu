@@ -417,9 +417,17 @@ bsp_status encode_heads(bsp_device* dev, CUtensorMap* tm, const HeadsView& x, in
   return encode_nd(dev, tm, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, x.p, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
+using PromptKernel = void (*)(PromptParams);
+PromptKernel pick(int d) { return d == 64 ? prompt_tcgen05<64> : prompt_tcgen05<128>; }
+
 }  // namespace
 
 int prompt_smem_bytes(int d) { return static_cast<int>(2048u + (2u + pr_slots(d)) * pr_tile(d)); }
+
+bsp_status prepare_prompt(const bsp_prompt_plan* plan) {
+  return cuda_check(cudaFuncSetAttribute(pick(plan->d), cudaFuncAttributeMaxDynamicSharedMemorySize, plan->smem_bytes),
+                    "cudaFuncSetAttribute(prompt)");
+}
 
 bsp_status launch_prompt(const bsp_prompt_plan* plan, PromptParams& p, cudaStream_t stream) {
   bsp_device* dev = plan->dev;
@@ -431,11 +439,7 @@ bsp_status launch_prompt(const bsp_prompt_plan* plan, PromptParams& p, cudaStrea
     if (st == BSP_OK) st = encode_heads(dev, &p.tm_v, p.v, plan->kv_tokens, plan->kv_heads, plan->d, 1, 128);
   }
   if (st != BSP_OK) return st;
-  const auto kernel = plan->d == 64 ? prompt_tcgen05<64> : prompt_tcgen05<128>;
-  st = cuda_check(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, plan->smem_bytes),
-                  "cudaFuncSetAttribute(prompt)");
-  if (st != BSP_OK) return st;
-  kernel<<<plan->grid, kPrThreads, plan->smem_bytes, stream>>>(p);
+  pick(plan->d)<<<plan->grid, kPrThreads, plan->smem_bytes, stream>>>(p);
   return cuda_check(cudaGetLastError(), "prompt attention launch");
 }
 
