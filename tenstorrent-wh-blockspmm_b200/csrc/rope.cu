@@ -33,31 +33,47 @@ __global__ void rope_table_kernel(float2* table, int64_t n_pos, int half, double
   }
 }
 
-// A thread turns unit u of one head of one token.
-template <typename T>
-__global__ void __launch_bounds__(256) rope_kernel(const RopeParams p, int units, int items_per_block) {
+// A thread turns unit u of kHeads heads of one token: (cos, sin) are loaded
+// once for them, and kHeads loads are in flight.
+template <typename T, int kHeads>
+__global__ void __launch_bounds__(256) rope_kernel(const RopeParams p, int units, int items_per_block, int groups) {
+  constexpr int kN = Vec<T>::kN;
   const int u = threadIdx.x % units, y = threadIdx.x / units;
   const uint32_t item = blockIdx.x * static_cast<uint32_t>(items_per_block) + y;
-  const uint32_t token = item / p.heads, head = item - token * p.heads;
+  const uint32_t token = item / groups, head0 = (item - token * groups) * kHeads;
   if (y >= items_per_block || token >= p.tokens) return;
-  const RopeUnit un(u, p.rot, p.interleaved);
-  const T* x = static_cast<const T*>(p.x.p) + token * p.x.token + head * p.x.head;
-  T* out = static_cast<T*>(p.y.p) + token * p.y.token + head * p.y.head;
+  const RopeUnit<kN> un(u, p.rot, p.d);
+  const T* x = static_cast<const T*>(p.x.p) + token * p.x.token + head0 * p.x.head;
+  T* out = static_cast<T*>(p.y.p) + token * p.y.token + head0 * p.y.head;
   const int32_t pos = __ldg(p.positions + token);
+  float lo[kHeads][kN], hi[kHeads][kN];
+#pragma unroll
+  for (int h = 0; h < kHeads; ++h)
+    if (head0 + h < p.heads) {
+      load_vec(x + h * p.x.head + un.lo, lo[h]);
+      load_vec(x + h * p.x.head + un.hi, hi[h]);
+    }
   if (pos < 0 || pos >= p.n_pos) {
     if (u == 0) atomicOr(p.status, ST_BAD_INDEX);
     return;
   }
-  float lo[8], hi[8];
-  load8(x + un.lo, lo);
-  load8(x + un.hi, hi);
-  if (un.turns) {
-    float2 cs[8];
-    load_turns(p.table + static_cast<int64_t>(pos) * (p.rot / 2), u, cs);
-    turn16(lo, hi, cs, p.interleaved, p.sign);
-  }
-  store8(out + un.lo, lo);
-  store8(out + un.hi, hi);
+  float2 cs[kN];
+  if (un.turns) load_turns<kN>(p.table + static_cast<int64_t>(pos) * (p.rot / 2), u, p.rot, p.interleaved, cs);
+#pragma unroll
+  for (int h = 0; h < kHeads; ++h)
+    if (head0 + h < p.heads) {
+      if (un.turns) turn_unit<kN>(lo[h], hi[h], cs, p.interleaved, p.sign);
+      store_vec(out + h * p.y.head + un.lo, lo[h]);
+      store_vec(out + h * p.y.head + un.hi, hi[h]);
+    }
+}
+
+template <typename T, int kHeads>
+void run_rope(const RopeParams& p, cudaStream_t stream) {
+  const int units = p.d / (2 * Vec<T>::kN), per_block = 256 / units, groups = (p.heads + kHeads - 1) / kHeads;
+  const int64_t items = p.tokens * groups;
+  const unsigned blocks = static_cast<unsigned>((items + per_block - 1) / per_block);
+  rope_kernel<T, kHeads><<<blocks, 256, 0, stream>>>(p, units, per_block, groups);
 }
 
 }  // namespace
@@ -71,15 +87,16 @@ bsp_status launch_rope_table(bsp_device* dev, int64_t n_pos, int32_t rot, double
   return cuda_check(cudaGetLastError(), "rotary table launch");
 }
 
-bsp_status launch_rope(const RopeParams& p, bsp_dtype type, cudaStream_t stream) {
-  const int units = p.d / 16;
-  const int per_block = 256 / units;
-  const int64_t items = p.tokens * p.heads;
-  const unsigned blocks = static_cast<unsigned>((items + per_block - 1) / per_block);
-  if (type == BSP_BF16)
-    rope_kernel<uint16_t><<<blocks, 256, 0, stream>>>(p, units, per_block);
-  else
-    rope_kernel<float><<<blocks, 256, 0, stream>>>(p, units, per_block);
+bsp_status launch_rope(const RopeParams& p, bsp_dtype type, int sm_count, cudaStream_t stream) {
+  // One head a thread while that does not fill the GPU (2048 threads an SM).
+  const bool few = p.tokens * p.heads * (p.d / 16) < static_cast<int64_t>(sm_count) * 2048;
+  if (type == BSP_BF16) {
+    if (few) run_rope<uint16_t, 1>(p, stream);
+    else run_rope<uint16_t, 4>(p, stream);
+  } else {
+    if (few) run_rope<float, 1>(p, stream);
+    else run_rope<float, 4>(p, stream);
+  }
   return cuda_check(cudaGetLastError(), "rotary kernel launch");
 }
 
