@@ -29,6 +29,12 @@
 //
 // Warps (320 threads, one CTA per SM): 0-3 softmax of tile a, 4-7 of tile b
 // (TMEM lane quarter = warp & 3), 8 MMA, 9 TMA.  Every wait is bounded.
+//
+// The softmax bounds the kernel: 16 exponentials per clock and SM alone take
+// as long as the two products of d = 128, and they are in the tile's chain
+// S -> P -> O -> S.  So some of them are computed in the FMA pipe (exp2_pair),
+// scaling and sums are packed two to an instruction, and P is handed over in
+// two parts, so that O += P V begins while the rest of the exponentials runs.
 #include <cuda_bf16.h>
 
 #include "bsp_ptx.cuh"
@@ -44,6 +50,7 @@ constexpr int kPrMmaWarp = 8, kPrTmaWarp = 9;
 constexpr uint32_t kPrAtom = 128 * 128;  // 128 rows x 128 bytes (64 values)
 constexpr float kPrRescale = 8.f;        // log2 of the growth that forces a rescale
 constexpr int kPrMaxSlots = 8;
+constexpr int kPrByFma = 2;              // of each 8 pairs of exponentials, those in the FMA pipe
 
 __host__ __device__ constexpr uint32_t pr_tile(int d) { return 128u * 2u * static_cast<uint32_t>(d); }
 __host__ __device__ constexpr int pr_slots(int d) { return d == 128 ? 5 : 8; }
@@ -51,12 +58,13 @@ __host__ __device__ constexpr int pr_slots(int d) { return d == 128 ? 5 : 8; }
 struct PrHeader {
   uint64_t q_full, q_empty;
   uint64_t kv_full[kPrMaxSlots], kv_empty[kPrMaxSlots];
-  uint64_t s_full[2], p_full[2], o_full[2], o_empty[2];
+  uint64_t s_full[2], p_full[2][2], o_full[2], o_empty[2];
   uint64_t drain;
   uint32_t tmem_base;
   int abort_flag;
 };
-static_assert(sizeof(PrHeader) <= 1024, "header must fit its 1 KiB slot");
+constexpr uint32_t kPrHeader = 1024;
+static_assert(sizeof(PrHeader) <= kPrHeader, "header must fit its slot");
 
 __device__ __forceinline__ uint32_t baddr(const uint64_t* b) { return smem_u32(b); }
 
@@ -76,6 +84,48 @@ __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
+}
+// Two fp32 values in a register pair: one instruction for both.
+__device__ __forceinline__ uint64_t pair_of(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void unpair(uint64_t p, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(p)); }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+
+// 2^x of two values without the exponential unit: x = n + f with n the nearest
+// whole number (adding 1.5 * 2^23 leaves it in the low bits), 2^f by a
+// polynomial of degree 4 on [-1/2, 1/2] with p(0) = 1, fitted for the least
+// relative error (2.9e-6), and n added to the exponent.  x <= 127; below -126
+// (a masked score) the result is 2^-126, which vanishes beside the maximum's
+// 2^-8 or more.
+__device__ __forceinline__ uint64_t exp2_pair(uint64_t x) {
+  const uint64_t magic = pair_of(12582912.f, 12582912.f), back = pair_of(-12582912.f, -12582912.f);
+  float a, b;
+  unpair(x, a, b);
+  x = pair_of(fmaxf(a, -126.f), fmaxf(b, -126.f));
+  const uint64_t t = add2(x, magic);
+  const uint64_t f = fma2(add2(t, back), pair_of(-1.f, -1.f), x);
+  uint64_t p = fma2(f, pair_of(0.009582852944731712f, 0.009582852944731712f),
+                    pair_of(0.055906426161527634f, 0.055906426161527634f));
+  p = fma2(p, f, pair_of(0.24024099111557007f, 0.24024099111557007f));
+  p = fma2(p, f, pair_of(0.6931241750717163f, 0.6931241750717163f));
+  p = fma2(p, f, pair_of(1.f, 1.f));
+  float ta, tb;
+  unpair(t, ta, tb);
+  unpair(p, a, b);
+  return pair_of(__uint_as_float(__float_as_uint(a) + (__float_as_uint(ta) << 23)),
+                 __uint_as_float(__float_as_uint(b) + (__float_as_uint(tb) << 23)));
 }
 __device__ __forceinline__ uint32_t pack2(float a, float b) {
   const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
@@ -131,90 +181,101 @@ __device__ __forceinline__ void pr_tma(const PromptParams& p, PrHeader* hdr, uin
   __syncwarp();
 }
 
+// The warp waits as one; each batch of MMAs and their commits sits in one
+// branch of a single elected thread.  (An MMA that every lane passes under a
+// predicate costs about 54 cycles of issue; in such a branch 33 or less, and
+// the warp shares its scheduler with four softmax warps.)
 template <int kD>
-__device__ __forceinline__ void pr_mma(const PromptParams& p, PrHeader* hdr, uint8_t* ring_ptr, uint32_t q_smem,
-                                      uint32_t ring, uint32_t tmem, int u0, int u1, const WaitCtl& ctl, int lane) {
+__device__ __forceinline__ void pr_mma(const PromptParams& p, PrHeader* hdr, uint32_t q_smem, uint32_t ring,
+                                      uint32_t tmem, int u0, int u1, const WaitCtl& ctl, int lane) {
   constexpr int kSlots = pr_slots(kD);
   constexpr uint32_t kTile = pr_tile(kD), kAtom16 = kPrAtom >> 4;
-  const uint32_t is0 = lane == 0 ? 1u : 0u;
   const uint32_t idesc_s = idesc_bf16_f32(128, 128, 0, 0), idesc_o = idesc_bf16_f32(128, kD, 0, 1);
   const uint64_t qd = smem_desc(q_smem, 16u, 1024u, 2u);
   const uint64_t kd = smem_desc(ring, 16u, 1024u, 2u);
   const uint64_t vd = smem_desc(ring, kPrAtom, 1024u, 2u);  // MN-major: LBO = next 64 columns of d
-  int64_t slot_n = 0;  // ring position of K0 of the unit
+  int slot = 0;          // ring slot of the next K or V
+  uint32_t phase = 0;    // and its parity
   uint32_t units = 0, steps[2] = {0, 0}, outs[2] = {0, 0};
   bool ok = true;
-  auto full = [&](int64_t k) {
-    return wait_all(&hdr->kv_full[k % kSlots], static_cast<uint32_t>((k / kSlots) & 1), ctl, ST_TIMEOUT_MMA);
+  auto full = [&]() { return wait_all(&hdr->kv_full[slot], phase, ctl, ST_TIMEOUT_MMA); };
+  auto next_slot = [&]() {
+    if (++slot == kSlots) slot = 0, phase ^= 1u;
   };
-  auto scores = [&](int t, int64_t k) {
-    const uint64_t a = qd + t * (kTile >> 4), b = kd + (k % kSlots) * (kTile >> 4);
+  auto scores = [&](int t, int at) {  // in an elected branch
+    const uint64_t a = qd + t * (kTile >> 4), b = kd + at * (kTile >> 4);
 #pragma unroll
     for (int i = 0; i < kD / 16; ++i)
-      mma_bf16_pred(tmem + 128u * t, a + (i >> 2) * kAtom16 + (i & 3) * 2u, b + (i >> 2) * kAtom16 + (i & 3) * 2u,
-                    idesc_s, i > 0, is0);
-    mma_commit_pred(baddr(&hdr->s_full[t]), is0);
+      mma_bf16(tmem + 128u * t, a + (i >> 2) * kAtom16 + (i & 3) * 2u, b + (i >> 2) * kAtom16 + (i & 3) * 2u, idesc_s,
+               i > 0);
+    mma_commit(baddr(&hdr->s_full[t]));
   };
 #pragma unroll 1
   for (int u = u0; u < u1 && ok; ++u) {
     const PromptUnit un = p.units[u];
     const int n = max(un.n[0], un.n[1]);
     if (n == 0) continue;
-    ok = wait_all(&hdr->q_full, units & 1, ctl, ST_TIMEOUT_MMA) && full(slot_n);
+    ok = wait_all(&hdr->q_full, units & 1, ctl, ST_TIMEOUT_MMA) && full();
     if (!ok) break;
     ++units;
     tc_fence_after();
-    for (int t = 0; t < 2; ++t)
-      if (un.n[t] > 0) scores(t, slot_n);
-    mma_commit_pred(baddr(&hdr->kv_empty[slot_n % kSlots]), is0);
-    if (n == 1) mma_commit_pred(baddr(&hdr->q_empty), is0);
+    if (elect_one()) {
+      for (int t = 0; t < 2; ++t)
+        if (un.n[t] > 0) scores(t, slot);
+      mma_commit(baddr(&hdr->kv_empty[slot]));
+      if (n == 1) mma_commit(baddr(&hdr->q_empty));
+    }
+    __syncwarp();
+    next_slot();
 #pragma unroll 1
     for (int j = 0; j < n && ok; ++j) {
-      const int64_t kv = slot_n + 2 * j + 1, kn = slot_n + 2 * j + 2;
-      ok = full(kv);
-      if (!ok) break;
-      // Rows of V behind the sequence's end belong to its neighbour; their
-      // weight is 0, but 0 times an infinity or NaN there is not: clear them.
-      const int rows = un.kv_len - 128 * j;
-      if (rows < 128) {
-        uint8_t* v = ring_ptr + (kv % kSlots) * kTile;
-        for (int i = rows * 8 + lane; i < 128 * 8; i += 32)
-          for (int h = 0; h < kD / 64; ++h)
-            *reinterpret_cast<uint4*>(v + h * kPrAtom + i * 16) = make_uint4(0, 0, 0, 0);
-        fence_proxy_async_smem();
-        __syncwarp();
+      ok = full();
+      const int v_slot = slot;
+      next_slot();
+      const int k_slot = slot;
+      if (ok && j + 1 < n) {
+        ok = full();
+        next_slot();
       }
-      const int last = j < un.n[1] ? 1 : 0;        // last tile that uses V of this step
-      const int last_next = j + 1 < un.n[1] ? 1 : 0;
-      if (j + 1 < n) ok = full(kn);
-      for (int t = 0; t < 2 && ok; ++t) {
-        if (j >= un.n[t]) continue;
+      const int last = j < un.n[1] ? 1 : 0;           // last tile that uses V of this step
+      const int last_next = j + 1 < un.n[1] ? 1 : 0;  // and K of the next
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        if (!ok || j >= un.n[t]) continue;
         if (j == 0) {
           ok = wait_all(&hdr->o_empty[t], (outs[t] & 1) ^ 1u, ctl, ST_TIMEOUT_MMA);
           ++outs[t];
         }
-        ok = ok && wait_all(&hdr->p_full[t], steps[t] & 1, ctl, ST_TIMEOUT_MMA);
-        if (!ok) break;
-        ++steps[t];
-        tc_fence_after();
-        const uint64_t b = vd + (kv % kSlots) * (kTile >> 4);
+        const uint64_t b = vd + v_slot * (kTile >> 4);
+        const bool more = j + 1 < un.n[t];
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-          mma_bf16_ts_pred(tmem + 256u + 128u * t, tmem + 128u * t + 8u * i, b + i * 128u, idesc_o, j > 0 || i > 0, is0);
-        if (j == un.n[t] - 1) mma_commit_pred(baddr(&hdr->o_full[t]), is0);
-        if (t == last) mma_commit_pred(baddr(&hdr->kv_empty[kv % kSlots]), is0);
-        if (j + 1 < un.n[t]) {
-          scores(t, kn);
-          if (t == last_next) {
-            mma_commit_pred(baddr(&hdr->kv_empty[kn % kSlots]), is0);
-            if (j + 2 == n) mma_commit_pred(baddr(&hdr->q_empty), is0);
+        for (int part = 0; part < 2; ++part) {
+          ok = ok && wait_all(&hdr->p_full[t][part], steps[t] & 1, ctl, ST_TIMEOUT_MMA);
+          if (!ok) break;
+          tc_fence_after();
+          if (elect_one()) {
+#pragma unroll
+            for (int i = 4 * part; i < 4 * part + 4; ++i)
+              mma_bf16_ts(tmem + 256u + 128u * t, tmem + 128u * t + 8u * i, b + i * 128u, idesc_o, i > 0 || j > 0);
+            if (part == 1) {
+              if (!more) mma_commit(baddr(&hdr->o_full[t]));
+              if (t == last) mma_commit(baddr(&hdr->kv_empty[v_slot]));
+              if (more) {
+                scores(t, k_slot);
+                if (t == last_next) {
+                  mma_commit(baddr(&hdr->kv_empty[k_slot]));
+                  if (j + 2 == n) mma_commit(baddr(&hdr->q_empty));
+                }
+              }
+            }
           }
+          __syncwarp();
         }
+        ++steps[t];
       }
     }
-    slot_n += 2 * n;
   }
-  if (lane == 0) {
+  if (elect_one()) {
     mma_commit(baddr(&hdr->drain));
     drain_wait(baddr(&hdr->drain), 0, ctl);
   }
@@ -232,12 +293,13 @@ __device__ __forceinline__ void store32(uint16_t* dst, const uint32_t (&o)[32], 
 }
 
 template <int kD>
-__device__ __forceinline__ void pr_softmax(const PromptParams& p, PrHeader* hdr, uint32_t tmem, int u0, int u1,
-                                          const WaitCtl& ctl, int warp, int lane) {
+__device__ __forceinline__ void pr_softmax(const PromptParams& p, PrHeader* hdr, uint8_t* ring_ptr, uint32_t tmem,
+                                          int u0, int u1, const WaitCtl& ctl, int warp, int lane) {
   const int t = warp >> 2, row = 32 * (warp & 3) + lane;
   const uint32_t lanes = tmem + (static_cast<uint32_t>(32 * (warp & 3)) << 16);
   const uint32_t t_s = lanes + 128u * t, t_o = lanes + 256u + 128u * t;
   const int dt = t * p.tile_tokens + row / p.packed, dh = row % p.packed;
+  int64_t slot_n = 0;  // ring position of K0 of the unit
   uint32_t steps = 0, outs = 0;
 #pragma unroll 1
   for (int u = u0; u < u1; ++u) {
@@ -248,6 +310,7 @@ __device__ __forceinline__ void pr_softmax(const PromptParams& p, PrHeader* hdr,
     uint16_t* orow = static_cast<uint16_t*>(p.o.p) + token * p.o.token + (un.head0 + dh) * p.o.head;
     float* lrow = p.lse ? p.lse + token * p.heads + un.head0 + dh : nullptr;
     if (n == 0) {
+      slot_n += 2 * max(un.n[0], un.n[1]);
       if (valid) {
         for (int c = 0; c < kD / 8; ++c) reinterpret_cast<uint4*>(orow)[c] = make_uint4(0, 0, 0, 0);
         if (lrow) *lrow = -INFINITY;
@@ -256,6 +319,7 @@ __device__ __forceinline__ void pr_softmax(const PromptParams& p, PrHeader* hdr,
     }
     const int sees = p.causal ? min(un.kv_len, un.sees + dt) : un.kv_len;  // keys this row attends to
     float m = -INFINITY, l = 0.f;
+    bool big = false;  // |m| > 2^24 somewhere in the warp
 #pragma unroll 1
     for (int j = 0; j < n; ++j) {
       if (!wait_all(&hdr->s_full[t], steps & 1, ctl, ST_TIMEOUT_EPILOGUE)) return;
@@ -263,78 +327,105 @@ __device__ __forceinline__ void pr_softmax(const PromptParams& p, PrHeader* hdr,
       tc_fence_after();
       uint32_t v[4][32];
 #pragma unroll
-      for (int c = 0; c < 4; ++c) tmem_ld_32x32b_x32(t_s + 32u * c, v[c]);
+      for (int k = 0; k < 4; ++k) tmem_ld_32x32b_x32(t_s + 32u * k, v[k]);
+      // Rows of V behind the sequence's end belong to its neighbour; their weight
+      // is 0, but 0 times an infinity or NaN there is not: clear them before P is
+      // handed over.
+      if (un.kv_len - 128 * j < 128) {
+        const int64_t kv = slot_n + 2 * j + 1;
+        if (!wait_all(&hdr->kv_full[kv % pr_slots(kD)], static_cast<uint32_t>((kv / pr_slots(kD)) & 1), ctl,
+                      ST_TIMEOUT_EPILOGUE))
+          return;
+        uint8_t* vt = ring_ptr + (kv % pr_slots(kD)) * pr_tile(kD);
+        for (int i = (un.kv_len - 128 * j) * 8 + row; i < 128 * 8; i += 128)
+          for (int h = 0; h < kD / 64; ++h) *reinterpret_cast<uint4*>(vt + h * kPrAtom + i * 16) = make_uint4(0, 0, 0, 0);
+        fence_proxy_async_smem();
+      }
       tmem_ld_wait();
       const int limit = sees - 128 * j;
       if (__any_sync(0xffffffffu, limit < 128)) {
 #pragma unroll
-        for (int c = 0; c < 4; ++c)
+        for (int k = 0; k < 4; ++k)
 #pragma unroll
           for (int i = 0; i < 32; ++i)
-            if (32 * c + i >= limit) v[c][i] = 0xFF800000u;
+            if (32 * k + i >= limit) v[k][i] = 0xFF800000u;
       }
-      float x0 = -INFINITY, x1 = -INFINITY, x2 = -INFINITY, x3 = -INFINITY;
+      float x[4];
 #pragma unroll
-      for (int i = 0; i < 32; ++i) {
-        x0 = fmaxf(x0, __uint_as_float(v[0][i]));
-        x1 = fmaxf(x1, __uint_as_float(v[1][i]));
-        x2 = fmaxf(x2, __uint_as_float(v[2][i]));
-        x3 = fmaxf(x3, __uint_as_float(v[3][i]));
+      for (int k = 0; k < 4; ++k) {
+        x[k] = fmaxf(__uint_as_float(v[k][0]), __uint_as_float(v[k][1]));
+#pragma unroll
+        for (int i = 2; i < 32; i += 2) x[k] = fmaxf(x[k], fmaxf(__uint_as_float(v[k][i]), __uint_as_float(v[k][i + 1])));
       }
-      const float mx = fmaxf(fmaxf(x0, x1), fmaxf(x2, x3)) * p.scale_log2;
+      const float mx = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])) * p.scale_log2;
       const bool need = mx > m + kPrRescale;
       if (__any_sync(0xffffffffu, need)) {
         const float mn = need ? mx : m;
         const float alpha = need ? (m == -INFINITY ? 0.f : ex2(m - mn)) : 1.f;
         if (j > 0) {
 #pragma unroll 1
-          for (int c = 0; c < kD / 32; ++c) {
-            uint32_t o[32];
-            tmem_ld_32x32b_x32(t_o + 32u * c, o);
+          for (int c = 0; c < kD / 16; ++c) {
+            uint32_t o[16];
+            tmem_ld_32x32b_x16(t_o + 16u * c, o);
             tmem_ld_wait();
 #pragma unroll
-            for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
-            tmem_st_32x32b_x32(t_o + 32u * c, o);
+            for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+            tmem_st_32x32b_x16(t_o + 16u * c, o);
           }
         }
         l *= alpha;
         m = mn;
+        big = __any_sync(0xffffffffu, fabsf(m) > 16777216.f && m != -INFINITY);
       }
       // Exponents S c - m in one fused step.  For |m| above 2^24 the rounding of
       // m itself would show in them: there the product is rounded like m first.
-      float c = p.scale_log2, mm = m == -INFINITY ? 0.f : m;
-      if (__any_sync(0xffffffffu, fabsf(mm) > 16777216.f)) {
+      const float mm = m == -INFINITY ? 0.f : m;
+      uint64_t c2 = pair_of(p.scale_log2, p.scale_log2), m2 = pair_of(-mm, -mm);
+      if (big) {
 #pragma unroll
         for (int k = 0; k < 4; ++k)
 #pragma unroll
           for (int i = 0; i < 32; ++i)
-            v[k][i] = __float_as_uint(__fsub_rn(__fmul_rn(__uint_as_float(v[k][i]), c), mm));
-        c = 1.f;
-        mm = 0.f;
+            v[k][i] = __float_as_uint(__fsub_rn(__fmul_rn(__uint_as_float(v[k][i]), p.scale_log2), mm));
+        c2 = pair_of(1.f, 1.f);
+        m2 = 0;
       }
-      float l0 = 0.f, l1 = 0.f;
+      uint64_t l0 = 0, l1 = 0;  // (0, 0)
 #pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        uint32_t w[32];
+      for (int k = 0; k < 4; ++k) {
+        uint32_t w[16];
 #pragma unroll
-        for (int i = 0; i < 32; ++i) {
-          const float a = ex2(fmaf(__uint_as_float(v[2 * k + i / 16][2 * (i % 16)]), c, -mm));
-          const float b = ex2(fmaf(__uint_as_float(v[2 * k + i / 16][2 * (i % 16) + 1]), c, -mm));
-          l0 += a;
-          l1 += b;
+        for (int i = 0; i < 16; ++i) {
+          const uint64_t e = fma2(pair_of(__uint_as_float(v[k][2 * i]), __uint_as_float(v[k][2 * i + 1])), c2, m2);
+          float a, b;
+          if (i % 8 < kPrByFma) {
+            unpair(exp2_pair(e), a, b);
+          } else {
+            unpair(e, a, b);
+            a = ex2(a);
+            b = ex2(b);
+          }
+          if (i & 1) l1 = add2(l1, pair_of(a, b));
+          else l0 = add2(l0, pair_of(a, b));
           w[i] = pack2(a, b);
         }
-        tmem_st_32x32b_x32(t_s + 32u * k, w);
+        tmem_st_32x32b_x16(t_s + 16u * k, w);
+        if (k & 1) {
+          tmem_st_wait();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(baddr(&hdr->p_full[t][k >> 1]));
+        }
       }
-      l += l0 + l1;
-      tmem_st_wait();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(baddr(&hdr->p_full[t]));
+      float la, lb;
+      unpair(add2(l0, l1), la, lb);
+      l += la + lb;
     }
+    slot_n += 2 * max(un.n[0], un.n[1]);
     if (!wait_all(&hdr->o_full[t], outs & 1, ctl, ST_TIMEOUT_EPILOGUE)) return;
     ++outs;
     tc_fence_after();
+    if (m == -INFINITY && l < 1.f) l = 0.f;  // no key: exp2_pair gave 2^-126 for each masked one
     const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);  // a NaN sum stays one
 #pragma unroll 1
     for (int c = 0; c < kD / 32; ++c) {
@@ -360,7 +451,7 @@ __global__ void __launch_bounds__(kPrThreads, 1) prompt_tcgen05(const __grid_con
   const uint32_t base = (raw + 1023u) & ~1023u;
   uint8_t* gbase = smem_raw + (base - raw);
   PrHeader* hdr = reinterpret_cast<PrHeader*>(gbase);
-  const uint32_t q_smem = base + 1024u, ring = q_smem + 2u * pr_tile(kD);
+  const uint32_t q_smem = base + kPrHeader, ring = q_smem + 2u * pr_tile(kD);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int u0 = p.cta_begin[blockIdx.x], u1 = p.cta_begin[blockIdx.x + 1];
   if (threadIdx.x == 0) {
@@ -372,7 +463,8 @@ __global__ void __launch_bounds__(kPrThreads, 1) prompt_tcgen05(const __grid_con
     }
     for (int t = 0; t < 2; ++t) {
       mbar_init(baddr(&hdr->s_full[t]), 1);
-      mbar_init(baddr(&hdr->p_full[t]), 4);
+      mbar_init(baddr(&hdr->p_full[t][0]), 4);
+      mbar_init(baddr(&hdr->p_full[t][1]), 4);
       mbar_init(baddr(&hdr->o_full[t]), 1);
       mbar_init(baddr(&hdr->o_empty[t]), 4);
     }
@@ -392,12 +484,14 @@ __global__ void __launch_bounds__(kPrThreads, 1) prompt_tcgen05(const __grid_con
   tc_fence_after();
   const uint32_t tmem = hdr->tmem_base;
   const WaitCtl ctl{&hdr->abort_flag, p.status, p.timeout_ns};
-  if (warp == kPrMmaWarp)
-    pr_mma<kD>(p, hdr, gbase + 1024 + 2 * pr_tile(kD), q_smem, ring, tmem, u0, u1, ctl, lane);
-  else if (warp == kPrTmaWarp)
-    pr_tma<kD>(p, hdr, q_smem, ring, u0, u1, ctl, lane);
-  else
-    pr_softmax<kD>(p, hdr, tmem, u0, u1, ctl, warp, lane);
+  if (warp >= kPrMmaWarp) {
+    if (warp == kPrMmaWarp)
+      pr_mma<kD>(p, hdr, q_smem, ring, tmem, u0, u1, ctl, lane);
+    else if (warp == kPrTmaWarp)
+      pr_tma<kD>(p, hdr, q_smem, ring, u0, u1, ctl, lane);
+  } else {
+    pr_softmax<kD>(p, hdr, gbase + kPrHeader + 2 * pr_tile(kD), tmem, u0, u1, ctl, warp, lane);
+  }
   tc_fence_before();
   __syncthreads();
   if (warp == kPrMmaWarp) {
@@ -422,7 +516,7 @@ PromptKernel pick(int d) { return d == 64 ? prompt_tcgen05<64> : prompt_tcgen05<
 
 }  // namespace
 
-int prompt_smem_bytes(int d) { return static_cast<int>(2048u + (2u + pr_slots(d)) * pr_tile(d)); }
+int prompt_smem_bytes(int d) { return static_cast<int>(1024u + kPrHeader + (2u + pr_slots(d)) * pr_tile(d)); }
 
 bsp_status prepare_prompt(const bsp_prompt_plan* plan) {
   return cuda_check(cudaFuncSetAttribute(pick(plan->d), cudaFuncAttributeMaxDynamicSharedMemorySize, plan->smem_bytes),
