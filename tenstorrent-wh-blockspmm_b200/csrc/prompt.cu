@@ -11,10 +11,10 @@
 //
 // Steps.  128 keys a step.  Per tile and step
 //   S = Q K^T            128 x 128 x d    fp32 in TMEM
-//   P = exp2(S c - m)    one thread a row; c = scale log2 e; the running maximum
-//                        m moves only when it grows by more than 8 (2^8), and
-//                        only then O and the row sum l are rescaled; P goes back
-//                        to TMEM as bf16 pairs, over S
+//   P = exp2(S c - m)    one thread a row; c = scale log2 e; m follows the
+//                        running maximum when it is 2^8 behind, and only then
+//                        O and the row sum l are rescaled; P goes back to TMEM
+//                        as bf16 pairs, over S
 //   O += P V             128 x d x 128, A = P read from TMEM
 // and at the end O / l, m ln 2 + ln l.  With two tiles the tensor cores work on
 // one while the softmax of the other runs: the MMA warp issues
@@ -30,11 +30,19 @@
 // Warps (320 threads, one CTA per SM): 0-3 softmax of tile a, 4-7 of tile b
 // (TMEM lane quarter = warp & 3), 8 MMA, 9 TMA.  Every wait is bounded.
 //
-// The softmax bounds the kernel: 16 exponentials per clock and SM alone take
-// as long as the two products of d = 128, and they are in the tile's chain
-// S -> P -> O -> S.  So some of them are computed in the FMA pipe (exp2_pair),
-// scaling and sums are packed two to an instruction, and P is handed over in
-// two parts, so that O += P V begins while the rest of the exponentials runs.
+// The chain S -> P -> O -> S of a tile bounds the kernel: at 16384 tokens, 8
+// heads of 128, one step takes 3300 cycles of which a tile's softmax is 2050,
+// its products with their hand-overs 1150 (the tensor cores are busy 63 %, the
+// exponential unit 47 %).  What shortens it: the softmax does not wait for its
+// own maximum (weights are formed with the maximum of the steps before, the
+// step's own is found beside them and only moves m for the next step, or at
+// once if it is 2^20 above); a quarter of the exponentials is computed in the
+// FMA pipe (exp2_pair); scaling and sums are packed two to an instruction; P is
+// handed over in two parts of 64 keys, so that O += P V begins while the second
+// part is worked on.  442 us for 0.55 TFLOP (1242 TFLOP/s).  Steps of 64 keys
+// with two S buffers (no product in the chain) measured 545 us: an N = 64
+// product takes as long as N = 128.  Two threads a row (16 softmax warps)
+// measured 471 us against 447 us then.
 #include <cuda_bf16.h>
 
 #include "bsp_ptx.cuh"
@@ -49,6 +57,7 @@ constexpr int kPrThreads = 320;
 constexpr int kPrMmaWarp = 8, kPrTmaWarp = 9;
 constexpr uint32_t kPrAtom = 128 * 128;  // 128 rows x 128 bytes (64 values)
 constexpr float kPrRescale = 8.f;        // log2 of the growth that forces a rescale
+constexpr float kPrLate = 20.f;          // and of the one that cannot wait for the next step
 constexpr int kPrMaxSlots = 8;
 constexpr int kPrByFma = 2;              // of each 8 pairs of exponentials, those in the FMA pipe
 
@@ -58,7 +67,7 @@ __host__ __device__ constexpr int pr_slots(int d) { return d == 128 ? 5 : 8; }
 struct PrHeader {
   uint64_t q_full, q_empty;
   uint64_t kv_full[kPrMaxSlots], kv_empty[kPrMaxSlots];
-  uint64_t s_full[2], p_full[2][2], o_full[2], o_empty[2];
+  uint64_t s_full[2], p_full[2][2], h_full[2], o_full[2], o_empty[2];
   uint64_t drain;
   uint32_t tmem_base;
   int abort_flag;
@@ -80,6 +89,11 @@ __device__ __noinline__ bool drain_wait(uint32_t bar, uint32_t parity, const Wai
   return mbar_wait_bounded(bar, parity, c2, ST_TIMEOUT_DRAIN);
 }
 
+__device__ __forceinline__ float max3(float a, float b, float c) {  // NaN if one is
+  float y;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
+  return y;
+}
 __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -257,7 +271,9 @@ __device__ __forceinline__ void pr_mma(const PromptParams& p, PrHeader* hdr, uin
 #pragma unroll
             for (int i = 4 * part; i < 4 * part + 4; ++i)
               mma_bf16_ts(tmem + 256u + 128u * t, tmem + 128u * t + 8u * i, b + i * 128u, idesc_o, i > 0 || j > 0);
-            if (part == 1) {
+            if (part == 0) {
+              mma_commit(baddr(&hdr->h_full[t]));
+            } else {
               if (!more) mma_commit(baddr(&hdr->o_full[t]));
               if (t == last) mma_commit(baddr(&hdr->kv_empty[v_slot]));
               if (more) {
@@ -292,6 +308,57 @@ __device__ __forceinline__ void store32(uint16_t* dst, const uint32_t (&o)[32], 
   *reinterpret_cast<uint4*>(dst + 8) = make_uint4(w[4], w[5], w[6], w[7]);
 }
 
+// Largest of 64 scores, NaN if one is.
+__device__ __forceinline__ float row_max(const uint32_t (&a)[32], const uint32_t (&b)[32]) {
+  float x[4];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const uint32_t* y = (k < 2 ? a : b) + 16 * (k & 1);
+    x[k] = max3(__uint_as_float(y[0]), __uint_as_float(y[1]), __uint_as_float(y[2]));
+#pragma unroll
+    for (int i = 3; i < 15; i += 2) x[k] = max3(x[k], __uint_as_float(y[i]), __uint_as_float(y[i + 1]));
+    x[k] = max3(x[k], __uint_as_float(y[15]), __uint_as_float(y[15]));
+  }
+  return max3(max3(x[0], x[1], x[2]), x[3], x[3]);
+}
+
+// w = exp2(s c - m) of 64 scores as bf16 pairs; their sum.
+__device__ __forceinline__ float pr_weights(uint32_t (&a)[32], uint32_t (&b)[32], float c, float m, uint32_t (&w)[32]) {
+  float mm = m == -INFINITY ? 0.f : m;
+  // The exponent is one fused step.  For |m| above 2^24 the rounding of m itself
+  // would show in it: there the product is rounded like m first.
+  if (__any_sync(0xffffffffu, fabsf(mm) > 16777216.f)) {
+#pragma unroll
+    for (int i = 0; i < 32; ++i) {
+      a[i] = __float_as_uint(__fsub_rn(__fmul_rn(__uint_as_float(a[i]), c), mm));
+      b[i] = __float_as_uint(__fsub_rn(__fmul_rn(__uint_as_float(b[i]), c), mm));
+    }
+    c = 1.f;
+    mm = 0.f;
+  }
+  const uint64_t c2 = pair_of(c, c), m2 = pair_of(-mm, -mm);
+  uint64_t l0 = 0, l1 = 0;  // (0, 0)
+#pragma unroll
+  for (int i = 0; i < 32; ++i) {
+    const uint32_t* y = i < 16 ? a + 2 * i : b + 2 * (i - 16);
+    const uint64_t e = fma2(pair_of(__uint_as_float(y[0]), __uint_as_float(y[1])), c2, m2);
+    float p, q;
+    if (i % 8 < kPrByFma) {
+      unpair(exp2_pair(e), p, q);
+    } else {
+      unpair(e, p, q);
+      p = ex2(p);
+      q = ex2(q);
+    }
+    if (i & 1) l1 = add2(l1, pair_of(p, q));
+    else l0 = add2(l0, pair_of(p, q));
+    w[i] = pack2(p, q);
+  }
+  float p, q;
+  unpair(add2(l0, l1), p, q);
+  return p + q;
+}
+
 template <int kD>
 __device__ __forceinline__ void pr_softmax(const PromptParams& p, PrHeader* hdr, uint8_t* ring_ptr, uint32_t tmem,
                                           int u0, int u1, const WaitCtl& ctl, int warp, int lane) {
@@ -301,6 +368,20 @@ __device__ __forceinline__ void pr_softmax(const PromptParams& p, PrHeader* hdr,
   const int dt = t * p.tile_tokens + row / p.packed, dh = row % p.packed;
   int64_t slot_n = 0;  // ring position of K0 of the unit
   uint32_t steps = 0, outs = 0;
+  auto scale_o = [&](float alpha) {
+#pragma unroll 1
+    for (int c = 0; c < kD / 16; ++c) {
+      uint32_t o[16];
+      tmem_ld_32x32b_x16(t_o + 16u * c, o);
+      tmem_ld_wait();
+#pragma unroll
+      for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+      tmem_st_32x32b_x16(t_o + 16u * c, o);
+    }
+  };
+  auto weights = [&](uint32_t (&a)[32], uint32_t (&b)[32], float m, uint32_t (&w)[32]) {
+    return pr_weights(a, b, p.scale_log2, m, w);
+  };
 #pragma unroll 1
   for (int u = u0; u < u1; ++u) {
     const PromptUnit un = p.units[u];
@@ -318,16 +399,16 @@ __device__ __forceinline__ void pr_softmax(const PromptParams& p, PrHeader* hdr,
       continue;
     }
     const int sees = p.causal ? min(un.kv_len, un.sees + dt) : un.kv_len;  // keys this row attends to
-    float m = -INFINITY, l = 0.f;
-    bool big = false;  // |m| > 2^24 somewhere in the warp
+    float m = -INFINITY, l = 0.f;  // reference of the exponents, sum of the weights
+    float seen = -INFINITY;        // largest score so far; m follows when it is 2^8 behind
 #pragma unroll 1
     for (int j = 0; j < n; ++j) {
       if (!wait_all(&hdr->s_full[t], steps & 1, ctl, ST_TIMEOUT_EPILOGUE)) return;
       ++steps;
       tc_fence_after();
-      uint32_t v[4][32];
-#pragma unroll
-      for (int k = 0; k < 4; ++k) tmem_ld_32x32b_x32(t_s + 32u * k, v[k]);
+      uint32_t v[2][32];
+      tmem_ld_32x32b_x32(t_s, v[0]);
+      tmem_ld_32x32b_x32(t_s + 32u, v[1]);
       // Rows of V behind the sequence's end belong to its neighbour; their weight
       // is 0, but 0 times an infinity or NaN there is not: clear them before P is
       // handed over.
@@ -341,85 +422,70 @@ __device__ __forceinline__ void pr_softmax(const PromptParams& p, PrHeader* hdr,
           for (int h = 0; h < kD / 64; ++h) *reinterpret_cast<uint4*>(vt + h * kPrAtom + i * 16) = make_uint4(0, 0, 0, 0);
         fence_proxy_async_smem();
       }
-      tmem_ld_wait();
-      const int limit = sees - 128 * j;
-      if (__any_sync(0xffffffffu, limit < 128)) {
-#pragma unroll
-        for (int k = 0; k < 4; ++k)
-#pragma unroll
-          for (int i = 0; i < 32; ++i)
-            if (32 * k + i >= limit) v[k][i] = 0xFF800000u;
-      }
-      float x[4];
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        x[k] = fmaxf(__uint_as_float(v[k][0]), __uint_as_float(v[k][1]));
-#pragma unroll
-        for (int i = 2; i < 32; i += 2) x[k] = fmaxf(x[k], fmaxf(__uint_as_float(v[k][i]), __uint_as_float(v[k][i + 1])));
-      }
-      const float mx = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])) * p.scale_log2;
-      const bool need = mx > m + kPrRescale;
-      if (__any_sync(0xffffffffu, need)) {
-        const float mn = need ? mx : m;
-        const float alpha = need ? (m == -INFINITY ? 0.f : ex2(m - mn)) : 1.f;
-        if (j > 0) {
-#pragma unroll 1
-          for (int c = 0; c < kD / 16; ++c) {
-            uint32_t o[16];
-            tmem_ld_32x32b_x16(t_o + 16u * c, o);
-            tmem_ld_wait();
-#pragma unroll
-            for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
-            tmem_st_32x32b_x16(t_o + 16u * c, o);
-          }
-        }
-        l *= alpha;
+      // The maximum grew in the step before: O holds exactly the steps before
+      // this one now.
+      if (__any_sync(0xffffffffu, seen > m + kPrRescale)) {
+        const float mn = seen > m + kPrRescale ? seen : m;
+        if (j > 0) scale_o(m == -INFINITY ? 0.f : ex2(m - mn));
+        l *= m == -INFINITY ? 0.f : ex2(m - mn);
         m = mn;
-        big = __any_sync(0xffffffffu, fabsf(m) > 16777216.f && m != -INFINITY);
       }
-      // Exponents S c - m in one fused step.  For |m| above 2^24 the rounding of
-      // m itself would show in them: there the product is rounded like m first.
-      const float mm = m == -INFINITY ? 0.f : m;
-      uint64_t c2 = pair_of(p.scale_log2, p.scale_log2), m2 = pair_of(-mm, -mm);
-      if (big) {
+      tmem_ld_wait_regs(v[0]);
+      tmem_ld_wait_regs(v[1]);
 #pragma unroll
-        for (int k = 0; k < 4; ++k)
+      for (int part = 0; part < 2; ++part) {
+        if (part == 1) {
+          tmem_ld_wait_regs(v[0]);
+          tmem_ld_wait_regs(v[1]);
+        }
+        uint32_t(&a)[32] = v[0];
+        uint32_t(&b)[32] = v[1];
+        const int limit = sees - 128 * j - 64 * part;
+        auto mask = [&]() {
+          if (__any_sync(0xffffffffu, limit < 64)) {
 #pragma unroll
-          for (int i = 0; i < 32; ++i)
-            v[k][i] = __float_as_uint(__fsub_rn(__fmul_rn(__uint_as_float(v[k][i]), p.scale_log2), mm));
-        c2 = pair_of(1.f, 1.f);
-        m2 = 0;
-      }
-      uint64_t l0 = 0, l1 = 0;  // (0, 0)
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        uint32_t w[16];
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const uint64_t e = fma2(pair_of(__uint_as_float(v[k][2 * i]), __uint_as_float(v[k][2 * i + 1])), c2, m2);
-          float a, b;
-          if (i % 8 < kPrByFma) {
-            unpair(exp2_pair(e), a, b);
-          } else {
-            unpair(e, a, b);
-            a = ex2(a);
-            b = ex2(b);
+            for (int i = 0; i < 32; ++i) {
+              if (i >= limit) a[i] = 0xFF800000u;
+              if (32 + i >= limit) b[i] = 0xFF800000u;
+            }
           }
-          if (i & 1) l1 = add2(l1, pair_of(a, b));
-          else l0 = add2(l0, pair_of(a, b));
-          w[i] = pack2(a, b);
+        };
+        mask();
+        if (part == 0 && j == 0) m = row_max(a, b) * p.scale_log2;
+        // Weights with the maximum known so far; this part's own is found on the way.
+        uint32_t w[32];
+        const float mx = row_max(a, b) * p.scale_log2;
+        float sum = weights(a, b, m, w);
+        if (__any_sync(0xffffffffu, !(mx <= m + kPrLate) && m == m)) {
+          // It is too far above: move to it now, from the scores in TMEM.
+          const float mn = max3(m, mx, mx);
+          const float alpha = m == -INFINITY ? 0.f : ex2(m - mn);
+          if (part == 1) {  // O holds part 0 of this step too: wait for that product
+            if (!wait_all(&hdr->h_full[t], (steps - 1) & 1, ctl, ST_TIMEOUT_EPILOGUE)) return;
+            tc_fence_after();
+          }
+          if (part == 1 || j > 0) scale_o(alpha);
+          l *= alpha;
+          m = mn;
+          tmem_ld_32x32b_x32(t_s + 64u * part, a);
+          tmem_ld_32x32b_x32(t_s + 64u * part + 32u, b);
+          tmem_ld_wait_regs(a);
+          tmem_ld_wait_regs(b);
+          mask();
+          sum = weights(a, b, m, w);
         }
-        tmem_st_32x32b_x16(t_s + 16u * k, w);
-        if (k & 1) {
-          tmem_st_wait();
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(baddr(&hdr->p_full[t][k >> 1]));
+        seen = fmaxf(seen, mx);
+        if (part == 0) {
+          tmem_ld_32x32b_x32(t_s + 64u, v[0]);
+          tmem_ld_32x32b_x32(t_s + 96u, v[1]);
         }
+        tmem_st_32x32b_x32(t_s + 32u * part, w);
+        tmem_st_wait();
+        tc_fence_before();
+        __syncwarp();
+        mbar_arrive_pred(baddr(&hdr->p_full[t][part]), lane == 0);
+        l += sum;
       }
-      float la, lb;
-      unpair(add2(l0, l1), la, lb);
-      l += la + lb;
     }
     slot_n += 2 * max(un.n[0], un.n[1]);
     if (!wait_all(&hdr->o_full[t], outs & 1, ctl, ST_TIMEOUT_EPILOGUE)) return;
@@ -465,6 +531,7 @@ __global__ void __launch_bounds__(kPrThreads, 1) prompt_tcgen05(const __grid_con
       mbar_init(baddr(&hdr->s_full[t]), 1);
       mbar_init(baddr(&hdr->p_full[t][0]), 4);
       mbar_init(baddr(&hdr->p_full[t][1]), 4);
+      mbar_init(baddr(&hdr->h_full[t]), 1);
       mbar_init(baddr(&hdr->o_full[t]), 1);
       mbar_init(baddr(&hdr->o_empty[t]), 4);
     }
