@@ -41,35 +41,37 @@ using namespace dev;
 
 namespace {
 
+constexpr int kDcSlices = 2;             // of 16 tokens that a warp takes of a tile
+constexpr int kDcTile = 64 * kDcSlices;  // tokens
 constexpr int kDcThreads = 160;
-constexpr int kDcTile = 64;          // tokens
 constexpr int kDcTmaWarp = 4;
-constexpr int kDcMaxStages = 12;
+constexpr int kDcMaxSlots = 12;
 constexpr float kDcRescale = 8.f;    // log2 of the growth that moves the maximum
 
 struct DcHeader {
-  uint64_t full[kDcMaxStages], empty[kDcMaxStages];
+  uint64_t full[kDcMaxSlots], empty[kDcMaxSlots];
   int64_t tiles, base;  // tiles of all rows; first tile of sequence `seq`
   int32_t seq;
   int32_t ctas;         // CTAs that take part
   int32_t last;         // this CTA joins the row
   int abort_flag;
-  float scales[kDcMaxStages][8];  // per stage: 2^a of four slices of 16 tokens, then 2^b
+  float scales[kDcMaxSlots][kDcTile / 16];  // 2^a or 2^b of each 16 tokens of a slot
 };
 static_assert(sizeof(DcHeader) <= 1024, "header must fit its 1 KiB slot");
 
-// Shared memory from the 1 KiB-aligned base: header, stages (K then V), then
-// the warps' results: O [4][heads][d], m [4][heads], l [4][heads].
-// As many stages as let two CTAs share an SM's 228 KB (1 KB of each is the
-// system's).
-__host__ __device__ constexpr int dc_stage_bytes(int d) { return 2 * kDcTile * d; }
+// Shared memory from the 1 KiB-aligned base: header, slots (K and V of a tile
+// in turn), then the warps' results: O [4][heads][d], m [4][heads], l [4][heads].
+// CTAs on an SM: two, or one with rows of 16 heads (registers).
+__host__ __device__ constexpr int dc_per_sm(int heads) { return heads > 8 ? 1 : 2; }
+// As many slots as fit the SM's 228 KB then (1 KB of each CTA is the system's).
+__host__ __device__ constexpr int dc_slot_bytes(int d) { return kDcTile * d; }
 __host__ __device__ constexpr int dc_result_bytes(int d, int heads) { return 16 * heads * (d + 2); }
-__host__ __device__ constexpr int dc_stages(int d, int heads) {
-  const int n = (113 * 1024 - 2048 - dc_result_bytes(d, heads)) / dc_stage_bytes(d);
-  return n < kDcMaxStages ? n : kDcMaxStages;
+__host__ __device__ constexpr int dc_slots(int d, int heads) {
+  const int n = ((228 / dc_per_sm(heads) - 1) * 1024 - 2048 - dc_result_bytes(d, heads)) / dc_slot_bytes(d);
+  return n < kDcMaxSlots ? n : kDcMaxSlots;
 }
 __host__ __device__ constexpr int dc_smem(int d, int heads) {
-  return 2048 + dc_stages(d, heads) * dc_stage_bytes(d) + dc_result_bytes(d, heads);
+  return 2048 + dc_slots(d, heads) * dc_slot_bytes(d) + dc_result_bytes(d, heads);
 }
 
 __device__ __forceinline__ uint32_t baddr(const uint64_t* b) { return smem_u32(b); }
@@ -166,18 +168,17 @@ __device__ __forceinline__ bool next_piece(const DecodeParams& p, Walk& w, Piece
   return true;
 }
 
-template <int kD, int kStages>
+template <int kD, int kSlots>
 __device__ __forceinline__ void dc_produce(const DecodeParams& p, DcHeader* hdr, uint32_t ring, Walk w,
                                           const WaitCtl& ctl, int lane) {
-  constexpr uint32_t kHalf = kDcTile * kD;
   const int page = p.cache.page, shift = __ffs(page) - 1;  // a power of two
   const int box = min(page, kDcTile), boxes = kDcTile / box;  // per tile and operand
   const int kind = lane >> 4, at = (lane & 15) / boxes, sub = (lane & 15) % boxes;
   const int per_batch = 16 / boxes;
   const float* scale = kind ? p.cache.v_scale : p.cache.k_scale;
   const CUtensorMap* tm = kind ? &p.tm_v : &p.tm_k;
-  int64_t it = 0;
-  uint32_t armed = 0, armed_parity = 0;
+  int slot = 0;
+  uint32_t phase = 0, armed = 0, armed_parity = 0;
   bool ok = true;
   Piece pc;
   while (ok && next_piece(p, w, pc)) {
@@ -205,24 +206,21 @@ __device__ __forceinline__ void dc_produce(const DecodeParams& p, DcHeader* hdr,
       const float sc_next = scale_of(idn);
       const int n = min(per_batch, pc.n - b);
 #pragma unroll 1
-      for (int k = 0; k < n; ++k, ++it) {
-        const int st = static_cast<int>(it % kStages);
-        const uint32_t ph = static_cast<uint32_t>((it / kStages) & 1);
-        ok = __all_sync(0xffffffffu, mbar_wait_bounded(baddr(&hdr->empty[st]), ph ^ 1u, ctl, ST_TIMEOUT_PRODUCER));
+      for (int k = 0; k < 2 * n; ++k) {  // K, then V of each tile
+        ok = __all_sync(0xffffffffu, mbar_wait_bounded(baddr(&hdr->empty[slot]), phase ^ 1u, ctl, ST_TIMEOUT_PRODUCER));
         if (!ok) break;
-        const bool mine = at == k && id != -2;
-        if (at == k)
-          for (int i = 0; i < 4 / boxes; ++i) hdr->scales[st][4 * kind + sub * (4 / boxes) + i] = sc;
+        const bool now = 2 * at + kind == k, mine = now && id != -2;
+        if (now)
+          for (int i = 0; i < box / 16; ++i) hdr->scales[slot][sub * (box / 16) + i] = sc;
         const uint32_t bytes = static_cast<uint32_t>(__popc(__ballot_sync(0xffffffffu, mine))) * box * kD;
         __syncwarp();  // the scales are written before lane 0 arrives
-        const uint32_t bar = baddr(&hdr->full[st]);
+        const uint32_t bar = baddr(&hdr->full[slot]);
         mbar_arrive_expect_tx_pred(bar, bytes, lane == 0);
-        const int in_page = ((pc.tile0 + b + k) * kDcTile) & (page - 1);
-        tma_load_4d_pred(ring + st * dc_stage_bytes(kD) + kind * kHalf + sub * box * kD, tm, 0,
-                         in_page, kvh, id >= 0 ? id : static_cast<int32_t>(p.cache.n_pages),
-                         bar, mine);
-        armed |= 1u << st;
-        armed_parity = (armed_parity & ~(1u << st)) | (ph << st);
+        tma_load_4d_pred(ring + slot * dc_slot_bytes(kD) + sub * box * kD, tm, 0, 0, kvh,
+                         id >= 0 ? id : static_cast<int32_t>(p.cache.n_pages), bar, mine);
+        armed |= 1u << slot;
+        armed_parity = (armed_parity & ~(1u << slot)) | (phase << slot);
+        if (++slot == kSlots) slot = 0, phase ^= 1u;
       }
       id = idn;
       sc = sc_next;
@@ -231,28 +229,54 @@ __device__ __forceinline__ void dc_produce(const DecodeParams& p, DcHeader* hdr,
   if (lane == 0) {  // no copy may be in flight when the CTA leaves
     int zero = 0;
     const WaitCtl c2{&zero, ctl.status, ctl.timeout_ns};
-    for (int s = 0; s < kStages; ++s)
+    for (int s = 0; s < kSlots; ++s)
       if (armed & (1u << s)) mbar_wait_bounded(baddr(&hdr->full[s]), (armed_parity >> s) & 1u, c2, ST_TIMEOUT_DRAIN);
   }
   __syncwarp();
 }
 
+// A warp's (m, l, O) to shared memory, slot of four.
+template <int kD, int kNt>
+__device__ __forceinline__ void put_result(float* red_o, float* red_m, float* red_l, int slot, int g, int t,
+                                          const float (&o)[kNt][kD / 16][4], const float (&m)[kNt][2],
+                                          const float (&l)[kNt][2]) {
+  constexpr int kHeads = 8 * kNt;
+#pragma unroll
+  for (int n = 0; n < kNt; ++n) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      float x = l[n][h];
+      x += __shfl_xor_sync(0xffffffffu, x, 4);
+      x += __shfl_xor_sync(0xffffffffu, x, 8);
+      x += __shfl_xor_sync(0xffffffffu, x, 16);
+      const int head = 8 * n + 2 * t + h;
+      if (g == 0) {
+        red_m[slot * kHeads + head] = m[n][h];
+        red_l[slot * kHeads + head] = x;
+      }
+      float* dst = red_o + (slot * kHeads + head) * kD + 2 * g;
+#pragma unroll
+      for (int c = 0; c < kD / 16; ++c) *reinterpret_cast<float2*>(dst + 16 * c) = make_float2(o[n][c][h], o[n][c][2 + h]);
+    }
+  }
+}
+
 template <int kD, int kNt>
 __device__ __forceinline__ void dc_consume(const DecodeParams& p, DcHeader* hdr, uint32_t ring, float* red, Walk w,
                                           const WaitCtl& ctl, int warp, int lane) {
-  constexpr int kChunks = kD / 16, kHeads = 8 * kNt, kStages = dc_stages(kD, kHeads);
-  constexpr uint32_t kHalf = kDcTile * kD;
+  constexpr int kChunks = kD / 16, kHeads = 8 * kNt, kSlots = dc_slots(kD, kHeads);
   const int g = lane >> 2, t = lane & 3;
-  // ldmatrix addresses inside a 16-token slice: lane's row and 16-byte chunk.
-  // K: matrices (tokens 0-7, 8-15) x (chunk c, c + 1); V the same.
-  const int row = (lane & 7) + ((lane >> 3) & 1) * 8, cadd = lane >> 4;
-  const int srow = 16 * warp + row;
-  const int swz = kD == 128 ? (srow & 7) : ((srow >> 1) & 3);
-  const uint32_t row_at = static_cast<uint32_t>(srow) * kD;
+  // ldmatrix: lane's row in a 16-token slice and its 16-byte chunk, swizzled.
+  // Matrices: (tokens 0-7, 8-15) x (chunk c, c + 1); chunk c is c * 16 exclusive-or
+  // this address.
+  const int row = (lane & 7) + ((lane >> 3) & 1) * 8;
+  const int swz = kD == 128 ? (row & 7) : ((row >> 1) & 3);
+  const uint32_t first = static_cast<uint32_t>((16 * kDcSlices * warp + row) * kD + (((lane >> 4) ^ swz) << 4));
   float* red_o = red;                            // [4][kHeads][kD]
   float* red_m = red + 4 * kHeads * kD;          // [4][kHeads]
   float* red_l = red_m + 4 * kHeads;
-  int64_t it = 0;
+  int slot = 0;
+  uint32_t phase = 0;
   bool ok = true;
   Piece pc;
   while (next_piece(p, w, pc)) {
@@ -298,45 +322,81 @@ __device__ __forceinline__ void dc_consume(const DecodeParams& p, DcHeader* hdr,
 #pragma unroll
       for (int c = 0; c < kChunks; ++c) o[n][c][0] = o[n][c][1] = o[n][c][2] = o[n][c][3] = 0.f;
     }
+    auto wait_slot = [&]() {
+      return __all_sync(0xffffffffu, mbar_wait_bounded(baddr(&hdr->full[slot]), phase, ctl, ST_TIMEOUT_EPILOGUE));
+    };
+    auto free_slot = [&]() {
+      __syncwarp();
+      mbar_arrive_pred(baddr(&hdr->empty[slot]), lane == 0);
+      if (++slot == kSlots) slot = 0, phase ^= 1u;
+    };
 #pragma unroll 1
-    for (int k = 0; k < pc.n && ok; ++k, ++it) {
-      const int st = static_cast<int>(it % kStages);
-      ok = __all_sync(0xffffffffu, mbar_wait_bounded(baddr(&hdr->full[st]), static_cast<uint32_t>((it / kStages) & 1),
-                                                     ctl, ST_TIMEOUT_EPILOGUE));
+    for (int k = 0; k < pc.n && ok; ++k) {
+      const int left = len - (pc.tile0 + k) * kDcTile - 16 * kDcSlices * warp;  // tokens of this warp
+      ok = wait_slot();
       if (!ok) break;
-      const int left = len - (pc.tile0 + k) * kDcTile - 16 * warp;  // tokens of this warp's slice
-      if (left > 0) {
-        const uint32_t kb = ring + st * dc_stage_bytes(kD) + row_at, vb = kb + kHalf;
-        const float ks = hdr->scales[st][warp], vs = hdr->scales[st][4 + warp];
-        float s[kNt][4];
-#pragma unroll
-        for (int n = 0; n < kNt; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
-#pragma unroll
-        for (int c = 0; c < kChunks; c += 2) {
-          uint32_t r[4];  // (tokens 0-7, chunk c), (8-15, c), (0-7, c + 1), (8-15, c + 1)
-          ldmatrix4(kb + static_cast<uint32_t>(((c + cadd) ^ swz) << 4), r);
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            uint32_t a0, a1, a2, a3;
-            codes_to_half(r[2 * i], a0, a2);
-            codes_to_half(r[2 * i + 1], a1, a3);
-#pragma unroll
-            for (int n = 0; n < kNt; ++n) mma16816(s[n], a0, a1, a2, a3, q[n][c + i][0], q[n][c + i][1]);
-          }
-        }
-        // s[n]: tokens g and g + 8 (rows) of heads 2 t, 2 t + 1 (columns)
-        const float eb = static_cast<float>(static_cast<int>(__float_as_uint(vs) >> 23) - 127), vs_inv = 1.f / vs;
-        const bool in0 = g < left, in1 = g + 8 < left;
+      if (left <= 0) {
+        free_slot();
+        ok = wait_slot();
+        if (!ok) break;
+      } else {
+        const uint32_t kb = ring + slot * dc_slot_bytes(kD) + first;
+        const float* k_scales = hdr->scales[slot] + kDcSlices * warp;
+        float s[kDcSlices][kNt][4], vs_inv[kDcSlices];
         bool grow = false;
         float mx[kNt][2];
+#pragma unroll
+        for (int n = 0; n < kNt; ++n) mx[n][0] = mx[n][1] = -INFINITY;
+#pragma unroll
+        for (int sl = 0; sl < kDcSlices; ++sl) {
+#pragma unroll
+          for (int n = 0; n < kNt; ++n) s[sl][n][0] = s[sl][n][1] = s[sl][n][2] = s[sl][n][3] = 0.f;
+#pragma unroll
+          for (int c = 0; c < kChunks; c += 2) {
+            uint32_t r[4];  // (tokens 0-7, chunk c), (8-15, c), (0-7, c + 1), (8-15, c + 1)
+            ldmatrix4((kb ^ (c << 4)) + sl * 16 * kD, r);
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              uint32_t a0, a1, a2, a3;
+              codes_to_half(r[2 * i], a0, a2);
+              codes_to_half(r[2 * i + 1], a1, a3);
+#pragma unroll
+              for (int n = 0; n < kNt; ++n) mma16816(s[sl][n], a0, a1, a2, a3, q[n][c + i][0], q[n][c + i][1]);
+            }
+          }
+          // s[sl][n]: tokens g and g + 8 (rows) of heads 2 t, 2 t + 1 (columns)
+#pragma unroll
+          for (int n = 0; n < kNt; ++n) {
+#pragma unroll
+            for (int h = 0; h < 4; ++h) s[sl][n][h] *= qs[n][h & 1] * k_scales[sl];
+          }
+        }
+        free_slot();
+        ok = wait_slot();
+        if (!ok) break;
+        const uint32_t vb = ring + slot * dc_slot_bytes(kD) + first;
+        const float* v_scales = hdr->scales[slot] + kDcSlices * warp;
+#pragma unroll
+        for (int sl = 0; sl < kDcSlices; ++sl) {
+          const float vs = v_scales[sl];
+          const float eb = static_cast<float>(static_cast<int>(__float_as_uint(vs) >> 23) - 127);
+          vs_inv[sl] = __uint_as_float((254u << 23) - __float_as_uint(vs));  // 2^-b of vs = 2^b
+          const bool in0 = 16 * sl + g < left, in1 = 16 * sl + g + 8 < left;
+#pragma unroll
+          for (int n = 0; n < kNt; ++n) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              s[sl][n][h] = in0 ? s[sl][n][h] + eb : -INFINITY;
+              s[sl][n][2 + h] = in1 ? s[sl][n][2 + h] + eb : -INFINITY;
+              mx[n][h] = fmaxf(mx[n][h], fmaxf(s[sl][n][h], s[sl][n][2 + h]));
+            }
+          }
+        }
 #pragma unroll
         for (int n = 0; n < kNt; ++n) {
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            const float f = qs[n][h] * ks;
-            s[n][h] = in0 ? fmaf(s[n][h], f, eb) : -INFINITY;
-            s[n][2 + h] = in1 ? fmaf(s[n][2 + h], f, eb) : -INFINITY;
-            float x = fmaxf(s[n][h], s[n][2 + h]);
+            float x = mx[n][h];
             x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
             x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
             x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
@@ -361,66 +421,52 @@ __device__ __forceinline__ void dc_consume(const DecodeParams& p, DcHeader* hdr,
             }
           }
         }
-        uint32_t pb[kNt][2];
-#pragma unroll
-        for (int n = 0; n < kNt; ++n) {
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const float mm = m[n][h] == -INFINITY ? 0.f : m[n][h];
-            s[n][h] = ex2(s[n][h] - mm);
-            s[n][2 + h] = ex2(s[n][2 + h] - mm);
-            l[n][h] += (s[n][h] + s[n][2 + h]) * vs_inv;
-          }
-          pb[n][0] = transpose8(half_pair(s[n][0], s[n][1]));  // B: tokens 2 t, 2 t + 1 of head g
-          pb[n][1] = transpose8(half_pair(s[n][2], s[n][3]));  // tokens 2 t + 8, 2 t + 9
-        }
         // Codes behind the last token are whatever the page held: clear them
         // (0 times a NaN code would not be 0).
-        const bool tail = left < 16;
-        uint32_t keep0 = ~0u, keep1 = ~0u;
-        if (tail) {
-          keep0 = (2 * t < left ? 0xFFFFu : 0u) | (2 * t + 1 < left ? 0xFFFF0000u : 0u);
-          keep1 = (2 * t + 8 < left ? 0xFFFFu : 0u) | (2 * t + 9 < left ? 0xFFFF0000u : 0u);
-        }
+        const bool tail = left < 16 * kDcSlices;
 #pragma unroll
-        for (int c = 0; c < kChunks; c += 2) {
-          uint32_t r[4];
-          ldmatrix4t(vb + static_cast<uint32_t>(((c + cadd) ^ swz) << 4), r);
+        for (int sl = 0; sl < kDcSlices; ++sl) {
+          uint32_t pb[kNt][2];
 #pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            // register: codes (token 2 t, d 2 g), (2 t, 2 g + 1), (2 t + 1, 2 g), (2 t + 1, 2 g + 1)
-            uint32_t a0, a1, a2, a3;  // rows 0-7 of A: even d, rows 8-15: odd d
-            codes_to_half(__byte_perm(r[2 * i], 0, 0x3120), a0, a1);
-            codes_to_half(__byte_perm(r[2 * i + 1], 0, 0x3120), a2, a3);
-            if (tail) a0 &= keep0, a1 &= keep0, a2 &= keep1, a3 &= keep1;
+          for (int n = 0; n < kNt; ++n) {
 #pragma unroll
-            for (int n = 0; n < kNt; ++n) mma16816(o[n][c + i], a0, a1, a2, a3, pb[n][0], pb[n][1]);
+            for (int h = 0; h < 2; ++h) {
+              const float mm = m[n][h] == -INFINITY ? 0.f : m[n][h];
+              s[sl][n][h] = ex2(s[sl][n][h] - mm);
+              s[sl][n][2 + h] = ex2(s[sl][n][2 + h] - mm);
+              l[n][h] += (s[sl][n][h] + s[sl][n][2 + h]) * vs_inv[sl];
+            }
+            pb[n][0] = transpose8(half_pair(s[sl][n][0], s[sl][n][1]));  // B: tokens 2 t, 2 t + 1 of head g
+            pb[n][1] = transpose8(half_pair(s[sl][n][2], s[sl][n][3]));  // tokens 2 t + 8, 2 t + 9
+          }
+          uint32_t keep0 = ~0u, keep1 = ~0u;
+          if (tail) {
+            const int at = left - 16 * sl - 2 * t;
+            keep0 = (0 < at ? 0xFFFFu : 0u) | (1 < at ? 0xFFFF0000u : 0u);
+            keep1 = (8 < at ? 0xFFFFu : 0u) | (9 < at ? 0xFFFF0000u : 0u);
+          }
+#pragma unroll
+          for (int c = 0; c < kChunks; c += 2) {
+            uint32_t r[4];
+            ldmatrix4t((vb ^ (c << 4)) + sl * 16 * kD, r);
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              // register: codes (token 2 t, d 2 g), (2 t, 2 g + 1), (2 t + 1, 2 g), (2 t + 1, 2 g + 1)
+              uint32_t a0, a1, a2, a3;  // rows 0-7 of A: even d, rows 8-15: odd d
+              codes_to_half(__byte_perm(r[2 * i], 0, 0x3120), a0, a1);
+              codes_to_half(__byte_perm(r[2 * i + 1], 0, 0x3120), a2, a3);
+              if (tail) a0 &= keep0, a1 &= keep0, a2 &= keep1, a3 &= keep1;
+#pragma unroll
+              for (int n = 0; n < kNt; ++n) mma16816(o[n][c + i], a0, a1, a2, a3, pb[n][0], pb[n][1]);
+            }
           }
         }
       }
-      __syncwarp();
-      if (lane == 0) mbar_arrive(baddr(&hdr->empty[st]));
+      free_slot();
     }
     // ---- the four warps' results of this piece
     consumers_sync();  // the last piece's have been read
-#pragma unroll
-    for (int n = 0; n < kNt; ++n) {
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        float x = l[n][h];
-        x += __shfl_xor_sync(0xffffffffu, x, 4);
-        x += __shfl_xor_sync(0xffffffffu, x, 8);
-        x += __shfl_xor_sync(0xffffffffu, x, 16);
-        const int head = 8 * n + 2 * t + h;
-        if (g == 0) {
-          red_m[warp * kHeads + head] = m[n][h];
-          red_l[warp * kHeads + head] = x;
-        }
-        float* dst = red_o + (warp * kHeads + head) * kD + 2 * g;
-#pragma unroll
-        for (int c = 0; c < kChunks; ++c) *reinterpret_cast<float2*>(dst + 16 * c) = make_float2(o[n][c][h], o[n][c][2 + h]);
-      }
-    }
+    put_result<kD, kNt>(red_o, red_m, red_l, warp, g, t, o, m, l);
     consumers_sync();
     const int tid = 32 * warp + lane;
     const bool whole = pc.n == pc.tiles;
@@ -494,17 +540,17 @@ __device__ __forceinline__ void dc_consume(const DecodeParams& p, DcHeader* hdr,
 }
 
 template <int kD, int kNt>
-__global__ void __launch_bounds__(kDcThreads) decode_kernel(const __grid_constant__ DecodeParams p) {
+__global__ void __launch_bounds__(kDcThreads, dc_per_sm(8 * kNt)) decode_kernel(const __grid_constant__ DecodeParams p) {
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   const uint32_t raw = smem_u32(smem_raw), base = (raw + 1023u) & ~1023u;
   uint8_t* gbase = smem_raw + (base - raw);
   DcHeader* hdr = reinterpret_cast<DcHeader*>(gbase);
   const uint32_t ring = base + 1024u;
-  constexpr int kStages = dc_stages(kD, 8 * kNt);
-  float* red = reinterpret_cast<float*>(gbase + 1024 + kStages * dc_stage_bytes(kD));
+  constexpr int kSlots = dc_slots(kD, 8 * kNt);
+  float* red = reinterpret_cast<float*>(gbase + 1024 + kSlots * dc_slot_bytes(kD));
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (warp == 0 && lane == 0) {
-    for (int s = 0; s < kStages; ++s) {
+    for (int s = 0; s < kSlots; ++s) {
       mbar_init(baddr(&hdr->full[s]), 1);
       mbar_init(baddr(&hdr->empty[s]), 4);
     }
@@ -522,10 +568,10 @@ __global__ void __launch_bounds__(kDcThreads) decode_kernel(const __grid_constan
     }
     for (int k = 16; k; k >>= 1) total += __shfl_xor_sync(0xffffffffu, total, k);
     total *= p.streams;
-    // at least two tiles to a CTA and at most 64 parts to a row on average: past
+    // at least a tile to a CTA and at most 64 parts to a row on average: past
     // that the joining costs more than the reading
     const int64_t rows = static_cast<int64_t>(p.n_seqs) * p.streams;
-    const int ctas = static_cast<int>(min(static_cast<int64_t>(gridDim.x), min((total + 1) / 2, 64 * rows)));
+    const int ctas = static_cast<int>(min(static_cast<int64_t>(gridDim.x), min(total, 64 * rows)));
     const int64_t g0 = ctas > 0 ? blockIdx.x * total / ctas : 0;
     int64_t at = 0;
     int seq = 0;
@@ -570,7 +616,7 @@ __global__ void __launch_bounds__(kDcThreads) decode_kernel(const __grid_constan
   w.seq = hdr->seq;
   w.tiles = dc_tiles(p, w.seq);
   const WaitCtl ctl{&hdr->abort_flag, p.status, p.timeout_ns};
-  if (warp == kDcTmaWarp) dc_produce<kD, kStages>(p, hdr, ring, w, ctl, lane);
+  if (warp == kDcTmaWarp) dc_produce<kD, kSlots>(p, hdr, ring, w, ctl, lane);
   else dc_consume<kD, kNt>(p, hdr, ring, red, w, ctl, warp, lane);
 }
 
@@ -594,8 +640,7 @@ DecodeKernel pick(int d, int group) {
 
 int64_t decode_work_floats(int32_t ctas, int32_t d) { return 2 * static_cast<int64_t>(ctas) * 16 * (d + 2); }
 
-// Two CTAs fit an SM (shared memory).
-int32_t decode_ctas(const bsp_device* dev) { return 2 * dev->sm_count; }
+int32_t decode_ctas(const bsp_device* dev, int group) { return dc_per_sm(group > 8 ? 16 : 8) * dev->sm_count; }
 
 int decode_smem_bytes(int d, int group) { return dc_smem(d, group > 8 ? 16 : 8); }
 
