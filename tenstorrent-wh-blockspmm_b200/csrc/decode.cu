@@ -43,14 +43,15 @@ namespace {
 
 constexpr int kDcSlices = 2;             // of 16 tokens that a warp takes of a tile
 constexpr int kDcTile = 64 * kDcSlices;  // tokens
-constexpr int kDcThreads = 160;
-constexpr int kDcTmaWarp = 4;
+constexpr int kDcThreads = 192;
+constexpr int kDcTmaWarp = 4;  // K; the next one V
 constexpr int kDcMaxSlots = 12;
+constexpr int kDcJoin = 8;
 constexpr float kDcRescale = 8.f;    // log2 of the growth that moves the maximum
 
 struct DcHeader {
   uint64_t full[kDcMaxSlots], empty[kDcMaxSlots];
-  int64_t tiles, base;  // tiles of all rows; first tile of sequence `seq`
+  int32_t tiles, base;  // tiles of all rows; first tile of sequence `seq`
   int32_t seq;
   int32_t ctas;         // CTAs that take part
   int32_t last;         // this CTA joins the row
@@ -141,44 +142,47 @@ __device__ __forceinline__ int dc_len(const DecodeParams& p, int s) {
 }
 __device__ __forceinline__ int dc_tiles(const DecodeParams& p, int s) { return (dc_len(p, s) + kDcTile - 1) / kDcTile; }
 
-// A CTA's way through its stretch [g, g1) of the list of tiles.
+// A CTA's way through its stretch [g, g1) of the list of tiles (under 2^31 in
+// all: 2^38 tokens).
 struct Walk {
-  int64_t g, g1, base;
+  int32_t g, g1, base;
   int seq, tiles;  // of the current sequence
 };
 struct Piece {
   int seq, stream, tile0, n, tiles;  // tiles [tile0, tile0 + n) of the row's `tiles`
-  int64_t row0;                      // the row's first tile in the list
+  int32_t row0;                      // the row's first tile in the list
 };
 __device__ __forceinline__ bool next_piece(const DecodeParams& p, Walk& w, Piece& pc) {
   if (w.g >= w.g1) return false;
-  while (w.g >= w.base + static_cast<int64_t>(w.tiles) * p.streams) {
-    w.base += static_cast<int64_t>(w.tiles) * p.streams;
+  while (w.g - w.base >= w.tiles * p.streams) {
+    w.base += w.tiles * p.streams;
     if (++w.seq >= p.n_seqs) return false;
     w.tiles = dc_tiles(p, w.seq);
   }
-  const int64_t rel = w.g - w.base;
+  const uint32_t rel = static_cast<uint32_t>(w.g - w.base);
   pc.seq = w.seq;
   pc.tiles = w.tiles;
-  pc.stream = static_cast<int>(rel / w.tiles);
-  pc.tile0 = static_cast<int>(rel - static_cast<int64_t>(pc.stream) * w.tiles);
-  pc.n = static_cast<int>(min(static_cast<int64_t>(w.tiles - pc.tile0), w.g1 - w.g));
-  pc.row0 = w.base + static_cast<int64_t>(pc.stream) * w.tiles;
+  pc.stream = static_cast<int>(rel / static_cast<uint32_t>(w.tiles));
+  pc.tile0 = static_cast<int>(rel) - pc.stream * w.tiles;
+  pc.n = min(w.tiles - pc.tile0, w.g1 - w.g);
+  pc.row0 = w.base + pc.stream * w.tiles;
   w.g += pc.n;
   return true;
 }
 
 template <int kD, int kSlots>
 __device__ __forceinline__ void dc_produce(const DecodeParams& p, DcHeader* hdr, uint32_t ring, Walk w,
-                                          const WaitCtl& ctl, int lane) {
+                                          const WaitCtl& ctl, int kind, int lane) {
   const int page = p.cache.page, shift = __ffs(page) - 1;  // a power of two
   const int box = min(page, kDcTile), boxes = kDcTile / box;  // per tile and operand
-  const int kind = lane >> 4, at = (lane & 15) / boxes, sub = (lane & 15) % boxes;
-  const int per_batch = 16 / boxes;
+  const int shift_b = __ffs(boxes) - 1;
+  const int at = lane >> shift_b, sub = lane & (boxes - 1);  // lane's tile of a batch, its box
+  const int per_batch = 32 >> shift_b;
   const float* scale = kind ? p.cache.v_scale : p.cache.k_scale;
   const CUtensorMap* tm = kind ? &p.tm_v : &p.tm_k;
-  int slot = 0;
-  uint32_t phase = 0, armed = 0, armed_parity = 0;
+  int slot = kind;  // K of the first tile has slot 0, V slot 1, K of the next 2 ...
+  uint32_t phase = 0;
+  int done = 0;  // tiles
   bool ok = true;
   Piece pc;
   while (ok && next_piece(p, w, pc)) {
@@ -206,31 +210,37 @@ __device__ __forceinline__ void dc_produce(const DecodeParams& p, DcHeader* hdr,
       const float sc_next = scale_of(idn);
       const int n = min(per_batch, pc.n - b);
 #pragma unroll 1
-      for (int k = 0; k < 2 * n; ++k) {  // K, then V of each tile
+      for (int k = 0; k < n; ++k) {
         ok = __all_sync(0xffffffffu, mbar_wait_bounded(baddr(&hdr->empty[slot]), phase ^ 1u, ctl, ST_TIMEOUT_PRODUCER));
         if (!ok) break;
-        const bool now = 2 * at + kind == k, mine = now && id != -2;
-        if (now)
+        const bool mine = at == k && id != -2;
+        const uint32_t bar = baddr(&hdr->full[slot]);
+        // The copies go first: their scales may still be on the way.
+        tma_load_4d_pred(ring + slot * dc_slot_bytes(kD) + sub * box * kD, tm, 0, 0, kvh,
+                         id >= 0 ? id : static_cast<int32_t>(p.cache.n_pages), bar, mine);
+        if (at == k)
           for (int i = 0; i < box / 16; ++i) hdr->scales[slot][sub * (box / 16) + i] = sc;
         const uint32_t bytes = static_cast<uint32_t>(__popc(__ballot_sync(0xffffffffu, mine))) * box * kD;
         __syncwarp();  // the scales are written before lane 0 arrives
-        const uint32_t bar = baddr(&hdr->full[slot]);
         mbar_arrive_expect_tx_pred(bar, bytes, lane == 0);
-        tma_load_4d_pred(ring + slot * dc_slot_bytes(kD) + sub * box * kD, tm, 0, 0, kvh,
-                         id >= 0 ? id : static_cast<int32_t>(p.cache.n_pages), bar, mine);
-        armed |= 1u << slot;
-        armed_parity = (armed_parity & ~(1u << slot)) | (phase << slot);
-        if (++slot == kSlots) slot = 0, phase ^= 1u;
+        ++done;
+        slot += 2;
+        if (slot >= kSlots) slot -= kSlots, phase ^= 1u;
       }
       id = idn;
       sc = sc_next;
     }
   }
-  if (lane == 0) {  // no copy may be in flight when the CTA leaves
+  if (lane == 0) {
+    // No copy may be in flight when the CTA leaves: wait for the last round of
+    // slots (one that was filled again since has been consumed).
     int zero = 0;
     const WaitCtl c2{&zero, ctl.status, ctl.timeout_ns};
-    for (int s = 0; s < kSlots; ++s)
-      if (armed & (1u << s)) mbar_wait_bounded(baddr(&hdr->full[s]), (armed_parity >> s) & 1u, c2, ST_TIMEOUT_DRAIN);
+    for (int i = max(0, done - (kSlots + 1) / 2); i < done; ++i) {
+      const int at = 2 * i + kind;
+      if (at + kSlots >= 2 * done)
+        mbar_wait_bounded(baddr(&hdr->full[at % kSlots]), static_cast<uint32_t>(at / kSlots) & 1u, c2, ST_TIMEOUT_DRAIN);
+    }
   }
   __syncwarp();
 }
@@ -239,7 +249,7 @@ __device__ __forceinline__ void dc_produce(const DecodeParams& p, DcHeader* hdr,
 template <int kD, int kNt>
 __device__ __forceinline__ void put_result(float* red_o, float* red_m, float* red_l, int slot, int g, int t,
                                           const float (&o)[kNt][kD / 16][4], const float (&m)[kNt][2],
-                                          const float (&l)[kNt][2]) {
+                                          const float (&l)[kNt][2], int nh) {
   constexpr int kHeads = 8 * kNt;
 #pragma unroll
   for (int n = 0; n < kNt; ++n) {
@@ -255,8 +265,9 @@ __device__ __forceinline__ void put_result(float* red_o, float* red_m, float* re
         red_l[slot * kHeads + head] = x;
       }
       float* dst = red_o + (slot * kHeads + head) * kD + 2 * g;
+      if (head < nh)
 #pragma unroll
-      for (int c = 0; c < kD / 16; ++c) *reinterpret_cast<float2*>(dst + 16 * c) = make_float2(o[n][c][h], o[n][c][2 + h]);
+        for (int c = 0; c < kD / 16; ++c) *reinterpret_cast<float2*>(dst + 16 * c) = make_float2(o[n][c][h], o[n][c][2 + h]);
     }
   }
 }
@@ -466,12 +477,19 @@ __device__ __forceinline__ void dc_consume(const DecodeParams& p, DcHeader* hdr,
     }
     // ---- the four warps' results of this piece
     consumers_sync();  // the last piece's have been read
-    put_result<kD, kNt>(red_o, red_m, red_l, warp, g, t, o, m, l);
+    put_result<kD, kNt>(red_o, red_m, red_l, warp, g, t, o, m, l, nh);
     consumers_sync();
     const int tid = 32 * warp + lane;
     const bool whole = pc.n == pc.tiles;
     const int64_t slot_floats = 16 * (kD + 2);
     float* ws = p.work + (2 * static_cast<int64_t>(blockIdx.x) + (pc.tile0 == 0 ? 1 : 0)) * slot_floats;
+    auto put_o = [&](int head, int col, float4 a, float M, float L) {
+      const float inv = 1.f / L;
+      uint16_t* dst = static_cast<uint16_t*>(p.o.p) + pc.seq * p.o.token + (h0 + head) * p.o.head + 4 * col;
+      *reinterpret_cast<uint2*>(dst) = make_uint2(bf16_two(a.x * inv, a.y * inv), bf16_two(a.z * inv, a.w * inv));
+      if (col == 0 && p.lse)
+        p.lse[static_cast<int64_t>(pc.seq) * p.heads + h0 + head] = (M + log2f(L)) * 0.6931471805599453f;
+    };
     for (int i = tid; i < nh * (kD / 4); i += 128) {
       const int head = i / (kD / 4), col = i % (kD / 4);
       float M = red_m[head];
@@ -487,11 +505,7 @@ __device__ __forceinline__ void dc_consume(const DecodeParams& p, DcHeader* hdr,
         L += f * red_l[k * kHeads + head];
       }
       if (whole) {
-        const float inv = 1.f / L;
-        uint16_t* dst = static_cast<uint16_t*>(p.o.p) + pc.seq * p.o.token + (h0 + head) * p.o.head + 4 * col;
-        *reinterpret_cast<uint2*>(dst) = make_uint2(bf16_two(a.x * inv, a.y * inv), bf16_two(a.z * inv, a.w * inv));
-        if (col == 0 && p.lse)
-          p.lse[static_cast<int64_t>(pc.seq) * p.heads + h0 + head] = (M + log2f(L)) * 0.6931471805599453f;
+        put_o(head, col, a, M, L);
       } else {
         __stcg(reinterpret_cast<float4*>(ws + head * kD) + col, a);
         if (col == 0) {
@@ -502,40 +516,52 @@ __device__ __forceinline__ void dc_consume(const DecodeParams& p, DcHeader* hdr,
     }
     if (whole) continue;
     // ---- a part of a row: the last of its CTAs joins the parts
-    const int64_t tiles = hdr->tiles;
-    const int first = static_cast<int>(((pc.row0 + 1) * hdr->ctas - 1) / tiles);
-    const int last = static_cast<int>(((pc.row0 + pc.tiles) * hdr->ctas - 1) / tiles);
-    const int parts = last - first + 1;
-    __threadfence();
-    consumers_sync();
-    if (tid == 0) hdr->last = atomicAdd(p.counters + first, 1) == parts - 1 ? 1 : 0;
+    const uint32_t tiles = hdr->tiles;
+    const int first_cta = static_cast<int>((static_cast<uint64_t>(pc.row0 + 1) * hdr->ctas - 1) / tiles);
+    const int last_cta = static_cast<int>((static_cast<uint64_t>(pc.row0 + pc.tiles) * hdr->ctas - 1) / tiles);
+    const int parts = last_cta - first_cta + 1;
+    consumers_sync();  // all of this part is written: the release below covers it
+    if (tid == 0) {
+      int before;
+      asm volatile("atom.acq_rel.gpu.global.add.s32 %0, [%1], 1;"
+                   : "=r"(before) : "l"(p.counters + first_cta) : "memory");
+      hdr->last = before == parts - 1 ? 1 : 0;
+    }
     consumers_sync();
     if (!hdr->last) continue;
-    __threadfence();
-    const float* first_ws = p.work + (2 * static_cast<int64_t>(first) + 1) * slot_floats;
-    auto part_ws = [&](int k) { return k == 0 ? first_ws : p.work + 2 * static_cast<int64_t>(first + k) * slot_floats; };
+    const float* first_ws = p.work + (2 * static_cast<int64_t>(first_cta) + 1) * slot_floats;
     for (int i = tid; i < nh * (kD / 4); i += 128) {
       const int head = i / (kD / 4), col = i % (kD / 4);
-      float M = -INFINITY;
-      for (int k = 0; k < parts; ++k) M = fmaxf(M, __ldcg(part_ws(k) + 16 * kD + head));
       float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-      float L = 0.f;
-#pragma unroll 4
-      for (int k = 0; k < parts; ++k) {
-        const float* src = part_ws(k);
-        const float mk = __ldcg(src + 16 * kD + head);
-        const float f = mk == -INFINITY ? 1.f : ex2(mk - M);
-        const float4 v = __ldcg(reinterpret_cast<const float4*>(src + head * kD) + col);
-        a.x += f * v.x, a.y += f * v.y, a.z += f * v.z, a.w += f * v.w;
-        L += f * __ldcg(src + 16 * kD + 16 + head);
+      float M = -INFINITY, L = 0.f;
+      for (int k0 = 0; k0 < parts; k0 += kDcJoin) {  // kDcJoin parts a round trip to L2
+        float4 v[kDcJoin];
+        float mk[kDcJoin], lk[kDcJoin];
+#pragma unroll
+        for (int k = 0; k < kDcJoin; ++k) {
+          const bool have = k0 + k < parts;
+          const float* src = k0 + k == 0 ? first_ws : p.work + 2 * static_cast<int64_t>(first_cta + k0 + k) * slot_floats;
+          v[k] = have ? __ldcg(reinterpret_cast<const float4*>(src + head * kD) + col) : make_float4(0.f, 0.f, 0.f, 0.f);
+          mk[k] = have ? __ldcg(src + 16 * kD + head) : -INFINITY;
+          lk[k] = have ? __ldcg(src + 16 * kD + 16 + head) : 0.f;
+        }
+        float top = M;
+#pragma unroll
+        for (int k = 0; k < kDcJoin; ++k) top = fmaxf(top, mk[k]);
+        const float f0 = M == -INFINITY ? 1.f : ex2(M - top);
+        a.x *= f0, a.y *= f0, a.z *= f0, a.w *= f0;
+        L *= f0;
+        M = top;
+#pragma unroll
+        for (int k = 0; k < kDcJoin; ++k) {
+          const float f = mk[k] == -INFINITY ? 1.f : ex2(mk[k] - top);
+          a.x += f * v[k].x, a.y += f * v[k].y, a.z += f * v[k].z, a.w += f * v[k].w;
+          L += f * lk[k];
+        }
       }
-      const float inv = 1.f / L;
-      uint16_t* dst = static_cast<uint16_t*>(p.o.p) + pc.seq * p.o.token + (h0 + head) * p.o.head + 4 * col;
-      *reinterpret_cast<uint2*>(dst) = make_uint2(bf16_two(a.x * inv, a.y * inv), bf16_two(a.z * inv, a.w * inv));
-      if (col == 0 && p.lse)
-        p.lse[static_cast<int64_t>(pc.seq) * p.heads + h0 + head] = (M + log2f(L)) * 0.6931471805599453f;
+      put_o(head, col, a, M, L);
     }
-    if (tid == 0) p.counters[first] = 0;  // ready for the next launch
+    if (tid == 0) p.counters[first_cta] = 0;  // ready for the next launch
   }
 }
 
@@ -560,38 +586,38 @@ __global__ void __launch_bounds__(kDcThreads, dc_per_sm(8 * kNt)) decode_kernel(
   if (warp == kDcTmaWarp) {
     if (lane < 2) tma_prefetch_desc(lane ? &p.tm_v : &p.tm_k);
     // tiles of all rows, then the sequence in which this CTA's stretch begins
-    int64_t total = 0;
-    for (int s = lane; s < p.n_seqs; s += 32) {
-      const int len = __ldg(p.lens + s);
-      if (blockIdx.x == 0 && (len < 0 || len > p.table_width * p.cache.page)) atomicOr(p.status, ST_BAD_INDEX);
-      total += dc_tiles(p, s);
-    }
+    const int first = lane < p.n_seqs ? dc_tiles(p, lane) : 0;
+    int64_t total = first;
+    for (int s = lane + 32; s < p.n_seqs; s += 32) total += dc_tiles(p, s);
     for (int k = 16; k; k >>= 1) total += __shfl_xor_sync(0xffffffffu, total, k);
     total *= p.streams;
+    if (total > 0x7FFFFFFF) {
+      if (lane == 0) atomicOr(p.status, ST_BAD_INDEX);
+      total = 0;
+    }
     // at least a tile to a CTA and at most 64 parts to a row on average: past
     // that the joining costs more than the reading
     const int64_t rows = static_cast<int64_t>(p.n_seqs) * p.streams;
     const int ctas = static_cast<int>(min(static_cast<int64_t>(gridDim.x), min(total, 64 * rows)));
-    const int64_t g0 = ctas > 0 ? blockIdx.x * total / ctas : 0;
-    int64_t at = 0;
-    int seq = 0;
+    const int g0 = ctas > 0 ? static_cast<int>(blockIdx.x * total / ctas) : 0;
+    int at = 0, seq = 0;
     bool found = false;
     for (int s0 = 0; s0 < p.n_seqs && !found; s0 += 32) {
-      const int64_t mine = s0 + lane < p.n_seqs ? static_cast<int64_t>(dc_tiles(p, s0 + lane)) * p.streams : 0;
-      int64_t upto = mine;
+      const int mine = (s0 == 0 ? first : s0 + lane < p.n_seqs ? dc_tiles(p, s0 + lane) : 0) * p.streams;
+      int upto = mine;
       for (int k = 1; k < 32; k <<= 1) {
-        const int64_t x = __shfl_up_sync(0xffffffffu, upto, k);
+        const int x = __shfl_up_sync(0xffffffffu, upto, k);
         if (lane >= k) upto += x;
       }
       const unsigned past = __ballot_sync(0xffffffffu, at + upto > g0);
       found = past != 0;
       const int src = found ? __ffs(past) - 1 : 31;
-      const int64_t incl = __shfl_sync(0xffffffffu, upto, src), own = __shfl_sync(0xffffffffu, mine, src);
+      const int incl = __shfl_sync(0xffffffffu, upto, src), own = __shfl_sync(0xffffffffu, mine, src);
       seq = s0 + src;
       at += found ? incl - own : incl;
     }
     if (lane == 0) {
-      hdr->tiles = total;
+      hdr->tiles = static_cast<int32_t>(total);
       hdr->ctas = ctas;
       hdr->seq = seq;
       hdr->base = at;
@@ -601,6 +627,7 @@ __global__ void __launch_bounds__(kDcThreads, dc_per_sm(8 * kNt)) decode_kernel(
   // sequences without a token: O = 0, lse = -inf
   for (int s = blockIdx.x; s < p.n_seqs; s += gridDim.x) {
     if (dc_len(p, s) > 0) continue;
+    if (threadIdx.x == 0 && __ldg(p.lens + s) != 0) atomicOr(p.status, ST_BAD_INDEX);
     for (int i = threadIdx.x; i < p.heads * (kD / 8); i += kDcThreads) {
       const int head = i / (kD / 8), col = i % (kD / 8);
       uint16_t* dst = static_cast<uint16_t*>(p.o.p) + s * p.o.token + head * p.o.head;
@@ -610,13 +637,13 @@ __global__ void __launch_bounds__(kDcThreads, dc_per_sm(8 * kNt)) decode_kernel(
   }
   if (static_cast<int>(blockIdx.x) >= hdr->ctas) return;
   Walk w;
-  w.g = blockIdx.x * hdr->tiles / hdr->ctas;
-  w.g1 = (blockIdx.x + 1) * hdr->tiles / hdr->ctas;
+  w.g = static_cast<int32_t>(static_cast<int64_t>(blockIdx.x) * hdr->tiles / hdr->ctas);
+  w.g1 = static_cast<int32_t>(static_cast<int64_t>(blockIdx.x + 1) * hdr->tiles / hdr->ctas);
   w.base = hdr->base;
   w.seq = hdr->seq;
   w.tiles = dc_tiles(p, w.seq);
   const WaitCtl ctl{&hdr->abort_flag, p.status, p.timeout_ns};
-  if (warp == kDcTmaWarp) dc_produce<kD, kSlots>(p, hdr, ring, w, ctl, lane);
+  if (warp >= kDcTmaWarp) dc_produce<kD, kSlots>(p, hdr, ring, w, ctl, warp - kDcTmaWarp, lane);
   else dc_consume<kD, kNt>(p, hdr, ring, red, w, ctl, warp, lane);
 }
 
