@@ -323,7 +323,7 @@ bsp_status bsp_decode_plan_create(bsp_device* dev, int32_t max_seqs, int32_t hea
   p->kv_heads = kv_heads;
   p->d = d;
   p->page = page;
-  p->grid = decode_ctas(dev, heads / kv_heads);
+  p->grid = decode_ctas(dev, d, heads / kv_heads);
   if (opts && opts->max_ctas > 0) p->grid = std::min(p->grid, opts->max_ctas);
   p->smem_bytes = decode_smem_bytes(d, heads / kv_heads);
   p->timeout_ns = static_cast<uint64_t>(opts && opts->timeout_ms > 0 ? opts->timeout_ms : 2000) * 1000000ull;

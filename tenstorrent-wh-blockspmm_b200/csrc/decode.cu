@@ -62,13 +62,15 @@ static_assert(sizeof(DcHeader) <= 1024, "header must fit its 1 KiB slot");
 
 // Shared memory from the 1 KiB-aligned base: header, slots (K and V of a tile
 // in turn), then the warps' results: O [4][heads][d], m [4][heads], l [4][heads].
-// CTAs on an SM: two, or one with rows of 16 heads (registers).
-__host__ __device__ constexpr int dc_per_sm(int heads) { return heads > 8 ? 1 : 2; }
+// CTAs on an SM: one with rows of 16 heads (registers), two for d = 128, four
+// for d = 64, whose tiles are half the bytes for the same work on scores (16
+// heads of 64 in pages of 16: 39 us with two, 32 with three, 29.5 with four).
+__host__ __device__ constexpr int dc_per_sm(int d, int heads) { return heads > 8 ? 1 : d == 64 ? 4 : 2; }
 // As many slots as fit the SM's 228 KB then (1 KB of each CTA is the system's).
 __host__ __device__ constexpr int dc_slot_bytes(int d) { return kDcTile * d; }
 __host__ __device__ constexpr int dc_result_bytes(int d, int heads) { return 16 * heads * (d + 2); }
 __host__ __device__ constexpr int dc_slots(int d, int heads) {
-  const int n = ((228 / dc_per_sm(heads) - 1) * 1024 - 2048 - dc_result_bytes(d, heads)) / dc_slot_bytes(d);
+  const int n = ((228 / dc_per_sm(d, heads) - 1) * 1024 - 2048 - dc_result_bytes(d, heads)) / dc_slot_bytes(d);
   return n < kDcMaxSlots ? n : kDcMaxSlots;
 }
 __host__ __device__ constexpr int dc_smem(int d, int heads) {
@@ -566,7 +568,7 @@ __device__ __forceinline__ void dc_consume(const DecodeParams& p, DcHeader* hdr,
 }
 
 template <int kD, int kNt>
-__global__ void __launch_bounds__(kDcThreads, dc_per_sm(8 * kNt)) decode_kernel(const __grid_constant__ DecodeParams p) {
+__global__ void __launch_bounds__(kDcThreads, dc_per_sm(kD, 8 * kNt)) decode_kernel(const __grid_constant__ DecodeParams p) {
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   const uint32_t raw = smem_u32(smem_raw), base = (raw + 1023u) & ~1023u;
   uint8_t* gbase = smem_raw + (base - raw);
@@ -667,7 +669,7 @@ DecodeKernel pick(int d, int group) {
 
 int64_t decode_work_floats(int32_t ctas, int32_t d) { return 2 * static_cast<int64_t>(ctas) * 16 * (d + 2); }
 
-int32_t decode_ctas(const bsp_device* dev, int group) { return dc_per_sm(group > 8 ? 16 : 8) * dev->sm_count; }
+int32_t decode_ctas(const bsp_device* dev, int d, int group) { return dc_per_sm(d, group > 8 ? 16 : 8) * dev->sm_count; }
 
 int decode_smem_bytes(int d, int group) { return dc_smem(d, group > 8 ? 16 : 8); }
 

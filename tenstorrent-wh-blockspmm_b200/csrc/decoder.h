@@ -130,7 +130,7 @@ bsp_status launch_append(AppendParams& p, int sm_count, cudaStream_t stream);
 bsp_status prepare_prompt(const bsp_prompt_plan* plan);
 bsp_status prepare_decode(const bsp_decode_plan* plan);
 bsp_status launch_decode(const bsp_decode_plan* plan, DecodeParams& p, cudaStream_t stream);
-int32_t decode_ctas(const bsp_device* dev, int group);
+int32_t decode_ctas(const bsp_device* dev, int d, int group);
 int64_t decode_work_floats(int32_t ctas, int32_t d);
 int decode_smem_bytes(int d, int group);
 bsp_status plan_prompt_host(bsp_prompt_plan* p, const int32_t* q_lens, const int32_t* kv_lens, int sm_count,
