@@ -4,20 +4,20 @@
 // Work is cut by (page, head): a page's scale belongs to all its tokens, so the
 // team of warps that writes new tokens of a page also finds their largest
 // magnitude, joins it with the page's scale and, where that grew, rounds the
-// page's earlier codes again.  Memory-bound: 16 tokens of a head stay in the
-// registers of a warp between the search for the maximum and the store, so each
-// value is read once.
+// page's earlier codes again.
 //
-// Jobs of a chunk (the new tokens of one sequence on one page): keys of a head,
-// values of a head, and queries of four heads, for which each (cos, sin) is
-// loaded once.  A team has one warp per 16 tokens of the page when sequences
-// bring pages of tokens, and a single warp when they bring one token each: a
-// warp with nothing to do still costs its start.  Finding the chunk is a chain
-// of dependent loads, so a team does several jobs of its chunk once there are
-// enough warps to fill the GPU, and the page number is not waited for before
-// the data are on their way.
+// A job is one head of the keys, the values or the queries of a chunk (the new
+// tokens of one sequence on one page); a team does several of a chunk's jobs.  A
+// team has one warp per 16 tokens of the page when sequences bring pages of
+// tokens, and a single warp when they bring one token each: a warp with nothing
+// to do still costs its start.  Memory-bound, so the loads of the next job are
+// always in flight: asynchronous copies bring its 16-bit values to shared
+// memory (each lane its own, two buffers), while (cos, sin) of the warp's 16
+// tokens stay in registers for all its jobs.  Keys are rotated twice, for their
+// maximum and for their codes: cheaper than keeping them in 32 bits.
 #include <cuda_fp8.h>
 
+#include "bsp_ptx.cuh"
 #include "rope.cuh"
 
 namespace bsp {
@@ -26,8 +26,7 @@ using namespace dev;
 namespace {
 
 constexpr int kApWarps = 8;
-constexpr int kApTokens = 16;  // of one head in a warp's registers
-constexpr int kApQHeads = 4;   // query heads of a job
+constexpr int kApTokens = 16;  // of one head that a warp takes at once
 
 // New tokens [t0, t0 + n) of one sequence, at slots [slot, slot + n) of page.
 struct Chunk {
@@ -105,96 +104,37 @@ __device__ __forceinline__ void team_sync(int team, int team_warps) {
   else asm volatile("bar.sync %0, %1;" ::"r"(team + 1), "r"(32 * team_warps) : "memory");
 }
 
-// Queries of up to four heads of a chunk, from h0 on.
-template <int kUnits, bool kInterleaved>
-__device__ __forceinline__ void append_queries(const AppendParams& p, const Chunk& ck, int h0, int in_team, int lane) {
-  constexpr int kAcross = 32 / kUnits, kD = 16 * kUnits;
-  const int u = lane % kUnits, nh = min(kApQHeads, p.heads - h0);
-  const RopeUnit<8> un(u, p.rot, kD);
-  const float2* turns = p.table + ck.pos0 * (p.rot / 2);
-  for (int t = in_team * kAcross + lane / kUnits; t < ck.n; t += kAcross * p.team_warps) {
-    const uint16_t* x = static_cast<const uint16_t*>(p.q.p) + (ck.t0 + t) * p.q.token + h0 * p.q.head;
-    uint16_t* y = static_cast<uint16_t*>(p.q_out.p) + (ck.t0 + t) * p.q_out.token + h0 * p.q_out.head;
-    uint4 raw[kApQHeads][2];
-#pragma unroll
-    for (int h = 0; h < kApQHeads; ++h)
-      if (h < nh) {
-        raw[h][0] = *reinterpret_cast<const uint4*>(x + h * p.q.head + un.lo);
-        raw[h][1] = *reinterpret_cast<const uint4*>(x + h * p.q.head + un.hi);
-      }
-    float2 cs[8];
-    if (un.turns) load_turns<8>(turns + static_cast<int64_t>(t) * (p.rot / 2), u, p.rot, kInterleaved, cs);
-#pragma unroll
-    for (int h = 0; h < kApQHeads; ++h)
-      if (h < nh) {
-        float lo[8], hi[8];
-        unpack8(raw[h][0], lo);
-        unpack8(raw[h][1], hi);
-        if (un.turns) turn_unit<8>(lo, hi, cs, kInterleaved, 1.f);
-        store_vec(y + h * p.q_out.head + un.lo, lo);
-        store_vec(y + h * p.q_out.head + un.hi, hi);
-      }
-  }
+__device__ __forceinline__ bool bad_page(const AppendParams& p, const Chunk& ck, int lane) {
+  if (ck.page >= 0 && ck.page < p.cache.n_pages) return false;
+  if (lane == 0) atomicOr(p.status, ST_BAD_INDEX);
+  return true;
 }
 
-// Keys or values of one head of a chunk.  What stays in registers between the
-// two passes are the 16-bit values as they came: the rotation is done in both.
-template <int kUnits, bool kInterleaved>
-__device__ __forceinline__ void append_codes(const AppendParams& p, const Chunk& ck, bool is_v, int h, int team,
-                                             int in_team, int lane, float* s_max) {
-  constexpr int kAcross = 32 / kUnits;           // tokens side by side in a warp
-  constexpr int kDeep = kApTokens / kAcross;     // and one after the other
-  constexpr int kD = 16 * kUnits;
-  const int u = lane % kUnits, at = lane / kUnits;
-  const int stride = kApTokens * p.team_warps;
-  const RopeUnit<8> un(u, p.table && !is_v ? p.rot : 0, kD);
-  const float2* turns = p.table + ck.pos0 * (p.rot / 2);
-  const HeadsView& in = is_v ? p.v : p.k;
-  const uint16_t* x = static_cast<const uint16_t*>(in.p) + ck.t0 * in.token + h * in.head;
-  uint4 raw[kDeep][2];
-  auto load = [&](int base) {
+// Largest finite magnitude.
+__device__ __forceinline__ float magnitude(const float (&lo)[8], const float (&hi)[8], float m) {
 #pragma unroll
-    for (int k = 0; k < kDeep; ++k) {
-      const int t = base + k * kAcross + at;
-      raw[k][0] = raw[k][1] = make_uint4(0, 0, 0, 0);
-      if (t < ck.n) {
-        raw[k][0] = *reinterpret_cast<const uint4*>(x + t * in.token + un.lo);
-        raw[k][1] = *reinterpret_cast<const uint4*>(x + t * in.token + un.hi);
-      }
-    }
-  };
-  float lo[8], hi[8];
-  auto values = [&](const uint4 (&r)[2], int t) {
-    unpack8(r[0], lo);
-    unpack8(r[1], hi);
-    if (un.turns && t < ck.n) {
-      float2 cs[8];
-      load_turns<8>(turns + static_cast<int64_t>(t) * (p.rot / 2), u, p.rot, kInterleaved, cs);
-      turn_unit<8>(lo, hi, cs, kInterleaved, 1.f);
-    }
-  };
-  float m = 0.f;
-  for (int base = in_team * kApTokens; base < ck.n; base += stride) {
-    load(base);
-#pragma unroll
-    for (int k = 0; k < kDeep; ++k) {
-      values(raw[k], base + k * kAcross + at);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const float a = fabsf(lo[j]), b = fabsf(hi[j]);
-        m = fmaxf(m, a <= 3.402823466e38f ? a : 0.f);
-        m = fmaxf(m, b <= 3.402823466e38f ? b : 0.f);
-      }
-    }
+  for (int j = 0; j < 8; ++j) {
+    const float a = fabsf(lo[j]), b = fabsf(hi[j]);
+    m = fmaxf(m, a <= 3.402823466e38f ? a : 0.f);
+    m = fmaxf(m, b <= 3.402823466e38f ? b : 0.f);
   }
-  if (ck.page < 0 || ck.page >= p.cache.n_pages) {  // the whole team leaves
-    if (lane == 0) atomicOr(p.status, ST_BAD_INDEX);
-    return;
-  }
+  return m;
+}
+
+// Where a team's keys or values of one head go.
+struct Target {
+  uint8_t* codes;  // of the chunk's first token
+  float scale;     // 2^-e
+};
+
+// The page's exponent from the lanes' maxima and what the page holds; earlier
+// codes are rounded again where it grew.
+template <int kD>
+__device__ __forceinline__ Target settle(const AppendParams& p, const Chunk& ck, bool is_v, int h, int team, int in_team,
+                                        int lane, float* s_max, float m) {
   uint8_t* codes = static_cast<uint8_t*>(is_v ? p.cache.v : p.cache.k) + ck.page * p.cache.page_stride +
                    h * p.cache.head_stride;
-  float* sp = (is_v ? p.cache.v_scale : p.cache.k_scale) +
-              static_cast<int64_t>(ck.page) * p.cache.kv_heads + h;
+  float* sp = (is_v ? p.cache.v_scale : p.cache.k_scale) + static_cast<int64_t>(ck.page) * p.cache.kv_heads + h;
   const uint32_t old_bits = ck.slot > 0 ? __float_as_uint(*sp) : 0;
   for (int k = 16; k; k >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, k));
   if (p.team_warps > 1) {
@@ -223,51 +163,186 @@ __device__ __forceinline__ void append_codes(const AppendParams& p, const Chunk&
   }
   // every thread of the team has its copy of the old scale by now
   if (in_team == 0 && lane == 0) *sp = two_to(e);
-  const float scale = two_to(-e);
-  codes += static_cast<int64_t>(ck.slot) * kD;
-  uint16_t* y = !is_v && p.k_out.p
-                    ? static_cast<uint16_t*>(p.k_out.p) + ck.t0 * p.k_out.token + h * p.k_out.head : nullptr;
-  const bool again = ck.n > stride;  // more tokens than the team's registers hold
-  for (int base = in_team * kApTokens; base < ck.n; base += stride) {
-    if (again) load(base);
+  return {codes + static_cast<int64_t>(ck.slot) * kD, two_to(-e)};
+}
+
+__device__ __forceinline__ void put_codes(uint8_t* c, const RopeUnit<8>& un, const float (&lo)[8], const float (&hi)[8],
+                                         float scale) {
+  *reinterpret_cast<uint2*>(c + un.lo) = make_uint2(codes4(lo, scale), codes4(lo + 4, scale));
+  *reinterpret_cast<uint2*>(c + un.hi) = make_uint2(codes4(hi, scale), codes4(hi + 4, scale));
+}
+
+// A job of a chunk: input, 16-bit output (may be null) and what becomes of it.
+struct Job {
+  const uint16_t* x;
+  uint16_t* y;
+  int64_t x_token, y_token;
+  int h;
+  bool is_q, is_v;
+};
+__device__ __forceinline__ Job job_of(const AppendParams& p, const Chunk& ck, int job) {
+  const int hk = p.cache.kv_heads;
+  Job j;
+  j.is_q = job >= 2 * hk;
+  j.is_v = !j.is_q && job >= hk;
+  j.h = j.is_q ? job - 2 * hk : j.is_v ? job - hk : job;
+  const HeadsView& in = j.is_q ? p.q : j.is_v ? p.v : p.k;
+  const HeadsOut& out = j.is_q ? p.q_out : p.k_out;
+  j.x_token = in.token;
+  j.y_token = out.token;
+  j.x = static_cast<const uint16_t*>(in.p) + ck.t0 * in.token + j.h * in.head;
+  j.y = !j.is_v && out.p ? static_cast<uint16_t*>(out.p) + ck.t0 * out.token + j.h * out.head : nullptr;
+  return j;
+}
+
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+
+// More tokens on the page than the team's warps hold at once (a long prompt
+// among many single tokens): straight from memory, twice for keys and values.
+template <int kUnits, bool kInterleaved>
+__device__ __noinline__ void append_long(const AppendParams& p, const Chunk& ck, int job, int team, int in_team,
+                                         int lane, float* s_max) {
+  constexpr int kAcross = 32 / kUnits, kD = 16 * kUnits;
+  const Job j = job_of(p, ck, job);
+  const int u = lane % kUnits;
+  const RopeUnit<8> un(u, p.table && !j.is_v ? p.rot : 0, kD);
+  float m = 0.f;
+  Target to{nullptr, 1.f};
+  for (int pass = j.is_q ? 1 : 0; pass < 2; ++pass) {
+    for (int t = in_team * kAcross + lane / kUnits; t < ck.n; t += kAcross * p.team_warps) {
+      float lo[8], hi[8];
+      load_vec(j.x + t * j.x_token + un.lo, lo);
+      load_vec(j.x + t * j.x_token + un.hi, hi);
+      if (un.turns) {
+        float2 cs[8];
+        load_turns<8>(p.table + (ck.pos0 + t) * (p.rot / 2), u, p.rot, kInterleaved, cs);
+        turn_unit<8>(lo, hi, cs, kInterleaved, 1.f);
+      }
+      if (pass == 0) {
+        m = magnitude(lo, hi, m);
+      } else {
+        if (!j.is_q) put_codes(to.codes + t * kD, un, lo, hi, to.scale);
+        if (j.y) {
+          store_vec(j.y + t * j.y_token + un.lo, lo);
+          store_vec(j.y + t * j.y_token + un.hi, hi);
+        }
+      }
+    }
+    if (pass == 0) to = settle<kD>(p, ck, j.is_v, j.h, team, in_team, lane, s_max, m);
+  }
+}
+
+// kUnits: units of two vectors of 8 values in a head (d / 16).
+template <int kUnits, bool kInterleaved>
+__global__ void __launch_bounds__(32 * kApWarps, 2) append_kernel(const __grid_constant__ AppendParams p) {
+  constexpr int kAcross = 32 / kUnits;        // tokens side by side in a warp
+  constexpr int kDeep = kApTokens / kAcross;  // and one after the other
+  constexpr int kD = 16 * kUnits;
+  __shared__ float s_max[kApWarps];
+  extern __shared__ uint4 s_raw[];            // per warp 2 x [kDeep][2][32]
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int team = warp / p.team_warps, in_team = warp % p.team_warps;
+  const int teams = kApWarps / p.team_warps;
+  const int jobs = 2 * p.cache.kv_heads + (p.q.p ? p.heads : 0);
+  const int first = blockIdx.y * teams + team, step = gridDim.y * teams;
+  Chunk ck;
+  if (!find_chunk(p, blockIdx.x, lane, ck)) return;
+  if (ck.n > kApTokens * p.team_warps) {
+    const bool bad = bad_page(p, ck, lane);
+    for (int job = first; job < jobs && !bad; job += step)
+      append_long<kUnits, kInterleaved>(p, ck, job, team, in_team, lane, s_max);
+    return;
+  }
+  const int u = lane % kUnits, t0 = in_team * kApTokens + lane / kUnits;  // this lane's tokens: t0 + kAcross k
+  const RopeUnit<8> turned(u, p.table ? p.rot : 0, kD), plain(u, 0, kD);
+  uint4* raw = s_raw + warp * (2 * kDeep * 2 * 32) + lane;
+  auto fetch = [&](int job, int buf) {
+    if (job < jobs) {
+      const Job j = job_of(p, ck, job);
+      const int lo = j.is_v ? plain.lo : turned.lo, hi = j.is_v ? plain.hi : turned.hi;
+#pragma unroll
+      for (int k = 0; k < kDeep; ++k) {
+        const int t = t0 + kAcross * k;
+        if (t < ck.n) {
+          copy16(smem_u32(raw + ((buf * kDeep + k) * 2 + 0) * 32), j.x + t * j.x_token + lo);
+          copy16(smem_u32(raw + ((buf * kDeep + k) * 2 + 1) * 32), j.x + t * j.x_token + hi);
+        }
+      }
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  fetch(first, 0);
+  float2 cs[kDeep][8];
+  if (turned.turns) {
+#pragma unroll
+    for (int k = 0; k < kDeep; ++k)
+      if (t0 + kAcross * k < ck.n)
+        load_turns<8>(p.table + (ck.pos0 + t0 + kAcross * k) * (p.rot / 2), u, p.rot, kInterleaved, cs[k]);
+  }
+  if (bad_page(p, ck, lane)) {  // (looked at behind the first copies, which do not wait for the page)
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+    return;
+  }
+  int buf = 0;
+  for (int job = first; job < jobs; job += step, buf ^= 1) {
+    fetch(job + step, buf ^ 1);
+    asm volatile("cp.async.wait_group 1;" ::: "memory");
+    const Job j = job_of(p, ck, job);
+    const RopeUnit<8>& un = j.is_v ? plain : turned;
+    float lo[8], hi[8];
+    auto take = [&](int k) {  // token t0 + kAcross k, rotated
+      unpack8(raw[((buf * kDeep + k) * 2 + 0) * 32], lo);
+      unpack8(raw[((buf * kDeep + k) * 2 + 1) * 32], hi);
+      if (un.turns) turn_unit<8>(lo, hi, cs[k], kInterleaved, 1.f);
+    };
+    Target to{nullptr, 1.f};
+    if (!j.is_q) {
+      float m = 0.f;
+#pragma unroll
+      for (int k = 0; k < kDeep; ++k)
+        if (t0 + kAcross * k < ck.n) {
+          take(k);
+          m = magnitude(lo, hi, m);
+        }
+      to = settle<kD>(p, ck, j.is_v, j.h, team, in_team, lane, s_max, m);
+    }
 #pragma unroll
     for (int k = 0; k < kDeep; ++k) {
-      const int t = base + k * kAcross + at;
+      const int t = t0 + kAcross * k;
       if (t < ck.n) {
-        values(raw[k], t);
-        uint8_t* c = codes + t * kD;
-        *reinterpret_cast<uint2*>(c + un.lo) = make_uint2(codes4(lo, scale), codes4(lo + 4, scale));
-        *reinterpret_cast<uint2*>(c + un.hi) = make_uint2(codes4(hi, scale), codes4(hi + 4, scale));
-        if (y) {
-          store_vec(y + t * p.k_out.token + un.lo, lo);
-          store_vec(y + t * p.k_out.token + un.hi, hi);
+        take(k);
+        if (!j.is_q) put_codes(to.codes + t * kD, un, lo, hi, to.scale);
+        if (j.y) {
+          store_vec(j.y + t * j.y_token + un.lo, lo);
+          store_vec(j.y + t * j.y_token + un.hi, hi);
         }
       }
     }
   }
 }
 
-// kUnits: units of two vectors of 8 values in a head (d / 16).
-template <int kUnits, bool kInterleaved>
-__global__ void __launch_bounds__(32 * kApWarps, 2) append_kernel(const AppendParams p) {
-  __shared__ float s_max[kApWarps];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int team = warp / p.team_warps, in_team = warp % p.team_warps;
-  const int teams = kApWarps / p.team_warps, hk = p.cache.kv_heads;
-  const int jobs = 2 * hk + (p.q.p ? (p.heads + kApQHeads - 1) / kApQHeads : 0);
-  Chunk ck;
-  if (!find_chunk(p, blockIdx.x, lane, ck)) return;
-  for (int job = blockIdx.y * teams + team; job < jobs; job += gridDim.y * teams) {
-    if (job < 2 * hk)
-      append_codes<kUnits, kInterleaved>(p, ck, job >= hk, job >= hk ? job - hk : job, team, in_team, lane, s_max);
-    else
-      append_queries<kUnits, kInterleaved>(p, ck, (job - 2 * hk) * kApQHeads, in_team, lane);
-  }
+using AppendKernel = void (*)(AppendParams);
+AppendKernel pick(int d, bool interleaved) {
+  return d == 64 ? (interleaved ? append_kernel<4, true> : append_kernel<4, false>)
+                 : (interleaved ? append_kernel<8, true> : append_kernel<8, false>);
 }
+constexpr int raw_bytes(int d) { return kApWarps * 2 * kApTokens * d * 2; }
 
 }  // namespace
 
-bsp_status launch_append(AppendParams& p, int sm_count, cudaStream_t stream) {
+bsp_status launch_append(AppendParams& p, bsp_device* dev, cudaStream_t stream) {
+  if (!dev->append_ready) {
+    for (int d : {64, 128})
+      for (bool i : {false, true}) {
+        const bsp_status s =
+            cuda_check(cudaFuncSetAttribute(pick(d, i), cudaFuncAttributeMaxDynamicSharedMemorySize, raw_bytes(d)),
+                       "cudaFuncSetAttribute(append)");
+        if (s != BSP_OK) return s;
+      }
+    dev->append_ready = true;
+  }
   const int page = p.cache.page;
   p.page_shift = __builtin_ctz(static_cast<unsigned>(page));
   const int64_t per_seq = p.tokens / p.n_seqs;
@@ -275,15 +350,15 @@ bsp_status launch_append(AppendParams& p, int sm_count, cudaStream_t stream) {
   while (p.team_warps * 2 * kApTokens <= std::min<int64_t>(per_seq, page)) p.team_warps *= 2;
   const int64_t chunks = p.tokens / page + 2 * static_cast<int64_t>(p.n_seqs);
   if (chunks > 0x7FFFFFFF) return set_error(BSP_ERR_UNSUPPORTED, "too many sequences");
-  const int jobs = 2 * p.cache.kv_heads + (p.q.p ? (p.heads + kApQHeads - 1) / kApQHeads : 0);
+  const int jobs = 2 * p.cache.kv_heads + (p.q.p ? p.heads : 0);
   const int teams = kApWarps / p.team_warps;
-  // as many blocks to a chunk as its jobs fill, or fewer once four rounds of
-  // blocks of all chunks fill the GPU (two of them fit an SM)
-  const int64_t most = (jobs + teams - 1) / teams, enough = 8 * static_cast<int64_t>(sm_count) / (p.tokens / page + 1) + 1;
+  // A job to a team while that is needed to fill the GPU, else several: 14278
+  // tokens in pages of 16 take 68 us with one block to a chunk (of 904), 74 us
+  // with three and 96 us with six.
+  const int64_t most = (jobs + teams - 1) / teams;
+  const int64_t enough = 4 * static_cast<int64_t>(dev->sm_count) / (p.tokens / page + p.n_seqs) + 1;
   const dim3 grid(static_cast<unsigned>(chunks), static_cast<unsigned>(std::min(most, enough)));
-  const auto kernel = p.cache.d == 64 ? (p.interleaved ? append_kernel<4, true> : append_kernel<4, false>)
-                                      : (p.interleaved ? append_kernel<8, true> : append_kernel<8, false>);
-  kernel<<<grid, 32 * kApWarps, 0, stream>>>(p);
+  pick(p.cache.d, p.interleaved)<<<grid, 32 * kApWarps, raw_bytes(p.cache.d), stream>>>(p);
   return cuda_check(cudaGetLastError(), "cache append launch");
 }
 

@@ -140,7 +140,7 @@ bsp_status bsp_kv_append(bsp_device* dev, const bsp_kv_cache* cache, const void*
     if ((s = check_heads("q", q, q_token, q_head, 2)) != BSP_OK) return s;
     if ((s = check_heads("q_out", q_out, qo_token, qo_head, 2)) != BSP_OK) return s;
   }
-  if (2 * static_cast<int64_t>(cache->kv_heads) + (q ? heads / 4 : 0) > 65000)
+  if (2 * static_cast<int64_t>(cache->kv_heads) + (q ? heads : 0) > 65000)
     return set_error(BSP_ERR_UNSUPPORTED, "too many heads");
   if (k_out && (s = check_heads("k_out", k_out, ko_token, ko_head, 2)) != BSP_OK) return s;
   if (!starts || !before || !page_table) return set_error(BSP_ERR_INVALID_ARG, "null index array");
@@ -165,7 +165,7 @@ bsp_status bsp_kv_append(bsp_device* dev, const bsp_kv_cache* cache, const void*
   p.interleaved = layout == BSP_ROPE_INTERLEAVED;
   p.status = dev->d_status;
   OnDevice on(dev->ordinal);
-  return launch_append(p, dev->sm_count, static_cast<cudaStream_t>(stream));
+  return launch_append(p, dev, static_cast<cudaStream_t>(stream));
 }
 
 bsp_status bsp_prompt_plan_create(bsp_device* dev, int32_t n_seqs, const int32_t* q_lens, const int32_t* kv_lens,

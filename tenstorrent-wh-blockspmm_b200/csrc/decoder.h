@@ -125,7 +125,7 @@ namespace bsp {
 bsp_status launch_rope_table(bsp_device* dev, int64_t n_pos, int32_t rot, double base, const bsp_rope_scaling& sc,
                              float* table, cudaStream_t stream);
 bsp_status launch_rope(const RopeParams& p, bsp_dtype type, int sm_count, cudaStream_t stream);
-bsp_status launch_append(AppendParams& p, int sm_count, cudaStream_t stream);
+bsp_status launch_append(AppendParams& p, bsp_device* dev, cudaStream_t stream);
 // one-time settings of the kernel that a plan launches
 bsp_status prepare_prompt(const bsp_prompt_plan* plan);
 bsp_status prepare_decode(const bsp_decode_plan* plan);

@@ -179,6 +179,8 @@ APPEND = [
     ([33, 200], [95, 0], 1, 8, 32, 64, 32),
     ([129, 300, 1], [127, 1, 255], 2, 2, 128, 128, 128),
     ([1] * 40, list(range(40)), 8, 32, 64, 128, 128),
+    ([1] * 30 + [150], [5] * 30 + [37], 2, 6, 64, 128, 64),   # a prompt among single tokens
+    ([1] * 20 + [200, 17], [100] * 20 + [90, 0], 1, 3, 128, 64, 64),
 ]
 
 
