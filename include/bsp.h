@@ -552,8 +552,10 @@ bsp_status bsp_decode_execute(const bsp_decode_plan* plan, const bsp_kv_cache* c
                               int64_t table_stride, int64_t table_width, float scale, void* o, int64_t o_token,
                               int64_t o_head, float* lse, void* stream);
 bsp_status bsp_decode_plan_destroy(bsp_decode_plan* plan);
-/* info[0] max_seqs, [1] grid, [2] heads, [3] kv_heads, [4] d, [5] page,
- * [8] workspace bytes, [9] shared memory. */
+/* info[0] max_seqs, [1] most CTAs, [2] heads, [3] kv_heads, [4] d, [5] page,
+ * [8] workspace bytes, [9] shared memory.  (Creating or destroying a prompt or
+ * decode plan takes tens of microseconds; both wait for the device's memory
+ * pool on the legacy stream, so not while a stream captures.) */
 bsp_status bsp_decode_plan_info(const bsp_decode_plan* plan, int64_t info[16]);
 
 /* ---- multi-GPU helpers (host logic; the exchange itself is NCCL) --------

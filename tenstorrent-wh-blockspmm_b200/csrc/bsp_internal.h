@@ -468,6 +468,9 @@ struct OnDevice {  // make `ordinal` current for a call, put the caller's device
   }
 };
 
+// Give the plan pool's unused memory on GPU `ordinal` back (capi_decoder.cpp).
+void trim_plan_pool(int ordinal);
+
 // error plumbing (capi.cpp)
 bsp_status set_error(bsp_status s, const std::string& msg);
 bsp_status cuda_check(cudaError_t e, const char* what);

@@ -287,6 +287,7 @@ bsp_status bsp_device_close(bsp_device* dev) {
   if (dev->pinned) cudaFreeHost(dev->pinned);
   if (dev->plan_ws) cudaFree(dev->plan_ws);
   if (dev->aux_ws) cudaFree(dev->aux_ws);
+  trim_plan_pool(dev->ordinal);
   for (auto& sl : dev->batch_slots) {
     if (sl.d) cudaFree(sl.d);
     if (sl.h) cudaFreeHost(sl.h);

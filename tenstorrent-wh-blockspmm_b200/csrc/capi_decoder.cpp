@@ -4,6 +4,7 @@
 #include <algorithm>
 #include <cstring>
 #include <exception>
+#include <mutex>
 #include <new>
 
 #include "bsp_testing.h"
@@ -56,7 +57,55 @@ bsp_status check_attention_heads(int32_t heads, int32_t kv_heads, int32_t d) {
   return BSP_OK;
 }
 
+// The prompt and decode plans come and go with a batch: their memory comes from
+// a pool per GPU that keeps what is freed (microseconds, where cudaMalloc takes
+// up to milliseconds).  It belongs to the process: plans may outlive the
+// bsp_device they were made with.
+constexpr int kMaxGpus = 64;
+std::mutex g_pool_mutex;
+cudaMemPool_t g_pools[kMaxGpus] = {};
+
+// `bytes` of the pool, ready on every stream once the legacy stream has been
+// synchronised (the callers do, behind their copies).
+bsp_status plan_alloc(int ordinal, size_t bytes, void** out) {
+  *out = nullptr;
+  if (ordinal < 0 || ordinal >= kMaxGpus) return set_error(BSP_ERR_UNSUPPORTED, "GPU ordinal out of range");
+  std::lock_guard<std::mutex> lock(g_pool_mutex);
+  cudaMemPool_t& pool = g_pools[ordinal];
+  if (!pool) {
+    cudaMemPoolProps props{};
+    props.allocType = cudaMemAllocationTypePinned;
+    props.location.type = cudaMemLocationTypeDevice;
+    props.location.id = ordinal;
+    const bsp_status s = cuda_check(cudaMemPoolCreate(&pool, &props), "cudaMemPoolCreate");
+    if (s != BSP_OK) {
+      pool = nullptr;
+      return s;
+    }
+    uint64_t keep = UINT64_MAX;
+    cudaMemPoolSetAttribute(pool, cudaMemPoolAttrReleaseThreshold, &keep);
+  }
+  if (cudaMallocFromPoolAsync(out, bytes, pool, nullptr) != cudaSuccess) {
+    *out = nullptr;
+    cudaGetLastError();
+    return set_error(BSP_ERR_ALLOC, "device memory of the plan");
+  }
+  return BSP_OK;
+}
+// Launches of the plan may be on any stream: wait for the device, as cudaFree does.
+void plan_free(int ordinal, void* p) {
+  if (!p) return;
+  OnDevice on(ordinal);
+  cudaDeviceSynchronize();
+  cudaFreeAsync(p, nullptr);
+}
+
 }  // namespace
+
+void bsp::trim_plan_pool(int ordinal) {
+  std::lock_guard<std::mutex> lock(g_pool_mutex);
+  if (ordinal >= 0 && ordinal < kMaxGpus && g_pools[ordinal]) cudaMemPoolTrimTo(g_pools[ordinal], 0);
+}
 
 extern "C" {
 
@@ -181,6 +230,7 @@ bsp_status bsp_prompt_plan_create(bsp_device* dev, int32_t n_seqs, const int32_t
   bsp_prompt_plan* p = new (std::nothrow) bsp_prompt_plan();
   if (!p) return set_error(BSP_ERR_ALLOC, "host allocation failed");
   p->dev = dev;
+  p->ordinal = dev->ordinal;
   p->n_seqs = n_seqs;
   p->heads = heads;
   p->kv_heads = kv_heads;
@@ -196,17 +246,17 @@ bsp_status bsp_prompt_plan_create(bsp_device* dev, int32_t n_seqs, const int32_t
     OnDevice on(dev->ordinal);
     const size_t ub = p->h_units.size() * sizeof(PromptUnit);
     p->blob_bytes = ub + p->h_cta_begin.size() * sizeof(int32_t);
-    if (cudaMalloc(&p->d_blob, p->blob_bytes) != cudaSuccess) {
-      p->d_blob = nullptr;
-      s = set_error(BSP_ERR_ALLOC, "cudaMalloc of the plan tables failed");
-    } else {
+    s = plan_alloc(dev->ordinal, p->blob_bytes, &p->d_blob);
+    if (s == BSP_OK) {
       p->d_units = static_cast<PromptUnit*>(p->d_blob);
       p->d_cta_begin = reinterpret_cast<int32_t*>(static_cast<uint8_t*>(p->d_blob) + ub);
-      s = cuda_check(cudaMemcpy(p->d_units, p->h_units.data(), ub, cudaMemcpyHostToDevice), "upload plan tables");
+      s = cuda_check(cudaMemcpyAsync(p->d_units, p->h_units.data(), ub, cudaMemcpyHostToDevice, nullptr),
+                     "upload plan tables");
       if (s == BSP_OK)
-        s = cuda_check(cudaMemcpy(p->d_cta_begin, p->h_cta_begin.data(), p->h_cta_begin.size() * sizeof(int32_t),
-                                  cudaMemcpyHostToDevice),
+        s = cuda_check(cudaMemcpyAsync(p->d_cta_begin, p->h_cta_begin.data(), p->h_cta_begin.size() * sizeof(int32_t),
+                                       cudaMemcpyHostToDevice, nullptr),
                        "upload plan tables");
+      if (s == BSP_OK) s = cuda_check(cudaStreamSynchronize(nullptr), "upload plan tables");
       if (s == BSP_OK) s = prepare_prompt(p);
     }
   }
@@ -254,10 +304,7 @@ bsp_status bsp_prompt_execute(const bsp_prompt_plan* plan, const void* q, int64_
 
 bsp_status bsp_prompt_plan_destroy(bsp_prompt_plan* plan) {
   if (!plan) return BSP_OK;
-  if (plan->d_blob) {
-    OnDevice on(plan->dev->ordinal);
-    cudaFree(plan->d_blob);
-  }
+  plan_free(plan->ordinal, plan->d_blob);
   delete plan;
   return BSP_OK;
 }
@@ -318,6 +365,7 @@ bsp_status bsp_decode_plan_create(bsp_device* dev, int32_t max_seqs, int32_t hea
   bsp_decode_plan* p = new (std::nothrow) bsp_decode_plan();
   if (!p) return set_error(BSP_ERR_ALLOC, "host allocation failed");
   p->dev = dev;
+  p->ordinal = dev->ordinal;
   p->max_seqs = max_seqs;
   p->heads = heads;
   p->kv_heads = kv_heads;
@@ -330,13 +378,14 @@ bsp_status bsp_decode_plan_create(bsp_device* dev, int32_t max_seqs, int32_t hea
   OnDevice on(dev->ordinal);
   const size_t counters = (sizeof(int32_t) * p->grid + 255) / 256 * 256;
   p->blob_bytes = counters + sizeof(float) * decode_work_floats(p->grid, d);
-  if (cudaMalloc(&p->d_blob, p->blob_bytes) != cudaSuccess) {
+  s = plan_alloc(dev->ordinal, p->blob_bytes, &p->d_blob);
+  if (s != BSP_OK) {
     delete p;
-    return set_error(BSP_ERR_ALLOC, "cudaMalloc of the decode workspace failed");
+    return s;
   }
   p->d_counters = static_cast<int32_t*>(p->d_blob);
   p->d_work = reinterpret_cast<float*>(static_cast<uint8_t*>(p->d_blob) + counters);
-  s = cuda_check(cudaMemset(p->d_counters, 0, counters), "clear the decode counters");
+  s = cuda_check(cudaMemsetAsync(p->d_counters, 0, counters, nullptr), "clear the decode counters");
   if (s == BSP_OK) s = prepare_decode(p);
   // the clearing ran on the legacy stream: executes may come on any other
   if (s == BSP_OK) s = cuda_check(cudaStreamSynchronize(nullptr), "clear the decode counters");
@@ -390,10 +439,7 @@ bsp_status bsp_decode_execute(const bsp_decode_plan* plan, const bsp_kv_cache* c
 
 bsp_status bsp_decode_plan_destroy(bsp_decode_plan* plan) {
   if (!plan) return BSP_OK;
-  if (plan->d_blob) {
-    OnDevice on(plan->dev->ordinal);
-    cudaFree(plan->d_blob);
-  }
+  plan_free(plan->ordinal, plan->d_blob);
   delete plan;
   return BSP_OK;
 }

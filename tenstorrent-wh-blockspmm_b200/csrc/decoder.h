@@ -96,6 +96,7 @@ struct PromptParams {
 
 struct bsp_prompt_plan {
   bsp_device* dev = nullptr;
+  int ordinal = 0;
   int32_t n_seqs = 0, heads = 0, kv_heads = 0, d = 0, causal = 0;
   int64_t q_tokens = 0, kv_tokens = 0;
   int32_t packed = 1, tile_tokens = 128;
@@ -112,6 +113,7 @@ struct bsp_prompt_plan {
 
 struct bsp_decode_plan {
   bsp_device* dev = nullptr;
+  int ordinal = 0;
   int32_t max_seqs = 0, heads = 0, kv_heads = 0, d = 0, page = 0;
   int32_t grid = 0, smem_bytes = 0;
   uint64_t timeout_ns = 0;

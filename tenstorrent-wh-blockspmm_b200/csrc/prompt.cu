@@ -495,6 +495,7 @@ __device__ __forceinline__ void pr_softmax(const PromptParams& p, PrHeader* hdr,
     ++outs;
     tc_fence_after();
     if (m == -INFINITY && l < 1.f) l = 0.f;  // no key: exp2_pair gave 2^-126 for each masked one
+    if (!(m < INFINITY)) l = __uint_as_float(0x7FC00000u);  // a NaN or infinite score: the row is NaN
     const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);  // a NaN sum stays one
 #pragma unroll 1
     for (int c = 0; c < kD / 32; ++c) {

@@ -424,6 +424,40 @@ def test_prompt_neighbours_do_not_leak(bsp, bad):
     assert torch.equal(o2[keep], o[keep]) and torch.isnan(o2[~keep]).any()
 
 
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+def test_prompt_bad_key_makes_its_rows_nan(bsp, d, bad):
+    """A key that is NaN (or gives an infinite score) makes the rows that see
+    it NaN, at whichever place of a step it stands; the rows before are right."""
+    torch = torch_()
+    n = 300
+    rng = np.random.default_rng(3)
+    q = ref.bf16(np.abs(rng.normal(0, 1, (n, 2, d))) + 0.1)
+    k, v = (ref.bf16(rng.normal(0, 1, (n, 1, d))) for _ in range(2))
+    gold = prompt_gold(q.astype(float), k.astype(float), v.astype(float), [n], [n], 1, 1 / np.sqrt(d), True)
+    plan = bsp.PromptPlan(bsp.device(), [n], [n], 2, 1, d)
+    qt, kt, vt = (cuda(x, torch.bfloat16) for x in (q, k, v))
+    o, lse = torch.empty_like(qt), torch.empty((n, 2), device="cuda")
+    for at in list(range(0, 20)) + [31, 32, 63, 64, 77, 96, 127, 128, 129, 200, 299]:
+        k2 = kt.clone()
+        k2[at, 0, 5] = bad
+        plan.execute(qt, k2, vt, o, lse=lse)
+        if at:
+            check_attention(o[:at], lse[:at], *(x[:at] for x in gold), ref.U16)
+        assert torch.isnan(o[at:]).all() and torch.isnan(lse[at:]).all(), at
+    bsp.device().synchronize()
+
+
+def test_plans_outlive_their_device(bsp):
+    """A plan destroyed after its device was closed frees its memory."""
+    dev = bsp.Device(0)
+    plans = [bsp.PromptPlan(dev, [5], [5], 2, 1, 64), bsp.DecodePlan(dev, 3, 2, 1, 64, 16)]
+    dev.close()
+    for p in plans:
+        p.close()
+    torch_().cuda.synchronize()
+
+
 # ------------------------------------------------------------------ decode --
 DECODE = [
     # lengths, heads, kv heads, d, page
@@ -514,6 +548,31 @@ def test_decode_scales_far_apart(bsp):
     top = np.array([448 * scales[1][pages[s][: -(-m // page)]].max() for s, m in enumerate(lens)])
     weight = weight + 2.0 ** -13 * top[:, None, None]
     check_attention(o, lse, gold, glse, weight, size, 2 * ref.UH)
+
+
+def test_decode_nan_stays_in_its_row(bsp):
+    """A NaN code in a key or a value reaches the heads and sequences that read
+    it (a value: its column) and no others."""
+    torch = torch_()
+    rng = np.random.default_rng(6)
+    lens, hq, hk, d, page = [200, 300, 150], 4, 2, 64, 32
+    cache, _, _ = make_cache(bsp, rng, 30, hk, page, d)
+    pages = page_table(rng, lens, page, 30)
+    q = cuda(ref.bf16(rng.normal(0, 1, (3, hq, d))), torch.bfloat16)
+    plan = bsp.DecodePlan(bsp.device(), 3, hq, hk, d, page)
+    o, o2 = torch.empty_like(q), torch.empty_like(q)
+    plan.execute(cache, q, i32(lens), cuda(pages), o)
+    k = cache.k.clone()
+    cache.k[int(pages[1][4]), 1, 7, 3] = 127
+    plan.execute(cache, q, i32(lens), cuda(pages), o2)
+    assert torch.isnan(o2[1, 2:]).all() and torch.equal(o2[1, :2], o[1, :2]) and torch.equal(o2[[0, 2]], o[[0, 2]])
+    cache.k.copy_(k)
+    cache.v[int(pages[1][4]), 1, 7, 3] = 127
+    plan.execute(cache, q, i32(lens), cuda(pages), o2)
+    hit = torch.zeros_like(o, dtype=torch.bool)
+    hit[1, 2:, 3] = True
+    assert torch.isnan(o2[hit]).all() and torch.equal(o2[~hit], o[~hit])
+    bsp.device().synchronize()
 
 
 def test_decode_far_pages(bsp):
