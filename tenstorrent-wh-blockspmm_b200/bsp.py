@@ -764,32 +764,45 @@ def _refuse(msg):
     raise BspError(BSP_ERR_INVALID_ARG, msg)
 
 
-def _heads_tensor(x, name, tokens, heads, d, dtype=None):
+def _heads_tensor(x, name, shape, dtype=None):
     """Pointer, token stride and head stride of a [tokens, heads, d] operand on
     the GPU, d contiguous; bf16 unless another type is asked for.  A dimension
     of one entry is never stepped over: its stride counts as 0."""
     if _Torch.bf16 is None:
         _Torch.load()
-    if not x.is_cuda or x.dtype is not (dtype or _Torch.bf16):
+    if x.dtype is not (dtype or _Torch.bf16) or not x.is_cuda:
         _refuse(f"{name} must be a {dtype or _Torch.bf16} cuda tensor, not {x.dtype} on {x.device}")
-    if x.shape != (tokens, heads, d):
-        _refuse(f"{name} is {tuple(x.shape)}, expected {(tokens, heads, d)}")
+    if x.shape != shape:
+        _refuse(f"{name} is {tuple(x.shape)}, expected {shape}")
+    tokens, heads, d = shape
+    if x.is_contiguous():
+        return x.data_ptr(), heads * d, d
     st, sh, sd = x.stride()
-    if sd != 1 and d > 1 and tokens > 0:
+    if sd != 1 and d > 1:
         _refuse(f"{name}: the values of a head must be contiguous")
     return x.data_ptr(), st if tokens > 1 else 0, sh if heads > 1 else 0
 
 
-def _index_tensor(x, name, *shape):
-    """Pointer of an int32 tensor on the GPU, contiguous rows; None: any size."""
+def _index_tensor(x, name, n):
+    """Pointer of an int32 tensor [n] on the GPU, contiguous."""
     if _Torch.i32 is None:
         _Torch.load()
-    if not x.is_cuda or x.dtype is not _Torch.i32 or x.dim() != len(shape) or (x.stride(-1) != 1 and x.numel() > 1):
-        _refuse(f"{name} must be an int32 cuda tensor of {len(shape)} dimension(s), contiguous rows")
-    for have, want in zip(x.shape, shape):
-        if want is not None and have != want:
-            _refuse(f"{name} is {tuple(x.shape)}, expected {shape}")
+    if x.dtype is not _Torch.i32 or not x.is_cuda or x.shape != (n,) or not x.is_contiguous():
+        _refuse(f"{name} must be a contiguous int32 cuda tensor [{n}], not {x.dtype} {tuple(x.shape)} on {x.device}")
     return x.data_ptr()
+
+
+def _page_table(x, n):
+    """Pointer, row stride and width of an int32 page table [n, width] on the
+    GPU, its rows contiguous."""
+    if x.dtype is not _Torch.i32 or not x.is_cuda or x.dim() != 2 or x.shape[0] != n:
+        _refuse(f"pages must be an int32 cuda tensor [{n}, width], not {x.dtype} {tuple(x.shape)} on {x.device}")
+    width = x.shape[1]
+    if x.is_contiguous():
+        return x.data_ptr(), width, width
+    if x.stride(1) != 1 and width > 1:
+        _refuse("the rows of pages must be contiguous")
+    return x.data_ptr(), x.stride(0) if n > 1 else 0, width
 
 
 def _rope_tensor(table):
@@ -832,21 +845,21 @@ def rope(x, positions, table, layout="half", transpose=False, out=None, dev: Dev
     result.  out may be x."""
     if x.dim() != 3:
         _refuse("x must be [tokens, heads, d]")
-    tokens, heads, d = x.shape
     if _Torch.bf16 is None:
         _Torch.load()
+    shape = tokens, heads, d = x.shape
     dtype = x.dtype if x.dtype is _Torch.f32 else _Torch.bf16
-    xp, xt, xh = _heads_tensor(x, "x", tokens, heads, d, dtype)
+    xp, xt, xh = _heads_tensor(x, "x", shape, dtype)
     pp = _index_tensor(positions, "positions", tokens)
     tp = _rope_tensor(table)
     if out is None:
         import torch
 
-        out = torch.empty((tokens, heads, d), dtype=x.dtype, device=x.device)
-    yp, yt, yh = _heads_tensor(out, "out", tokens, heads, d, dtype)
+        out = torch.empty(shape, dtype=dtype, device=x.device)
+    yp, yt, yh = _heads_tensor(out, "out", shape, dtype)
     if tokens == 0 or heads == 0:
         return out
-    dev = dev or device(x.device.index or 0)
+    dev = dev or device(x.get_device())
     n_pos, half, _ = table.shape
     _check(lib().bsp_rope(dev.handle, xp, xt, xh, pp, tp, n_pos, tokens, heads, d, 2 * half, _rope_layout(layout),
                           1 if transpose else 0, F32 if dtype is _Torch.f32 else BF16, yp, yt, yh,
@@ -899,36 +912,35 @@ def kv_append(cache: KvCache, k, v, starts, before, pages, table=None, layout="h
     keys are rotated on the way; q [tokens, heads, d] is rotated to q_out and
     the rotated keys go to k_out where these are given (bsp_kv_append)."""
     hk, d = cache.kv_heads, cache.d
-    tokens = k.shape[0]
-    kp, kt, kh = _heads_tensor(k, "k", tokens, hk, d)
-    vp, vt, vh = _heads_tensor(v, "v", tokens, hk, d)
-    n = before.shape[0]
+    tokens, n = k.shape[0], before.shape[0]
+    shape = (tokens, hk, d)
+    ka = _heads_tensor(k, "k", shape)
+    va = _heads_tensor(v, "v", shape)
     sp = _index_tensor(starts, "starts", n + 1)
     bp = _index_tensor(before, "before", n)
-    gp = _index_tensor(pages, "pages", n, None)
-    width = pages.shape[1]
-    rot = n_pos = 0
+    gp, g_stride, width = _page_table(pages, n)
+    rot = n_pos = heads = 0
     tp = None
     if table is not None:
         tp = _rope_tensor(table)
-        n_pos, rot = table.shape[0], 2 * table.shape[1]
-    if (q is None) != (q_out is None):
-        _refuse("q and q_out come together")
-    qp = qt = qh = op = ot = oh = yp = yt = yh = None
-    heads = 0
+        n_pos, half, _ = table.shape
+        rot = 2 * half
+    qa = oa = ya = (None, 0, 0)
     if q is not None:
+        if q_out is None:
+            _refuse("q and q_out come together")
         heads = q.shape[1]
-        qp, qt, qh = _heads_tensor(q, "q", tokens, heads, d)
-        op, ot, oh = _heads_tensor(q_out, "q_out", tokens, heads, d)
+        qa = _heads_tensor(q, "q", (tokens, heads, d))
+        oa = _heads_tensor(q_out, "q_out", (tokens, heads, d))
+    elif q_out is not None:
+        _refuse("q and q_out come together")
     if k_out is not None:
-        yp, yt, yh = _heads_tensor(k_out, "k_out", tokens, hk, d)
+        ya = _heads_tensor(k_out, "k_out", shape)
     if tokens == 0 or n == 0:
         return cache
-    dev = dev or device(k.device.index or 0)
-    _check(lib().bsp_kv_append(dev.handle, cache.ref, kp, kt, kh, vp, vt, vh, tokens, n, sp, bp, gp,
-                               pages.stride(0) if n > 1 else 0, width, tp, n_pos, rot, _rope_layout(layout), qp,
-                               qt or 0, qh or 0, heads, op, ot or 0, oh or 0, yp, yt or 0, yh or 0,
-                               _stream_of(stream, dev)))
+    dev = dev or device(k.get_device())
+    _check(lib().bsp_kv_append(dev.handle, cache.ref, *ka, *va, tokens, n, sp, bp, gp, g_stride, width, tp, n_pos, rot,
+                               _rope_layout(layout), *qa, heads, *oa, *ya, _stream_of(stream, dev)))
     return cache
 
 
@@ -972,13 +984,12 @@ class PromptPlan:
     def execute(self, q, k, v, o, scale=None, lse=None, stream=None):
         """q, o: bf16 cuda [q_tokens, heads, d]; k, v [kv_tokens, kv_heads, d];
         lse (optional): f32 [q_tokens, heads]."""
-        n, m, d = self.q_tokens, self.kv_tokens, self.d
-        qa = _heads_tensor(q, "q", n, self.heads, d)
-        ka = _heads_tensor(k, "k", m, self.kv_heads, d)
-        va = _heads_tensor(v, "v", m, self.kv_heads, d)
-        oa = _heads_tensor(o, "o", n, self.heads, d)
-        _check(lib().bsp_prompt_execute(self.handle, *qa, *ka, *va, self.scale if scale is None else scale, *oa,
-                                        _lse_tensor(lse, n, self.heads), _stream_of(stream, self.dev)))
+        q_shape = n, heads, d = self.q_tokens, self.heads, self.d
+        kv_shape = (self.kv_tokens, self.kv_heads, d)
+        _check(lib().bsp_prompt_execute(
+            self.handle, *_heads_tensor(q, "q", q_shape), *_heads_tensor(k, "k", kv_shape),
+            *_heads_tensor(v, "v", kv_shape), self.scale if scale is None else scale, *_heads_tensor(o, "o", q_shape),
+            _lse_tensor(lse, n, heads), _stream_of(stream, self.dev)))
 
     def close(self):
         if self.handle:
@@ -1036,14 +1047,11 @@ class DecodePlan:
         """q, o: bf16 cuda [sequences, heads, d]; lens: int32 tokens in the
         cache; pages: int32 [sequences, width]; lse (optional): f32
         [sequences, heads]."""
-        n = q.shape[0]
-        qa = _heads_tensor(q, "q", n, self.heads, self.d)
-        oa = _heads_tensor(o, "o", n, self.heads, self.d)
-        lp = _index_tensor(lens, "lens", n)
-        gp = _index_tensor(pages, "pages", n, None)
-        _check(lib().bsp_decode_execute(self.handle, cache.ref, *qa, n, lp, gp, pages.stride(0) if n > 1 else 0,
-                                        pages.shape[1], self.scale if scale is None else scale, *oa,
-                                        _lse_tensor(lse, n, self.heads), _stream_of(stream, self.dev)))
+        shape = n, heads, d = q.shape[0], self.heads, self.d
+        _check(lib().bsp_decode_execute(
+            self.handle, cache.ref, *_heads_tensor(q, "q", shape), n, _index_tensor(lens, "lens", n),
+            *_page_table(pages, n), self.scale if scale is None else scale, *_heads_tensor(o, "o", shape),
+            _lse_tensor(lse, n, heads), _stream_of(stream, self.dev)))
 
     def close(self):
         if self.handle:

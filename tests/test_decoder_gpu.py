@@ -644,6 +644,18 @@ def test_prompt_then_tokens(bsp):
     assert float((a - b).norm() / b.norm()) <= 0.1
 
 
+def test_example(bsp):
+    """examples/serve_attention.py: prompts, then tokens, checked at its end."""
+    import importlib.util
+    import os
+
+    path = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "examples", "serve_attention.py")
+    spec = importlib.util.spec_from_file_location("serve_attention", path)
+    m = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(m)
+    assert m.main(["--steps", "5"]) < 0.1
+
+
 def test_graph_capture(bsp):
     """Every execute is captured in one graph and replayed on new inputs."""
     torch = torch_()
