@@ -247,6 +247,8 @@ __global__ void __launch_bounds__(32 * kApWarps, 2) append_kernel(const __grid_c
   const int teams = kApWarps / p.team_warps;
   const int jobs = 2 * p.cache.kv_heads + (p.q.p ? p.heads : 0);
   const int first = blockIdx.y * teams + team, step = gridDim.y * teams;
+  stream_release();
+  stream_wait();
   Chunk ck;
   if (!find_chunk(p, blockIdx.x, lane, ck)) return;
   if (ck.n > kApTokens * p.team_warps) {
@@ -358,8 +360,8 @@ bsp_status launch_append(AppendParams& p, bsp_device* dev, cudaStream_t stream) 
   const int64_t most = (jobs + teams - 1) / teams;
   const int64_t enough = 4 * static_cast<int64_t>(dev->sm_count) / (p.tokens / page + p.n_seqs) + 1;
   const dim3 grid(static_cast<unsigned>(chunks), static_cast<unsigned>(std::min(most, enough)));
-  pick(p.cache.d, p.interleaved)<<<grid, 32 * kApWarps, raw_bytes(p.cache.d), stream>>>(p);
-  return cuda_check(cudaGetLastError(), "cache append launch");
+  return launch_overlapped(pick(p.cache.d, p.interleaved), grid, 32 * kApWarps, raw_bytes(p.cache.d), stream, p,
+                           "cache append launch");
 }
 
 }  // namespace bsp

@@ -107,6 +107,13 @@ __device__ __forceinline__ bool mbar_wait_bounded(uint32_t bar, uint32_t parity,
   return mbar_wait_slow(bar, parity, ctl.abort_flag, ctl.status, ctl.timeout_ns, who);
 }
 
+// ---- overlap with the kernels before and after in the stream ----------------
+// Wait until the kernel before this one has finished and its writes are seen
+// (at once where the launch did not allow an early start).
+__device__ __forceinline__ void stream_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+// The kernel behind this one may start (it waits in its own stream_wait).
+__device__ __forceinline__ void stream_release() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
 // ---- TMA --------------------------------------------------------------------
 __device__ __forceinline__ void tma_prefetch_desc(const void* tmap) {
   asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(tmap)) : "memory");

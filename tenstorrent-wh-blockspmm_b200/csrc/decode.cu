@@ -585,8 +585,10 @@ __global__ void __launch_bounds__(kDcThreads, dc_per_sm(kD, 8 * kNt)) decode_ker
     hdr->abort_flag = 0;
     fence_mbar_init();
   }
+  if (warp == kDcTmaWarp && lane < 2) tma_prefetch_desc(lane ? &p.tm_v : &p.tm_k);
+  stream_release();
+  stream_wait();
   if (warp == kDcTmaWarp) {
-    if (lane < 2) tma_prefetch_desc(lane ? &p.tm_v : &p.tm_k);
     // tiles of all rows, then the sequence in which this CTA's stretch begins
     const int first = lane < p.n_seqs ? dc_tiles(p, lane) : 0;
     int64_t total = first;
@@ -659,7 +661,7 @@ bsp_status encode_codes(bsp_device* dev, CUtensorMap* tm, const bsp_kv_cache& c,
                    c.d == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B);
 }
 
-using DecodeKernel = void (*)(DecodeParams);
+using DecodeKernel = void (*)(const DecodeParams);
 DecodeKernel pick(int d, int group) {
   if (d == 64) return group > 8 ? decode_kernel<64, 2> : decode_kernel<64, 1>;
   return group > 8 ? decode_kernel<128, 2> : decode_kernel<128, 1>;
@@ -683,8 +685,8 @@ bsp_status launch_decode(const bsp_decode_plan* plan, DecodeParams& p, cudaStrea
   bsp_status st = encode_codes(plan->dev, &p.tm_k, p.cache, p.cache.k);
   if (st == BSP_OK) st = encode_codes(plan->dev, &p.tm_v, p.cache, p.cache.v);
   if (st != BSP_OK) return st;
-  pick(plan->d, p.group)<<<plan->grid, kDcThreads, plan->smem_bytes, stream>>>(p);
-  return cuda_check(cudaGetLastError(), "decode attention launch");
+  return launch_overlapped(pick(plan->d, p.group), dim3(plan->grid), kDcThreads, plan->smem_bytes, stream, p,
+                           "decode attention launch");
 }
 
 }  // namespace bsp

@@ -25,6 +25,9 @@ struct RopeParams {
   int32_t heads, d, rot;
   int32_t interleaved;
   float sign;            // -1: transposed rotation
+  // set at the launch: units of a head, (token, head group) items of a block,
+  // head groups of a token
+  int32_t units, items_per_block, groups;
   unsigned int* status;
 };
 
@@ -92,6 +95,25 @@ struct PromptParams {
   uint64_t timeout_ns;
 };
 
+// Launch so that the kernel may start while the one before it in the stream is
+// still finishing: it sets itself up (barriers, tensor memory, its place on an
+// SM) and calls stream_wait() before it touches what others wrote.
+template <typename P>
+inline bsp_status launch_overlapped(void (*kernel)(P), dim3 grid, int threads, int smem, cudaStream_t stream,
+                                    const P& params, const char* what) {
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = static_cast<size_t>(smem);
+  cfg.stream = stream;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return cuda_check(cudaLaunchKernelEx(&cfg, kernel, params), what);
+}
+
 }  // namespace bsp
 
 struct bsp_prompt_plan {
@@ -126,7 +148,7 @@ struct bsp_decode_plan {
 namespace bsp {
 bsp_status launch_rope_table(bsp_device* dev, int64_t n_pos, int32_t rot, double base, const bsp_rope_scaling& sc,
                              float* table, cudaStream_t stream);
-bsp_status launch_rope(const RopeParams& p, bsp_dtype type, int sm_count, cudaStream_t stream);
+bsp_status launch_rope(RopeParams& p, bsp_dtype type, int sm_count, cudaStream_t stream);
 bsp_status launch_append(AppendParams& p, bsp_device* dev, cudaStream_t stream);
 // one-time settings of the kernel that a plan launches
 bsp_status prepare_prompt(const bsp_prompt_plan* plan);

@@ -554,6 +554,8 @@ __global__ void __launch_bounds__(kPrThreads, 1) prompt_tcgen05(const __grid_con
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = hdr->tmem_base;
+  stream_release();
+  stream_wait();
   const WaitCtl ctl{&hdr->abort_flag, p.status, p.timeout_ns};
   if (warp >= kPrMmaWarp) {
     if (warp == kPrMmaWarp)
@@ -604,8 +606,8 @@ bsp_status launch_prompt(const bsp_prompt_plan* plan, PromptParams& p, cudaStrea
     if (st == BSP_OK) st = encode_heads(dev, &p.tm_v, p.v, plan->kv_tokens, plan->kv_heads, plan->d, 1, 128);
   }
   if (st != BSP_OK) return st;
-  pick(plan->d)<<<plan->grid, kPrThreads, plan->smem_bytes, stream>>>(p);
-  return cuda_check(cudaGetLastError(), "prompt attention launch");
+  return launch_overlapped(pick(plan->d), dim3(plan->grid), kPrThreads, plan->smem_bytes, stream, p,
+                           "prompt attention launch");
 }
 
 }  // namespace bsp

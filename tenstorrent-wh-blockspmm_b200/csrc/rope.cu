@@ -2,6 +2,7 @@
 // or their gradients.
 #include <math.h>
 
+#include "bsp_ptx.cuh"
 #include "rope.cuh"
 
 namespace bsp {
@@ -36,7 +37,10 @@ __global__ void rope_table_kernel(float2* table, int64_t n_pos, int half, double
 // A thread turns unit u of kHeads heads of one token: (cos, sin) are loaded
 // once for them, and kHeads loads are in flight.
 template <typename T, int kHeads>
-__global__ void __launch_bounds__(256) rope_kernel(const RopeParams p, int units, int items_per_block, int groups) {
+__global__ void __launch_bounds__(256) rope_kernel(const RopeParams p) {
+  const int units = p.units, items_per_block = p.items_per_block, groups = p.groups;
+  stream_release();
+  stream_wait();
   constexpr int kN = Vec<T>::kN;
   const int u = threadIdx.x % units, y = threadIdx.x / units;
   const uint32_t item = blockIdx.x * static_cast<uint32_t>(items_per_block) + y;
@@ -69,11 +73,13 @@ __global__ void __launch_bounds__(256) rope_kernel(const RopeParams p, int units
 }
 
 template <typename T, int kHeads>
-void run_rope(const RopeParams& p, cudaStream_t stream) {
-  const int units = p.d / (2 * Vec<T>::kN), per_block = 256 / units, groups = (p.heads + kHeads - 1) / kHeads;
-  const int64_t items = p.tokens * groups;
-  const unsigned blocks = static_cast<unsigned>((items + per_block - 1) / per_block);
-  rope_kernel<T, kHeads><<<blocks, 256, 0, stream>>>(p, units, per_block, groups);
+bsp_status run_rope(RopeParams& p, cudaStream_t stream) {
+  p.units = p.d / (2 * Vec<T>::kN);
+  p.items_per_block = 256 / p.units;
+  p.groups = (p.heads + kHeads - 1) / kHeads;
+  const int64_t items = p.tokens * p.groups;
+  const unsigned blocks = static_cast<unsigned>((items + p.items_per_block - 1) / p.items_per_block);
+  return launch_overlapped(rope_kernel<T, kHeads>, dim3(blocks), 256, 0, stream, p, "rotary kernel launch");
 }
 
 }  // namespace
@@ -87,17 +93,11 @@ bsp_status launch_rope_table(bsp_device* dev, int64_t n_pos, int32_t rot, double
   return cuda_check(cudaGetLastError(), "rotary table launch");
 }
 
-bsp_status launch_rope(const RopeParams& p, bsp_dtype type, int sm_count, cudaStream_t stream) {
+bsp_status launch_rope(RopeParams& p, bsp_dtype type, int sm_count, cudaStream_t stream) {
   // One head a thread while that does not fill the GPU (2048 threads an SM).
   const bool few = p.tokens * p.heads * (p.d / 16) < static_cast<int64_t>(sm_count) * 2048;
-  if (type == BSP_BF16) {
-    if (few) run_rope<uint16_t, 1>(p, stream);
-    else run_rope<uint16_t, 4>(p, stream);
-  } else {
-    if (few) run_rope<float, 1>(p, stream);
-    else run_rope<float, 4>(p, stream);
-  }
-  return cuda_check(cudaGetLastError(), "rotary kernel launch");
+  if (type == BSP_BF16) return few ? run_rope<uint16_t, 1>(p, stream) : run_rope<uint16_t, 4>(p, stream);
+  return few ? run_rope<float, 1>(p, stream) : run_rope<float, 4>(p, stream);
 }
 
 }  // namespace bsp
