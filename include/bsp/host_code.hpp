@@ -32,19 +32,24 @@
 
 namespace bsp {
 
+// The handle is shared with the storage made on it: a Buffer or DeviceBsr that
+// outlives CloseDevice still frees through an open handle, which closes with
+// the last of them.
 class IDevice {
  public:
   explicit IDevice(int ordinal) {
-    if (bsp_device_open(ordinal, &dev_) != BSP_OK)
+    bsp_device* d = nullptr;
+    if (bsp_device_open(ordinal, &d) != BSP_OK)
       throw std::runtime_error(std::string("bsp: cannot open device: ") + bsp_last_error_string());
+    dev_.reset(d, [](bsp_device* p) { bsp_device_close(p); });
   }
-  ~IDevice() { bsp_device_close(dev_); }
   IDevice(const IDevice&) = delete;
   IDevice& operator=(const IDevice&) = delete;
-  bsp_device* handle() const { return dev_; }
+  bsp_device* handle() const { return dev_.get(); }
+  const std::shared_ptr<bsp_device>& shared_handle() const { return dev_; }
 
  private:
-  bsp_device* dev_ = nullptr;
+  std::shared_ptr<bsp_device> dev_;
 };
 
 inline IDevice* CreateDevice(int ordinal) { return new IDevice(ordinal); }
@@ -66,19 +71,22 @@ inline void check(bsp_status s, const char* what) {
 // kept for callers that read it back; device memory is not paged here.
 class Buffer {
  public:
-  Buffer(IDevice* device, uint64_t size, uint64_t page_size) : dev_(device), size_(size), page_(page_size) {
-    check(bsp_buffer_alloc(dev_->handle(), static_cast<int64_t>(size), &ptr_), "MakeBuffer");
+  Buffer(IDevice* device, uint64_t size, uint64_t page_size)
+      : dev_(device), held_(device->shared_handle()), size_(size), page_(page_size) {
+    check(bsp_buffer_alloc(held_.get(), static_cast<int64_t>(size), &ptr_), "MakeBuffer");
   }
-  ~Buffer() { bsp_buffer_free(dev_->handle(), ptr_); }
+  ~Buffer() { bsp_buffer_free(held_.get(), ptr_); }
   Buffer(const Buffer&) = delete;
   Buffer& operator=(const Buffer&) = delete;
   void* address() const { return ptr_; }
   uint64_t size() const { return size_; }
   uint64_t page_size() const { return page_; }
-  IDevice* device() const { return dev_; }
+  bsp_device* handle() const { return held_.get(); }
+  IDevice* device() const { return dev_; }  // not valid once the device is closed
 
  private:
   IDevice* dev_;
+  std::shared_ptr<bsp_device> held_;
   void* ptr_ = nullptr;
   uint64_t size_, page_;
 };
@@ -89,14 +97,14 @@ class Buffer {
 template <typename T>
 void EnqueueWriteBuffer(Buffer& buf, const std::vector<T>& src, bool /*blocking*/ = true) {
   if (src.size() * sizeof(T) > buf.size()) throw std::runtime_error("bsp: EnqueueWriteBuffer: source larger than buffer");
-  check(bsp_buffer_write(buf.device()->handle(), buf.address(), src.data(),
+  check(bsp_buffer_write(buf.handle(), buf.address(), src.data(),
                          static_cast<int64_t>(src.size() * sizeof(T))),
         "EnqueueWriteBuffer");
 }
 template <typename T>
 void EnqueueReadBuffer(Buffer& buf, std::vector<T>& dst, bool /*blocking*/ = true) {
   dst.resize(buf.size() / sizeof(T));
-  check(bsp_buffer_read(buf.device()->handle(), dst.data(), buf.address(),
+  check(bsp_buffer_read(buf.handle(), dst.data(), buf.address(),
                         static_cast<int64_t>(dst.size() * sizeof(T))),
         "EnqueueReadBuffer");
 }
@@ -105,24 +113,25 @@ void EnqueueReadBuffer(Buffer& buf, std::vector<T>& dst, bool /*blocking*/ = tru
 // once, then run any number of plans on desc().
 class DeviceBsr {
  public:
-  DeviceBsr(IDevice* device, const bsr_matrix<bfloat16>& a, bool with_values = true) : dev_(device) {
+  DeviceBsr(IDevice* device, const bsr_matrix<bfloat16>& a, bool with_values = true)
+      : held_(device->shared_handle()) {
     std::vector<uint16_t> v;
     if (with_values) {
       v.resize(a.data.size());
       for (size_t i = 0; i < v.size(); ++i) v[i] = a.data[i].to_uint16();
     }
-    check(bsp_bsr_upload(dev_->handle(), static_cast<int64_t>(a.H), static_cast<int64_t>(a.W),
+    check(bsp_bsr_upload(held_.get(), static_cast<int64_t>(a.H), static_cast<int64_t>(a.W),
                          static_cast<int32_t>(a.R), static_cast<int32_t>(a.C), static_cast<int64_t>(a.nblocks),
                          a.indptr.data(), a.indices.data(), with_values ? v.data() : nullptr, &desc_),
           "bsp_bsr_upload");
   }
-  ~DeviceBsr() { bsp_bsr_free(dev_->handle(), &desc_); }
+  ~DeviceBsr() { bsp_bsr_free(held_.get(), &desc_); }
   DeviceBsr(const DeviceBsr&) = delete;
   DeviceBsr& operator=(const DeviceBsr&) = delete;
   const bsp_bsr_desc& desc() const { return desc_; }
 
  private:
-  IDevice* dev_;
+  std::shared_ptr<bsp_device> held_;
   bsp_bsr_desc desc_{};
 };
 
