@@ -59,10 +59,7 @@ constexpr uint32_t kPrAtom = 128 * 128;  // 128 rows x 128 bytes (64 values)
 constexpr float kPrRescale = 8.f;        // log2 of the growth that forces a rescale
 constexpr float kPrLate = 20.f;          // and of the one that cannot wait for the next step
 constexpr int kPrMaxSlots = 8;
-#ifndef PRF
-#define PRF 2
-#endif
-constexpr int kPrByFma = PRF;              // of each 8 pairs of exponentials, those in the FMA pipe
+constexpr int kPrByFma = 2;                // of each 8 pairs of exponentials, those in the FMA pipe
 
 __host__ __device__ constexpr uint32_t pr_tile(int d) { return 128u * 2u * static_cast<uint32_t>(d); }
 __host__ __device__ constexpr int pr_slots(int d) { return d == 128 ? 5 : 8; }
