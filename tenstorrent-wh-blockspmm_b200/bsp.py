@@ -1,4 +1,6 @@
-"""Python binding of libbsp.so (the C ABI in include/bsp.h), via ctypes.
+"""Python binding of libbsp.so (the C ABI in include/bsp.h), via ctypes; the
+decoder-attention entries that are called once a layer and token go through
+_bsp_calls.so (csrc/calls.cpp), which costs a call less.
 
 Device memory comes from torch tensors (torch is plumbing here: allocation,
 streams, NCCL); every multiply runs in libbsp's sm_100a kernels.  There is no
@@ -7,6 +9,7 @@ CPU or torch fallback: if libbsp.so is missing or the call fails, this raises.
 from __future__ import annotations
 
 import ctypes
+import importlib.util
 import os
 from dataclasses import dataclass
 from typing import Optional
@@ -736,82 +739,38 @@ ROPE_LAYOUTS = {"half": 0, "interleaved": 1}
 ROPE_KINDS = {"none": 0, "linear": 1, "base": 2, "parts": 3}
 
 
-class _Torch:
-    """The names of torch that every call below needs, looked up once: a call
-    costs a few microseconds, and `import torch` in each helper or a Stream
-    object for the stream's number would be most of it."""
-    bf16 = f32 = i32 = raw_stream = None
+_calls = None
 
-    @classmethod
-    def load(cls):
-        import torch
 
-        cls.bf16, cls.f32, cls.i32 = torch.bfloat16, torch.float32, torch.int32
-        raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
-        cls.raw_stream = raw or (lambda index: torch.cuda.current_stream(index).cuda_stream)
+def _load_calls():
+    """The module through which these entries are called with torch tensors
+    (csrc/calls.cpp); raises if it was not built."""
+    global _calls
+    import torch  # noqa: F401  (the module resolves its symbols)
+
+    lib()
+    path = os.path.join(HERE, "_bsp_calls.so")
+    if not os.path.exists(path):
+        raise RuntimeError(f"_bsp_calls.so not built at {path}; run __graft_entry__.build()")
+    spec = importlib.util.spec_from_file_location("_bsp_calls", path)
+    m = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(m)
+    m.setup(BspError, device)
+    _calls = m
+    return m
 
 
 def _stream_of(stream, dev: Device):
     """Stream number: the given stream, or the current one of dev's GPU."""
     if stream is None:
-        if _Torch.raw_stream is None:
-            _Torch.load()
-        return _Torch.raw_stream(dev.ordinal)
+        import torch
+
+        return torch.cuda.current_stream(dev.ordinal).cuda_stream
     return stream.cuda_stream if hasattr(stream, "cuda_stream") else int(stream)
 
 
 def _refuse(msg):
     raise BspError(BSP_ERR_INVALID_ARG, msg)
-
-
-def _heads_tensor(x, name, shape, dtype=None):
-    """Pointer, token stride and head stride of a [tokens, heads, d] operand on
-    the GPU, d contiguous; bf16 unless another type is asked for.  A dimension
-    of one entry is never stepped over: its stride counts as 0."""
-    if _Torch.bf16 is None:
-        _Torch.load()
-    if x.dtype is not (dtype or _Torch.bf16) or not x.is_cuda:
-        _refuse(f"{name} must be a {dtype or _Torch.bf16} cuda tensor, not {x.dtype} on {x.device}")
-    if x.shape != shape:
-        _refuse(f"{name} is {tuple(x.shape)}, expected {shape}")
-    tokens, heads, d = shape
-    if x.is_contiguous():
-        return x.data_ptr(), heads * d, d
-    st, sh, sd = x.stride()
-    if sd != 1 and d > 1:
-        _refuse(f"{name}: the values of a head must be contiguous")
-    return x.data_ptr(), st if tokens > 1 else 0, sh if heads > 1 else 0
-
-
-def _index_tensor(x, name, n):
-    """Pointer of an int32 tensor [n] on the GPU, contiguous."""
-    if _Torch.i32 is None:
-        _Torch.load()
-    if x.dtype is not _Torch.i32 or not x.is_cuda or x.shape != (n,) or not x.is_contiguous():
-        _refuse(f"{name} must be a contiguous int32 cuda tensor [{n}], not {x.dtype} {tuple(x.shape)} on {x.device}")
-    return x.data_ptr()
-
-
-def _page_table(x, n):
-    """Pointer, row stride and width of an int32 page table [n, width] on the
-    GPU, its rows contiguous."""
-    if x.dtype is not _Torch.i32 or not x.is_cuda or x.dim() != 2 or x.shape[0] != n:
-        _refuse(f"pages must be an int32 cuda tensor [{n}, width], not {x.dtype} {tuple(x.shape)} on {x.device}")
-    width = x.shape[1]
-    if x.is_contiguous():
-        return x.data_ptr(), width, width
-    if x.stride(1) != 1 and width > 1:
-        _refuse("the rows of pages must be contiguous")
-    return x.data_ptr(), x.stride(0) if n > 1 else 0, width
-
-
-def _rope_tensor(table):
-    if _Torch.f32 is None:
-        _Torch.load()
-    if not table.is_cuda or table.dtype is not _Torch.f32 or table.dim() != 3 or table.shape[2] != 2 \
-            or not table.is_contiguous():
-        _refuse("a rotary table is a contiguous f32 cuda tensor [positions, rot / 2, 2]")
-    return table.data_ptr()
 
 
 def _rope_layout(layout):
@@ -843,27 +802,11 @@ def rope(x, positions, table, layout="half", transpose=False, out=None, dev: Dev
     (i, i + rot/2) for "half", (2i, 2i + 1) for "interleaved"; the rest of a
     head is copied.  transpose=True gives the gradient of x from that of the
     result.  out may be x."""
-    if x.dim() != 3:
-        _refuse("x must be [tokens, heads, d]")
-    if _Torch.bf16 is None:
-        _Torch.load()
-    shape = tokens, heads, d = x.shape
-    dtype = x.dtype if x.dtype is _Torch.f32 else _Torch.bf16
-    xp, xt, xh = _heads_tensor(x, "x", shape, dtype)
-    pp = _index_tensor(positions, "positions", tokens)
-    tp = _rope_tensor(table)
     if out is None:
         import torch
 
-        out = torch.empty(shape, dtype=dtype, device=x.device)
-    yp, yt, yh = _heads_tensor(out, "out", shape, dtype)
-    if tokens == 0 or heads == 0:
-        return out
-    dev = dev or device(x.get_device())
-    n_pos, half, _ = table.shape
-    _check(lib().bsp_rope(dev.handle, xp, xt, xh, pp, tp, n_pos, tokens, heads, d, 2 * half, _rope_layout(layout),
-                          1 if transpose else 0, F32 if dtype is _Torch.f32 else BF16, yp, yt, yh,
-                          _stream_of(stream, dev)))
+        out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    (_calls or _load_calls()).rope(x, positions, table, _rope_layout(layout), bool(transpose), out, dev, stream)
     return out
 
 
@@ -890,7 +833,7 @@ class KvCache:
         ps = k.stride(0) if n > 1 else h * hs
         self.desc = KvCacheDesc(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), n, ps, hs, h,
                                 page, d)
-        self.ref = ctypes.byref(self.desc)
+        self.address = ctypes.addressof(self.desc)
         self.kv_heads, self.page, self.d = h, page, d
 
     @staticmethod
@@ -911,45 +854,9 @@ def kv_append(cache: KvCache, k, v, starts, before, pages, table=None, layout="h
     pages[s, i] is the page of its positions i * page ....  With a rotary table
     keys are rotated on the way; q [tokens, heads, d] is rotated to q_out and
     the rotated keys go to k_out where these are given (bsp_kv_append)."""
-    hk, d = cache.kv_heads, cache.d
-    tokens, n = k.shape[0], before.shape[0]
-    shape = (tokens, hk, d)
-    ka = _heads_tensor(k, "k", shape)
-    va = _heads_tensor(v, "v", shape)
-    sp = _index_tensor(starts, "starts", n + 1)
-    bp = _index_tensor(before, "before", n)
-    gp, g_stride, width = _page_table(pages, n)
-    rot = n_pos = heads = 0
-    tp = None
-    if table is not None:
-        tp = _rope_tensor(table)
-        n_pos, half, _ = table.shape
-        rot = 2 * half
-    qa = oa = ya = (None, 0, 0)
-    if q is not None:
-        if q_out is None:
-            _refuse("q and q_out come together")
-        heads = q.shape[1]
-        qa = _heads_tensor(q, "q", (tokens, heads, d))
-        oa = _heads_tensor(q_out, "q_out", (tokens, heads, d))
-    elif q_out is not None:
-        _refuse("q and q_out come together")
-    if k_out is not None:
-        ya = _heads_tensor(k_out, "k_out", shape)
-    if tokens == 0 or n == 0:
-        return cache
-    dev = dev or device(k.get_device())
-    _check(lib().bsp_kv_append(dev.handle, cache.ref, *ka, *va, tokens, n, sp, bp, gp, g_stride, width, tp, n_pos, rot,
-                               _rope_layout(layout), *qa, heads, *oa, *ya, _stream_of(stream, dev)))
+    (_calls or _load_calls()).kv_append(cache, k, v, starts, before, pages, table, _rope_layout(layout), q, q_out,
+                                        k_out, dev, stream)
     return cache
-
-
-def _lse_tensor(lse, tokens, heads):
-    if lse is None:
-        return None
-    if not lse.is_cuda or lse.dtype is not _Torch.f32 or lse.shape != (tokens, heads) or not lse.is_contiguous():
-        _refuse(f"lse must be a contiguous f32 cuda tensor {(tokens, heads)}")
-    return lse.data_ptr()
 
 
 PROMPT_INFO_KEYS = ["units", "ctas", "q_tokens", "kv_tokens", "heads", "kv_heads", "d", "tiles", "plan_bytes",
@@ -984,12 +891,8 @@ class PromptPlan:
     def execute(self, q, k, v, o, scale=None, lse=None, stream=None):
         """q, o: bf16 cuda [q_tokens, heads, d]; k, v [kv_tokens, kv_heads, d];
         lse (optional): f32 [q_tokens, heads]."""
-        q_shape = n, heads, d = self.q_tokens, self.heads, self.d
-        kv_shape = (self.kv_tokens, self.kv_heads, d)
-        _check(lib().bsp_prompt_execute(
-            self.handle, *_heads_tensor(q, "q", q_shape), *_heads_tensor(k, "k", kv_shape),
-            *_heads_tensor(v, "v", kv_shape), self.scale if scale is None else scale, *_heads_tensor(o, "o", q_shape),
-            _lse_tensor(lse, n, heads), _stream_of(stream, self.dev)))
+        (_calls or _load_calls()).prompt(self, self.dev.ordinal, q, k, v, o, self.scale if scale is None else scale,
+                                         lse, stream)
 
     def close(self):
         if self.handle:
@@ -1047,11 +950,8 @@ class DecodePlan:
         """q, o: bf16 cuda [sequences, heads, d]; lens: int32 tokens in the
         cache; pages: int32 [sequences, width]; lse (optional): f32
         [sequences, heads]."""
-        shape = n, heads, d = q.shape[0], self.heads, self.d
-        _check(lib().bsp_decode_execute(
-            self.handle, cache.ref, *_heads_tensor(q, "q", shape), n, _index_tensor(lens, "lens", n),
-            *_page_table(pages, n), self.scale if scale is None else scale, *_heads_tensor(o, "o", shape),
-            _lse_tensor(lse, n, heads), _stream_of(stream, self.dev)))
+        (_calls or _load_calls()).decode(self, self.dev.ordinal, cache, q, lens, pages, o,
+                                         self.scale if scale is None else scale, lse, stream)
 
     def close(self):
         if self.handle:
