@@ -35,11 +35,14 @@ struct Chunk {
 };
 
 // Chunk c of the launch: sequence s owns the chunks from starts[s] / page + 2 s
-// on (it touches at most (starts[s + 1] - starts[s]) / page + 2 pages), so the
-// sequence is found by a search in steps of 32 and no host copy of the lengths
-// is needed.
+// on (it touches at most (starts[s + 1] - starts[s]) / page + 2 pages), or from
+// starts[s] on where that is fewer in all (it touches at most a page a token: a
+// token each of 64 sequences takes 4.9 us that way, 6.0 us with twice as many
+// blocks, half of them without a chunk).  So the sequence is found by a search in
+// steps of 32 and no host copy of the lengths is needed.
 __device__ __forceinline__ int64_t first_chunk(const AppendParams& p, int s) {
-  return (static_cast<int64_t>(__ldg(p.starts + s)) >> p.page_shift) + 2 * static_cast<int64_t>(s);
+  const int64_t start = __ldg(p.starts + s);
+  return p.by_token ? start : (start >> p.page_shift) + 2 * static_cast<int64_t>(s);
 }
 __device__ __forceinline__ bool find_chunk(const AppendParams& p, int64_t c, int lane, Chunk& out) {
   const int page = p.cache.page;
@@ -56,7 +59,7 @@ __device__ __forceinline__ bool find_chunk(const AppendParams& p, int64_t c, int
     if (lane == 0) atomicOr(p.status, ST_BAD_INDEX);
     return false;
   }
-  const int64_t local = c - ((t0 >> p.page_shift) + 2 * static_cast<int64_t>(lo));
+  const int64_t local = c - (p.by_token ? t0 : (t0 >> p.page_shift) + 2 * static_cast<int64_t>(lo));
   const int64_t off = b & (page - 1);
   if (local < 0 || n == 0 || local >= (off + n + page - 1) >> p.page_shift) return false;
   const int64_t index = (b >> p.page_shift) + local;
@@ -350,15 +353,18 @@ bsp_status launch_append(AppendParams& p, bsp_device* dev, cudaStream_t stream) 
   const int64_t per_seq = p.tokens / p.n_seqs;
   p.team_warps = 1;
   while (p.team_warps * 2 * kApTokens <= std::min<int64_t>(per_seq, page)) p.team_warps *= 2;
-  const int64_t chunks = p.tokens / page + 2 * static_cast<int64_t>(p.n_seqs);
+  const int64_t by_page = p.tokens / page + 2 * static_cast<int64_t>(p.n_seqs);
+  p.by_token = p.tokens < by_page;
+  const int64_t chunks = std::min(p.tokens, by_page);
   if (chunks > 0x7FFFFFFF) return set_error(BSP_ERR_UNSUPPORTED, "too many sequences");
   const int jobs = 2 * p.cache.kv_heads + (p.q.p ? p.heads : 0);
   const int teams = kApWarps / p.team_warps;
-  // A job to a team while that is needed to fill the GPU, else several: 14278
-  // tokens in pages of 16 take 68 us with one block to a chunk (of 904), 74 us
-  // with three and 96 us with six.
+  // A job to a team while that does not need more blocks than the GPU holds at
+  // once (two an SM), else several: 14278 tokens in pages of 16 take 68 us with
+  // one block to a chunk (of 904), 74 us with three and 96 us with six; a token
+  // each of 64 sequences 4.9 us with four blocks to a chunk, 5.1 us with six.
   const int64_t most = (jobs + teams - 1) / teams;
-  const int64_t enough = 4 * static_cast<int64_t>(dev->sm_count) / (p.tokens / page + p.n_seqs) + 1;
+  const int64_t enough = std::max<int64_t>(2 * static_cast<int64_t>(dev->sm_count) / (p.tokens / page + p.n_seqs), 1);
   const dim3 grid(static_cast<unsigned>(chunks), static_cast<unsigned>(std::min(most, enough)));
   return launch_overlapped(pick(p.cache.d, p.interleaved), grid, 32 * kApWarps, raw_bytes(p.cache.d), stream, p,
                            "cache append launch");
