@@ -518,9 +518,15 @@ bsp_status bsp_kv_append(bsp_device* dev, const bsp_kv_cache* cache, const void*
  * every key.  A query that sees no key gets O = 0 and lse = -inf.  lse (may be
  * NULL): float [tokens][heads], the log of the sum of exp(scale q k).
  * A plan belongs to one set of lengths (host arrays) and head counts and
- * serves every layer and step of that batch, on any stream.  d 64 or 128.
+ * serves every layer and step of that batch.  d 64 or 128.  Few rows of many
+ * keys are cut along the keys: such a plan has a workspace (info[12] > 0), in
+ * which the parts' results meet, so run its launches one after the other (on
+ * one stream); any other plan may run on several streams at once.
  * Scores, softmax and sums in fp32; probabilities are rounded to bf16 for the
- * product with V; O is rounded once.  Options: max_ctas, timeout_ms. */
+ * product with V; O is rounded once.  A hidden key may hold anything, but V is
+ * multiplied in steps of 128 keys with weights that are 0 for hidden ones: a NaN
+ * or infinity in V reaches the rows that see any key of its step.
+ * Options: max_ctas, timeout_ms, group_rows = -1 (nothing is cut). */
 typedef struct bsp_prompt_plan bsp_prompt_plan;
 
 bsp_status bsp_prompt_plan_create(bsp_device* dev, int32_t n_seqs, const int32_t* q_lens, const int32_t* kv_lens,
@@ -533,7 +539,8 @@ bsp_status bsp_prompt_execute(const bsp_prompt_plan* plan, const void* q, int64_
 bsp_status bsp_prompt_plan_destroy(bsp_prompt_plan* plan);
 /* info[0] work units, [1] grid, [2] query tokens, [3] key tokens, [4] heads,
  * [5] kv_heads, [6] d, [7] key tiles over all units, [8] table bytes,
- * [9] shared memory, [10] TMEM columns, [11] heads packed into a tile's rows. */
+ * [9] shared memory, [10] TMEM columns, [11] heads packed into a tile's rows,
+ * [12] workspace bytes (0: nothing is cut). */
 bsp_status bsp_prompt_plan_info(const bsp_prompt_plan* plan, int64_t info[16]);
 
 /* Attention of one new token of each sequence over the cache: q, o

@@ -104,7 +104,8 @@ bsp_status bsp_testing_spmm_counters(const bsp_spmm_plan* plan, void** counters,
 bsp_status bsp_testing_spmm_drop_stage(bsp_spmm_plan* plan, int32_t stage_plus_one);
 
 /* The prompt attention planner (host only): units_out[info[0] * 12] (q0,
- * q_end, kv0, kv_len, sees, head0, steps of tile a and b, two tiles, pad[3]) in
+ * q_end, kv0, kv_len, sees, head0, steps of tile a and b, two tiles, parts,
+ * part, first workspace slot; the keys of a part count from its own first) in
  * CTA order, cta_begin_out[info[1] + 1]; info as bsp_prompt_plan_info. */
 bsp_status bsp_prompt_plan_inspect(int32_t n_seqs, const int32_t* q_lens, const int32_t* kv_lens, int32_t heads,
                                    int32_t kv_heads, int32_t d, int32_t causal, const bsp_spmm_opts* opts,

@@ -860,13 +860,15 @@ def kv_append(cache: KvCache, k, v, starts, before, pages, table=None, layout="h
 
 
 PROMPT_INFO_KEYS = ["units", "ctas", "q_tokens", "kv_tokens", "heads", "kv_heads", "d", "tiles", "plan_bytes",
-                    "smem_bytes", "tmem_cols", "packed_heads"]
+                    "smem_bytes", "tmem_cols", "packed_heads", "workspace_bytes"]
 
 
 class PromptPlan:
     """Attention over whole prompts packed one after the other: q_lens[s]
     queries and kv_lens[s] keys of sequence s (host lists); causal: query i
-    sees the keys up to i + (kv_len - q_len)."""
+    sees the keys up to i + (kv_len - q_len).  A plan with a workspace
+    (info()["workspace_bytes"]: few rows of many keys are cut along the keys)
+    runs on one stream at a time."""
 
     def __init__(self, dev: Device, q_lens, kv_lens, heads, kv_heads, d, causal=True, opts=None):
         ql = np.ascontiguousarray(q_lens, dtype=np.int32)

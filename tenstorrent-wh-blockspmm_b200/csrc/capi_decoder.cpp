@@ -244,18 +244,23 @@ bsp_status bsp_prompt_plan_create(bsp_device* dev, int32_t n_seqs, const int32_t
   p->smem_bytes = prompt_smem_bytes(d);
   if (s == BSP_OK && p->n_units > 0) {
     OnDevice on(dev->ordinal);
-    const size_t ub = p->h_units.size() * sizeof(PromptUnit);
-    p->blob_bytes = ub + p->h_cta_begin.size() * sizeof(int32_t);
+    const size_t ub = p->h_units.size() * sizeof(PromptUnit), jb = p->h_joins.size() * sizeof(PromptUnit);
+    const size_t cb = p->h_cta_begin.size() * sizeof(int32_t), tables = (ub + jb + cb + 255) / 256 * 256;
+    p->blob_bytes = tables + static_cast<size_t>(p->slots * prompt_slot_floats(d)) * sizeof(float);
     s = plan_alloc(dev->ordinal, p->blob_bytes, &p->d_blob);
     if (s == BSP_OK) {
-      p->d_units = static_cast<PromptUnit*>(p->d_blob);
-      p->d_cta_begin = reinterpret_cast<int32_t*>(static_cast<uint8_t*>(p->d_blob) + ub);
-      s = cuda_check(cudaMemcpyAsync(p->d_units, p->h_units.data(), ub, cudaMemcpyHostToDevice, nullptr),
-                     "upload plan tables");
-      if (s == BSP_OK)
-        s = cuda_check(cudaMemcpyAsync(p->d_cta_begin, p->h_cta_begin.data(), p->h_cta_begin.size() * sizeof(int32_t),
-                                       cudaMemcpyHostToDevice, nullptr),
-                       "upload plan tables");
+      uint8_t* at = static_cast<uint8_t*>(p->d_blob);
+      p->d_units = reinterpret_cast<PromptUnit*>(at);
+      p->d_joins = reinterpret_cast<PromptUnit*>(at + ub);
+      p->d_cta_begin = reinterpret_cast<int32_t*>(at + ub + jb);
+      p->d_work = reinterpret_cast<float*>(at + tables);
+      auto upload = [&](void* dst, const void* src, size_t bytes) {
+        if (s == BSP_OK && bytes > 0)
+          s = cuda_check(cudaMemcpyAsync(dst, src, bytes, cudaMemcpyHostToDevice, nullptr), "upload plan tables");
+      };
+      upload(p->d_units, p->h_units.data(), ub);
+      upload(p->d_joins, p->h_joins.data(), jb);
+      upload(p->d_cta_begin, p->h_cta_begin.data(), cb);
       if (s == BSP_OK) s = cuda_check(cudaStreamSynchronize(nullptr), "upload plan tables");
       if (s == BSP_OK) s = prepare_prompt(p);
     }
@@ -290,6 +295,8 @@ bsp_status bsp_prompt_execute(const bsp_prompt_plan* plan, const void* q, int64_
   p.lse = lse;
   p.units = plan->d_units;
   p.cta_begin = plan->d_cta_begin;
+  p.work = plan->d_work;
+  p.joins = plan->d_joins;
   p.heads = plan->heads;
   p.group = plan->heads / plan->kv_heads;
   p.packed = plan->packed;
@@ -324,6 +331,7 @@ bsp_status bsp_prompt_plan_info(const bsp_prompt_plan* p, int64_t info[16]) {
   info[9] = p->smem_bytes;
   info[10] = 512;
   info[11] = p->packed;
+  info[12] = p->slots * prompt_slot_floats(p->d) * static_cast<int64_t>(sizeof(float));
   return BSP_OK;
 }
 

@@ -77,7 +77,10 @@ struct PromptUnit {
   int32_t head0;         // first query head
   int32_t n[2];          // steps of 128 keys of tile a and b (0: the tile sees no key)
   int32_t two;           // the unit has a tile b
-  int32_t pad[3];
+  // A unit may be one part of a block's keys: kv0, kv_len and sees then count
+  // from the part's first key, n its steps.
+  int32_t parts, part;   // 1, 0: the whole
+  int32_t first;         // first of the block's 2 x parts workspace slots (tile t of part k: 2 k + t)
 };
 static_assert(sizeof(PromptUnit) == 48, "unit layout");
 
@@ -88,6 +91,8 @@ struct PromptParams {
   float* lse;
   const PromptUnit* units;
   const int32_t* cta_begin;       // [grid + 1]
+  float* work;                    // slots of 128 rows: O [d / 4][128][4], exponents' reference [128], sums [128]
+  const PromptUnit* joins;        // the blocks that are cut, their part 0
   int32_t heads, group;           // group: query heads of one key/value head
   int32_t packed, tile_tokens;
   int32_t causal;
@@ -126,11 +131,14 @@ struct bsp_prompt_plan {
   int32_t grid = 0, smem_bytes = 0;
   int64_t n_units = 0, n_tiles = 0;
   uint64_t timeout_ns = 0;
-  void* d_blob = nullptr;  // units | cta_begin
+  int64_t slots = 0;       // workspace slots of the blocks that are cut
+  void* d_blob = nullptr;  // units | joins | cta_begin | workspace
   size_t blob_bytes = 0;
   bsp::PromptUnit* d_units = nullptr;
   int32_t* d_cta_begin = nullptr;
-  std::vector<bsp::PromptUnit> h_units;
+  bsp::PromptUnit* d_joins = nullptr;
+  float* d_work = nullptr;
+  std::vector<bsp::PromptUnit> h_units, h_joins;
   std::vector<int32_t> h_cta_begin;
 };
 
@@ -162,4 +170,5 @@ bsp_status plan_prompt_host(bsp_prompt_plan* p, const int32_t* q_lens, const int
                             const bsp_spmm_opts* opts);
 bsp_status launch_prompt(const bsp_prompt_plan* plan, PromptParams& p, cudaStream_t stream);
 int prompt_smem_bytes(int d);
+__host__ __device__ constexpr int64_t prompt_slot_floats(int d) { return 128 * (static_cast<int64_t>(d) + 2); }
 }  // namespace bsp

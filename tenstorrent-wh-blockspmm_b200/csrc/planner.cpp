@@ -2470,6 +2470,7 @@ bsp_status plan_prompt_host(bsp_prompt_plan* p, const int32_t* q_lens, const int
       u.kv_len = kv_lens[s];
       u.sees = static_cast<int32_t>(kv_lens[s] - q_lens[s] + a + 1);
       u.two = tiles == 2 && a + p->tile_tokens < q_lens[s];
+      u.parts = 1;
       for (int t = 0; t <= u.two; ++t) {
         // keys of the tile's last query
         const int64_t last = std::min<int64_t>(a + (t + 1) * p->tile_tokens, q_lens[s]) - 1;
@@ -2488,21 +2489,100 @@ bsp_status plan_prompt_host(bsp_prompt_plan* p, const int32_t* q_lens, const int
   // A step takes the time of one tile's chain of products and softmax, whether
   // the other tile takes part or not (3200 and 3300 cycles measured); a unit's
   // start and epilogue take about one step more.
-  auto cost = [](const PromptUnit& u) {
-    return 32 * int64_t(std::max(u.n[0], u.n[1])) + std::min(u.n[0], u.n[1]) + 32;
+  auto cost = [](int32_t n0, int32_t n1) { return 32 * int64_t(std::max(n0, n1)) + std::min(n0, n1) + 32; };
+  // Part k of a unit cut into `parts`: steps [from, to).
+  auto part_of = [](const PromptUnit& u, int32_t parts, int32_t k, int32_t (&n)[2]) {
+    const int64_t steps = std::max(u.n[0], u.n[1]);
+    const int32_t from = static_cast<int32_t>(steps * k / parts), to = static_cast<int32_t>(steps * (k + 1) / parts);
+    for (int t = 0; t < 2; ++t) n[t] = std::max(std::min(u.n[t], to) - from, 0);
+    return from;
   };
-  std::stable_sort(units.begin(), units.end(),
-                   [&](const PromptUnit& x, const PromptUnit& y) { return cost(x) > cost(y); });
-  ctas = static_cast<int>(std::min<int64_t>(ctas, static_cast<int64_t>(units.size())));
-  std::priority_queue<std::pair<int64_t, int>, std::vector<std::pair<int64_t, int>>, std::greater<>> least;
-  for (int c = 0; c < ctas; ++c) least.push({0, c});
-  std::vector<std::vector<int32_t>> mine(static_cast<size_t>(std::max(ctas, 1)));
-  for (size_t i = 0; i < units.size(); ++i) {
-    const auto [load, c] = least.top();
-    least.pop();
-    mine[static_cast<size_t>(c)].push_back(static_cast<int32_t>(i));
-    least.push({load + cost(units[i]), c});
+  auto parts_of = [](const PromptUnit& u, int64_t len) {
+    return static_cast<int32_t>(std::max<int64_t>((std::max(u.n[0], u.n[1]) + len - 1) / len, 1));
+  };
+  using Load = std::pair<int64_t, int32_t>;
+  // Deal items, heaviest first, to the least loaded CTA; the largest load.
+  std::vector<std::vector<int32_t>> mine;
+  auto deal = [&](std::vector<Load>& items, bool keep) {
+    std::stable_sort(items.begin(), items.end(), [](const Load& x, const Load& y) { return x.first > y.first; });
+    const size_t n = std::min(static_cast<size_t>(ctas), items.size());
+    std::priority_queue<Load, std::vector<Load>, std::greater<>> least;
+    for (size_t c = 0; c < n; ++c) least.push({0, static_cast<int32_t>(c)});
+    if (keep) mine.assign(n, {});
+    int64_t most = 0;
+    for (const Load& x : items) {
+      const auto [load, c] = least.top();
+      least.pop();
+      if (keep) mine[static_cast<size_t>(c)].push_back(x.second);
+      least.push({load + x.first, c});
+      most = std::max(most, load + x.first);
+    }
+    return most;
+  };
+  std::vector<Load> items;
+  int64_t total = 0, steps = 0;
+  for (const PromptUnit& u : units) {
+    items.push_back({cost(u.n[0], u.n[1]), static_cast<int32_t>(items.size())});
+    total += items.back().first;
+    steps += std::max(u.n[0], u.n[1]);
   }
+  int64_t best = deal(items, true);
+  // Few rows of many keys would leave CTAs idle: cut the blocks' keys into parts
+  // of at most `len` steps where that ends sooner.  A part writes its rows to the
+  // workspace, which takes most of a step, and a second kernel joins them: a step
+  // and a half for its launch, and its traffic.  16 tokens behind 32768 keys (32
+  // heads, 8 of keys) take 39 us so, whole 395 us; 1000 tokens of 4 heads 12 us,
+  // whole 18 us.
+  int64_t best_len = 0;
+  if (!(opts && opts->group_rows < 0) && ctas > 0 && best > total / ctas + 64) {
+    const double even = static_cast<double>(steps) / ctas;
+    for (const double f : {1.03, 1.25, 1.6, 2.2, 3.2, 0.6}) {
+      const int64_t len = std::max<int64_t>(static_cast<int64_t>(std::ceil(even * f)), 2);
+      items.clear();
+      int64_t slots = 0;
+      int32_t most = 1;
+      for (const PromptUnit& u : units) {
+        const int32_t parts = parts_of(u, len);
+        if (parts > 1) slots += 2 * parts;
+        most = std::max(most, parts);
+        for (int32_t k = 0; k < parts; ++k) {
+          int32_t n[2];
+          part_of(u, parts, k, n);
+          items.push_back({cost(n[0], n[1]) + (parts > 1 ? 24 : 0), 0});
+        }
+      }
+      if (slots == 0 || slots > 8 * static_cast<int64_t>(ctas)) continue;
+      const int64_t end = deal(items, false) + 48 + slots / 3 + 2 * most;
+      if (end < best) {
+        best = end;
+        best_len = len;
+      }
+    }
+  }
+  if (best_len > 0) {
+    std::vector<PromptUnit> cut;
+    items.clear();
+    for (const PromptUnit& u : units) {
+      const int32_t parts = parts_of(u, best_len);
+      for (int32_t k = 0; k < parts; ++k) {
+        PromptUnit x = u;
+        const int32_t from = part_of(u, parts, k, x.n);
+        x.kv0 += 128 * from;
+        x.kv_len -= 128 * from;
+        x.sees -= 128 * from;
+        x.parts = parts;
+        x.part = k;
+        x.first = static_cast<int32_t>(p->slots);
+        items.push_back({cost(x.n[0], x.n[1]) + (parts > 1 ? 24 : 0), static_cast<int32_t>(cut.size())});
+        cut.push_back(x);
+        if (parts > 1 && k == 0) p->h_joins.push_back(x);
+      }
+      if (parts > 1) p->slots += 2 * parts;
+    }
+    units.swap(cut);
+    deal(items, true);
+  }
+  ctas = static_cast<int>(mine.size());
   p->h_units.reserve(units.size());
   p->h_cta_begin.assign(1, 0);
   for (int c = 0; c < ctas; ++c) {

@@ -359,6 +359,16 @@ __device__ __forceinline__ float pr_weights(uint32_t (&a)[32], uint32_t (&b)[32]
   return p + q;
 }
 
+// What a row's sums are multiplied with: 1 / l; 0 where the row saw no key (l is
+// 0 then).  A NaN or infinite score makes m NaN or infinite, and the row NaN.
+__device__ __forceinline__ float share_of(float m, float& l) {
+  if (!(m < INFINITY)) l = __uint_as_float(0x7FC00000u);
+  return l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);  // a NaN sum stays one
+}
+__device__ __forceinline__ float lse_of(float m, float l) {
+  return l == 0.f ? -INFINITY : m * 0.6931471805599453f + logf(l);
+}
+
 template <int kD>
 __device__ __forceinline__ void pr_softmax(const PromptParams& p, PrHeader* hdr, uint8_t* ring_ptr, uint32_t tmem,
                                           int u0, int u1, const WaitCtl& ctl, int warp, int lane) {
@@ -390,9 +400,13 @@ __device__ __forceinline__ void pr_softmax(const PromptParams& p, PrHeader* hdr,
     const bool valid = token < un.q_end && (t == 0 || un.two);
     uint16_t* orow = static_cast<uint16_t*>(p.o.p) + token * p.o.token + (un.head0 + dh) * p.o.head;
     float* lrow = p.lse ? p.lse + token * p.heads + un.head0 + dh : nullptr;
+    float* work = p.work + (static_cast<int64_t>(un.first) + 2 * un.part + t) * prompt_slot_floats(kD);
     if (n == 0) {
       slot_n += 2 * max(un.n[0], un.n[1]);
-      if (valid) {
+      if (valid && un.parts > 1) {
+        work[128 * kD + row] = -INFINITY;
+        work[128 * kD + 128 + row] = 0.f;
+      } else if (valid) {
         for (int c = 0; c < kD / 8; ++c) reinterpret_cast<uint4*>(orow)[c] = make_uint4(0, 0, 0, 0);
         if (lrow) *lrow = -INFINITY;
       }
@@ -492,19 +506,29 @@ __device__ __forceinline__ void pr_softmax(const PromptParams& p, PrHeader* hdr,
     ++outs;
     tc_fence_after();
     if (m == -INFINITY && l < 1.f) l = 0.f;  // no key: exp2_pair gave 2^-126 for each masked one
-    if (!(m < INFINITY)) l = __uint_as_float(0x7FC00000u);  // a NaN or infinite score: the row is NaN
-    const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);  // a NaN sum stays one
+    const bool whole = un.parts == 1;
+    const float inv = whole ? share_of(m, l) : 1.f;
 #pragma unroll 1
     for (int c = 0; c < kD / 32; ++c) {
       uint32_t o[32];
       tmem_ld_32x32b_x32(t_o + 32u * c, o);
       tmem_ld_wait();
-      if (valid) {
+      if (valid && !whole) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          reinterpret_cast<uint4*>(work)[(8 * c + i) * 128 + row] =
+              make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+      } else if (valid) {
         store32(orow + 32 * c, o, 0, inv);
         store32(orow + 32 * c + 16, o, 16, inv);
       }
     }
-    if (valid && lrow) *lrow = l == 0.f ? -INFINITY : m * 0.6931471805599453f + logf(l);
+    if (valid && !whole) {
+      work[128 * kD + row] = m;
+      work[128 * kD + 128 + row] = l;
+    } else if (valid && lrow) {
+      *lrow = lse_of(m, l);
+    }
     tc_fence_before();
     __syncwarp();
     if (lane == 0) mbar_arrive(baddr(&hdr->o_empty[t]));
@@ -570,6 +594,68 @@ __global__ void __launch_bounds__(kPrThreads, 1) prompt_tcgen05(const __grid_con
   }
 }
 
+// The parts of the blocks that are cut, joined in their order:
+//   m = max m_k,  l = sum 2^(m_k - m) l_k,  O = sum 2^(m_k - m) O_k / l.
+// A thread takes 16 columns of a row of tile blockIdx.x & 1.
+constexpr int kPrDeep = 4;  // parts whose loads are in flight
+template <int kD>
+__global__ void __launch_bounds__(256) prompt_join(const __grid_constant__ PromptParams p) {
+  constexpr int kGroups = kD / 16, kRows = 256 / kGroups;
+  const int t = blockIdx.x & 1, row = blockIdx.y * kRows + threadIdx.x % kRows, g = threadIdx.x / kRows;
+  const PromptUnit un = p.joins[blockIdx.x >> 1];
+  const int token = un.q0 + t * p.tile_tokens + row / p.packed, head = un.head0 + row % p.packed;
+  stream_release();
+  stream_wait();
+  if (token >= un.q_end || (t == 1 && !un.two)) return;
+  const int64_t stride = 2 * prompt_slot_floats(kD);
+  const float* work = p.work + (static_cast<int64_t>(un.first) + t) * prompt_slot_floats(kD);
+  const float* ms = work + 128 * kD + row;
+  const float4* src = reinterpret_cast<const float4*>(work) + 4 * g * 128 + row;
+  float m = -INFINITY, l = 0.f, sum[16];
+#pragma unroll
+  for (int i = 0; i < 16; ++i) sum[i] = 0.f;
+  for (int k0 = 0; k0 < un.parts; k0 += kPrDeep) {
+    float4 v[kPrDeep][4];
+    float mk[kPrDeep], lk[kPrDeep];
+#pragma unroll
+    for (int k = 0; k < kPrDeep; ++k) {
+      const bool have = k0 + k < un.parts;
+      mk[k] = have ? __ldcg(ms + (k0 + k) * stride) : -INFINITY;
+      lk[k] = have ? __ldcg(ms + (k0 + k) * stride + 128) : 0.f;
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        v[k][i] = have ? __ldcg(src + (k0 + k) * (stride / 4) + i * 128) : make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+    float top = m;
+#pragma unroll
+    for (int k = 0; k < kPrDeep; ++k) top = max3(top, mk[k], mk[k]);
+    const float f0 = m == -INFINITY ? 0.f : ex2(m - top);
+    m = top;
+    l *= f0;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) sum[i] *= f0;
+#pragma unroll
+    for (int k = 0; k < kPrDeep; ++k) {
+      if (mk[k] == -INFINITY) continue;  // a part without keys has written no sums
+      const float f = ex2(mk[k] - m);
+      l += f * lk[k];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        sum[4 * i] += f * v[k][i].x, sum[4 * i + 1] += f * v[k][i].y;
+        sum[4 * i + 2] += f * v[k][i].z, sum[4 * i + 3] += f * v[k][i].w;
+      }
+    }
+  }
+  const float inv = share_of(m, l);
+  uint32_t w[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) w[i] = pack2(sum[2 * i] * inv, sum[2 * i + 1] * inv);
+  uint16_t* dst = static_cast<uint16_t*>(p.o.p) + token * p.o.token + head * p.o.head + 16 * g;
+  *reinterpret_cast<uint4*>(dst) = make_uint4(w[0], w[1], w[2], w[3]);
+  *reinterpret_cast<uint4*>(dst + 8) = make_uint4(w[4], w[5], w[6], w[7]);
+  if (g == 0 && p.lse) p.lse[static_cast<int64_t>(token) * p.heads + head] = lse_of(m, l);
+}
+
 // Tensor map of a [tokens][heads][d] operand, box {64, box_heads, box_tokens}.
 // A dimension of one entry is never stepped over: its stride is any valid one.
 bsp_status encode_heads(bsp_device* dev, CUtensorMap* tm, const HeadsView& x, int64_t tokens, int heads, int d,
@@ -603,8 +689,12 @@ bsp_status launch_prompt(const bsp_prompt_plan* plan, PromptParams& p, cudaStrea
     if (st == BSP_OK) st = encode_heads(dev, &p.tm_v, p.v, plan->kv_tokens, plan->kv_heads, plan->d, 1, 128);
   }
   if (st != BSP_OK) return st;
-  return launch_overlapped(pick(plan->d), dim3(plan->grid), kPrThreads, plan->smem_bytes, stream, p,
-                           "prompt attention launch");
+  st = launch_overlapped(pick(plan->d), dim3(plan->grid), kPrThreads, plan->smem_bytes, stream, p,
+                         "prompt attention launch");
+  if (st != BSP_OK || plan->h_joins.empty()) return st;
+  return launch_overlapped(plan->d == 64 ? prompt_join<64> : prompt_join<128>,
+                           dim3(2 * static_cast<unsigned>(plan->h_joins.size()), plan->d / 32), 256, 0, stream, p,
+                           "prompt join launch");
 }
 
 }  // namespace bsp

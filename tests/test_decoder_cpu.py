@@ -22,8 +22,9 @@ CASES = [([1], [1], 1, 1), ([37], [37], 8, 2), ([2048, 513, 1, 0, 96], [2048, 70
 @pytest.mark.parametrize("causal", [True, False])
 @pytest.mark.parametrize("max_ctas", [0, 5])
 def test_prompt_units_cover_every_row_and_key_once(ql, kl, heads, kv_heads, causal, max_ctas):
-    plan, units, cta = inspect(ql, kl, heads, kv_heads, causal=causal, max_ctas=max_ctas)
+    plan, units, cta = inspect(ql, kl, heads, kv_heads, causal=causal, max_ctas=max_ctas, group_rows=-1)
     packed = plan["packed_heads"]
+    assert (units[:, 9] == 1).all() and plan["workspace_bytes"] == 0
     tokens = 128 // packed
     assert (heads // kv_heads) % packed == 0 and cta[0] == 0 and cta[-1] == len(units) and (np.diff(cta) > 0).all()
     starts_q, starts_k = np.concatenate([[0], np.cumsum(ql)]), np.concatenate([[0], np.cumsum(kl)])
@@ -48,6 +49,40 @@ def test_prompt_units_cover_every_row_and_key_once(ql, kl, heads, kv_heads, caus
     cost = 32 * units[:, 6:8].max(1) + units[:, 6:8].min(1) + 32
     loads = [cost[a:b].sum() for a, b in zip(cta[:-1], cta[1:])]
     assert max(loads) <= cost.sum() / len(loads) + cost.max()
+
+
+@pytest.mark.parametrize("ql,kl,heads,kv_heads", CASES + [([16], [32768], 32, 8), ([2, 1], [600, 30000], 4, 2),
+                                                          ([300, 1], [200, 131072], 5, 1)])
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("max_ctas", [0, 5])
+def test_prompt_cut_units_join_to_the_whole(ql, kl, heads, kv_heads, causal, max_ctas):
+    """The parts of a unit that is cut are the whole plan's unit: the same rows,
+    its steps one after the other, each with a workspace slot of its own."""
+    whole = inspect(ql, kl, heads, kv_heads, causal=causal, max_ctas=max_ctas, group_rows=-1)[1]
+    plan, units, cta = inspect(ql, kl, heads, kv_heads, causal=causal, max_ctas=max_ctas)
+    assert cta[0] == 0 and cta[-1] == len(units) and (np.diff(cta) > 0).all()
+    rows = {}
+    for u in units.tolist():
+        rows.setdefault((u[0], u[5]), []).append(u)
+    assert sorted(rows) == sorted((u[0], u[5]) for u in whole.tolist())
+    slots = []
+    for w in whole.tolist():
+        parts = sorted(rows[w[0], w[5]], key=lambda u: u[10])
+        assert [u[10] for u in parts] == list(range(len(parts))) and all(u[9] == len(parts) for u in parts)
+        at = 0
+        for u in parts:
+            assert u[:2] + [u[5], u[8]] == w[:2] + [w[5], w[8]]
+            assert (u[2], u[3], u[4]) == (w[2] + 128 * at, w[3] - 128 * at, w[4] - 128 * at)
+            assert [min(max(n - at, 0), max(u[6:8])) for n in w[6:8]] == u[6:8]
+            at += max(u[6:8])
+            if len(parts) > 1:
+                assert u[11] == parts[0][11] and max(u[6:8]) > 0
+                slots += [u[11] + 2 * u[10], u[11] + 2 * u[10] + 1]
+        assert at == max(w[6:8])
+    assert sorted(slots) == list(range(len(slots)))
+    assert plan["workspace_bytes"] == len(slots) * 128 * (128 + 2) * 4
+    if (ql, kl) == ([16], [32768]) and max_ctas == 0:
+        assert plan["ctas"] > 100
 
 
 def test_prompt_plan_refusals():

@@ -369,6 +369,73 @@ def test_prompt(bsp, ql, kl, hq, hk, d, causal):
     bsp.device().synchronize()
 
 
+CUT = [
+    ([16], [5000], 8, 2, 128, True),
+    ([1], [20011], 4, 4, 64, True),
+    ([3, 1, 130], [700, 9001, 130], 6, 2, 64, True),
+    ([2100], [1500], 2, 1, 128, True),          # the first 600 queries see no key
+    ([1500], [1500], 5, 1, 128, True),          # rows that see keys of the first parts only
+    ([40, 200], [4097, 3000], 3, 1, 128, False),
+    ([1500], [1500], 4, 1, 64, False),
+]
+
+
+@pytest.mark.parametrize("ql,kl,hq,hk,d,causal", CUT, ids=[f"q{sum(c[0])}_kv{sum(c[1])}_d{c[4]}_{c[5]}" for c in CUT])
+def test_prompt_cut_keys(bsp, ql, kl, hq, hk, d, causal):
+    """Few rows of many keys: the keys are cut into parts that a second kernel
+    joins.  The same values as the whole up to rounding, the same bits again."""
+    torch = torch_()
+    rng = np.random.default_rng(sum(kl))
+    q = ref.bf16(rng.normal(0, 1, (sum(ql), hq, d)))
+    k, v = (ref.bf16(rng.normal(0, 1, (sum(kl), hk, d))) for _ in range(2))
+    k *= np.float32(1 + 3 * (np.arange(len(k)) % 997 > 900))[:, None, None]  # parts of different weight
+    k = ref.bf16(k)
+    plan = bsp.PromptPlan(bsp.device(), ql, kl, hq, hk, d, causal=causal)
+    assert plan.info()["workspace_bytes"] > 0
+    qt, kt, vt = (cuda(x, torch.bfloat16) for x in (q, k, v))
+    gold = prompt_gold(q.astype(float), k.astype(float), v.astype(float), ql, kl, hk, 1 / np.sqrt(d), causal)
+    o, lse = torch.full_like(qt, float("nan")), torch.full((sum(ql), hq), float("nan"), device="cuda")
+    plan.execute(qt, kt, vt, o, lse=lse)
+    bsp.device().synchronize()
+    check_attention(o, lse, *gold, ref.U16)
+    o2, lse2 = spread(torch.zeros_like(o), rng), torch.zeros_like(lse)
+    for _ in range(3):
+        plan.execute(spread(qt, rng), spread(kt, rng), spread(vt, rng), o2, lse=lse2)
+        assert torch.equal(o2, o) and torch.equal(lse2, lse)
+    plan.execute(qt, kt, vt, o2)  # no lse
+    assert torch.equal(o2, o)
+    # few CTAs, so other parts; and whole
+    for kw in (dict(max_ctas=20), dict(group_rows=-1)):
+        other = bsp.PromptPlan(bsp.device(), ql, kl, hq, hk, d, causal=causal, opts=bsp.make_opts(**kw))
+        other.execute(qt, kt, vt, o2, lse=lse2)
+        bsp.device().synchronize()
+        check_attention(o2, lse2, *gold, ref.U16)
+    assert other.info()["workspace_bytes"] == 0
+
+
+@pytest.mark.parametrize("at", [0, 127, 128, 1000, 2999])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+def test_prompt_cut_bad_key(bsp, at, bad):
+    """A bad key in one part makes the joined rows that see it NaN, and no other."""
+    torch = torch_()
+    n, m, d = 600, 3000, 128
+    rng = np.random.default_rng(5)
+    q = ref.bf16(np.abs(rng.normal(0, 1, (n, 1, d))) + 0.1)
+    k, v = (ref.bf16(rng.normal(0, 1, (m, 1, d))) for _ in range(2))
+    plan = bsp.PromptPlan(bsp.device(), [n], [m], 1, 1, d)
+    assert plan.info()["workspace_bytes"] > 0
+    gold = prompt_gold(q.astype(float), k.astype(float), v.astype(float), [n], [m], 1, 1 / np.sqrt(d), True)
+    qt, kt, vt = (cuda(x, torch.bfloat16) for x in (q, k, v))
+    kt[at, 0, 5] = bad
+    o, lse = torch.empty_like(qt), torch.empty((n, 1), device="cuda")
+    plan.execute(qt, kt, vt, o, lse=lse)
+    bsp.device().synchronize()
+    first = max(0, at - (m - n))  # the first query that sees the key
+    if first:
+        check_attention(o[:first], lse[:first], *(x[:first] for x in gold), ref.U16)
+    assert torch.isnan(o[first:]).all() and torch.isnan(lse[first:]).all()
+
+
 @pytest.mark.parametrize("scale", [1e-3, 30.0])
 def test_prompt_scales_and_rising_scores(bsp, scale):
     """Flat and one-hot softmax, and scores that rise along the keys so that
