@@ -2529,10 +2529,10 @@ bsp_status plan_prompt_host(bsp_prompt_plan* p, const int32_t* q_lens, const int
   int64_t best = deal(items, true);
   // Few rows of many keys would leave CTAs idle: cut the blocks' keys into parts
   // of at most `len` steps where that ends sooner.  A part writes its rows to the
-  // workspace, which takes most of a step, and a second kernel joins them: a step
-  // and a half for its launch, and its traffic.  16 tokens behind 32768 keys (32
-  // heads, 8 of keys) take 39 us so, whole 395 us; 1000 tokens of 4 heads 12 us,
-  // whole 18 us.
+  // workspace, a third of a step, and a second kernel joins them: a step for its
+  // launch, its traffic, and a round trip to L2 for four parts.  16 tokens behind
+  // 32768 keys (32 heads, 8 of keys) take 39 us so, whole 395 us; 1000 tokens of 4
+  // heads 12 us, whole 18 us.
   int64_t best_len = 0;
   if (!(opts && opts->group_rows < 0) && ctas > 0 && best > total / ctas + 64) {
     const double even = static_cast<double>(steps) / ctas;
@@ -2548,11 +2548,11 @@ bsp_status plan_prompt_host(bsp_prompt_plan* p, const int32_t* q_lens, const int
         for (int32_t k = 0; k < parts; ++k) {
           int32_t n[2];
           part_of(u, parts, k, n);
-          items.push_back({cost(n[0], n[1]) + (parts > 1 ? 24 : 0), 0});
+          items.push_back({cost(n[0], n[1]) + (parts > 1 ? 12 : 0), 0});
         }
       }
       if (slots == 0 || slots > 8 * static_cast<int64_t>(ctas)) continue;
-      const int64_t end = deal(items, false) + 48 + slots / 3 + 2 * most;
+      const int64_t end = deal(items, false) + 32 + slots / 4 + 2 * most;
       if (end < best) {
         best = end;
         best_len = len;
@@ -2573,7 +2573,7 @@ bsp_status plan_prompt_host(bsp_prompt_plan* p, const int32_t* q_lens, const int
         x.parts = parts;
         x.part = k;
         x.first = static_cast<int32_t>(p->slots);
-        items.push_back({cost(x.n[0], x.n[1]) + (parts > 1 ? 24 : 0), static_cast<int32_t>(cut.size())});
+        items.push_back({cost(x.n[0], x.n[1]) + (parts > 1 ? 12 : 0), static_cast<int32_t>(cut.size())});
         cut.push_back(x);
         if (parts > 1 && k == 0) p->h_joins.push_back(x);
       }
