@@ -14,7 +14,12 @@
 // always in flight: asynchronous copies bring its 16-bit values to shared
 // memory (each lane its own, two buffers), while (cos, sin) of the warp's 16
 // tokens stay in registers for all its jobs.  Keys are rotated twice, for their
-// maximum and for their codes: cheaper than keeping them in 32 bits.
+// maximum and for their codes: cheaper than keeping them in 32 bits (fp32 between
+// the passes spilled: 140 us against 91 then).
+//
+// 14278 tokens, 32 + 2 x 8 heads of 128, pages of 16: 66 us, 5400 GB/s, 83 % of a
+// plain copy's rate (56 % of the issue slots, 23 % of the warps: registers allow
+// two blocks an SM).  A token each of 64 sequences: 4.9 us, latency.
 #include <cuda_fp8.h>
 
 #include "bsp_ptx.cuh"
@@ -351,6 +356,9 @@ bsp_status launch_append(AppendParams& p, bsp_device* dev, cudaStream_t stream) 
   const int page = p.cache.page;
   p.page_shift = __builtin_ctz(static_cast<unsigned>(page));
   const int64_t per_seq = p.tokens / p.n_seqs;
+  // A warp to 16 tokens of a page, at the calls' average (pages of 64: 14278
+  // tokens of six sequences 69 us, with single warps 166; a token each of 64
+  // sequences 4.9 us with single warps, 7.9 with four).
   p.team_warps = 1;
   while (p.team_warps * 2 * kApTokens <= std::min<int64_t>(per_seq, page)) p.team_warps *= 2;
   const int64_t by_page = p.tokens / page + 2 * static_cast<int64_t>(p.n_seqs);

@@ -49,7 +49,7 @@ struct AppendParams {
 };
 
 struct DecodeParams {
-  CUtensorMap tm_k, tm_v;     // codes: [page][head][token][d], boxes of up to 64 tokens of one page and head
+  CUtensorMap tm_k, tm_v;     // codes: [page][head][token][d], boxes of up to 128 tokens of one page and head
   HeadsView q;
   HeadsOut o;
   float* lse;

@@ -2455,6 +2455,8 @@ bsp_status plan_prompt_host(bsp_prompt_plan* p, const int32_t* q_lens, const int
     pairs += (static_cast<int64_t>(q_lens[s]) + 2 * p->tile_tokens - 1) / (2 * p->tile_tokens) * bands;
   }
   int ctas = opts && opts->max_ctas > 0 ? std::min(opts->max_ctas, sm_count) : sm_count;
+  // Single tiles where CTAs are left over: 37 tokens of 8 heads of 64 take 4.85 us,
+  // in pairs 5.6; 300 of 8 heads of 128 9.2 and 10.6.
   const int32_t tiles = 2 * pairs <= ctas ? 1 : 2;
   if (pairs > (int64_t(1) << 28)) return set_error(BSP_ERR_UNSUPPORTED, "too many work units");
   std::vector<PromptUnit> units;

@@ -30,19 +30,30 @@
 // Warps (320 threads, one CTA per SM): 0-3 softmax of tile a, 4-7 of tile b
 // (TMEM lane quarter = warp & 3), 8 MMA, 9 TMA.  Every wait is bounded.
 //
-// The chain S -> P -> O -> S of a tile bounds the kernel: at 16384 tokens, 8
-// heads of 128, one step takes 3300 cycles of which a tile's softmax is 2050,
-// its products with their hand-overs 1150 (the tensor cores are busy 63 %, the
-// exponential unit 47 %).  What shortens it: the softmax does not wait for its
-// own maximum (weights are formed with the maximum of the steps before, the
-// step's own is found beside them and only moves m for the next step, or at
-// once if it is 2^20 above); a quarter of the exponentials is computed in the
-// FMA pipe (exp2_pair); scaling and sums are packed two to an instruction; P is
-// handed over in two parts of 64 keys, so that O += P V begins while the second
-// part is worked on.  442 us for 0.55 TFLOP (1242 TFLOP/s).  Steps of 64 keys
-// with two S buffers (no product in the chain) measured 545 us: an N = 64
-// product takes as long as N = 128.  Two threads a row (16 softmax warps)
-// measured 471 us against 447 us then.
+// What bounds it: the tensor cores with their hand-overs, and power.  At 16384
+// tokens, 8 heads of 128, one step of both tiles takes 3000 cycles, of which the
+// products need 2048 (64 for each MMA of 128 x 128 x 16); without any softmax
+// work the same waits and products take 83 % of the time, without its arithmetic
+// 87 %.  The MMAs are 62 % of the cycles, the exponential unit 47 %.  The SMs run
+// at 1.62 GHz in a burst and at 1.35 GHz once the power limit holds: 442 us (1240
+// TFLOP/s) and 512 us for 0.55 TFLOP.  Heads of 64 do half the products on the
+// same softmax and hand-overs: 16 heads, 6025 tokens 57 us (500 TFLOP/s).
+//
+// What shortens a step: the softmax does not wait for its own maximum (weights
+// are formed with the maximum of the steps before, the step's own is found
+// beside them and only moves m for the next step, or at once if it is 2^20
+// above); a quarter of the exponentials is computed in the FMA pipe (exp2_pair);
+// scaling and sums are packed two to an instruction; P is handed over in two
+// parts of 64 keys, so that O += P V begins while the second part is worked on.
+// What did not: steps of 64 keys with two S buffers (545 us against 442), two
+// threads a row (471), an MMA warp for each tile (566), P of d = 64 in columns of
+// its own so that S comes a step ahead (416 against 392), the next unit's first
+// scores behind the unit's last products (457).
+//
+// Few rows of many keys: the planner cuts a block's keys into parts.  A part
+// leaves O unnormalised in fp32 with m and l; prompt_join puts them together.
+// (Joined by the part that ends last, inside this kernel, 16 tokens behind 32768
+// keys took 61 us; with a kernel of its own 39 us.)
 #include <cuda_bf16.h>
 
 #include "bsp_ptx.cuh"
@@ -596,7 +607,8 @@ __global__ void __launch_bounds__(kPrThreads, 1) prompt_tcgen05(const __grid_con
 
 // The parts of the blocks that are cut, joined in their order:
 //   m = max m_k,  l = sum 2^(m_k - m) l_k,  O = sum 2^(m_k - m) O_k / l.
-// A thread takes 16 columns of a row of tile blockIdx.x & 1.
+// A thread takes 16 columns of a row of tile blockIdx.x & 1.  Bound by the round
+// trips to L2, one for kPrDeep parts: about 3 us behind the kernel before it.
 constexpr int kPrDeep = 4;  // parts whose loads are in flight
 template <int kD>
 __global__ void __launch_bounds__(256) prompt_join(const __grid_constant__ PromptParams p) {
