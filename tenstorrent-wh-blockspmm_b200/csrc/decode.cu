@@ -606,17 +606,26 @@ __global__ void __launch_bounds__(kDcThreads, dc_per_sm(kD, 8 * kNt)) decode_ker
     // tiles of all rows, then the sequence in which this CTA's stretch begins
     const int first = lane < p.n_seqs ? dc_tiles(p, lane) : 0;
     int64_t total = first;
-    for (int s = lane + 32; s < p.n_seqs; s += 32) total += dc_tiles(p, s);
+    int longest = first;  // tiles of the longest row
+    for (int s = lane + 32; s < p.n_seqs; s += 32) {
+      const int n = dc_tiles(p, s);
+      total += n;
+      longest = max(longest, n);
+    }
     for (int k = 16; k; k >>= 1) total += __shfl_xor_sync(0xffffffffu, total, k);
+    longest = __reduce_max_sync(0xffffffffu, longest);
     total *= p.streams;
     if (total > 0x7FFFFFFF) {
       if (lane == 0) atomicOr(p.status, ST_BAD_INDEX);
       total = 0;
     }
-    // at least a tile to a CTA and at most 64 parts to a row on average: past
-    // that the joining costs more than the reading
-    const int64_t rows = static_cast<int64_t>(p.n_seqs) * p.streams;
-    const int ctas = static_cast<int>(min(static_cast<int64_t>(gridDim.x), min(total, 64 * rows)));
+    // A tile takes a CTA 1 us, and each part of a row 0.1 us more where they are
+    // joined: a row of n tiles in parts of t takes t + 0.1 n / t, least at t =
+    // sqrt(0.1 n).  Fewer tiles to a CTA only lengthen the joining (131072 tokens,
+    // one key/value head: 16 tiles a CTA 30 us, 8 32 us, 4 51 us; 8000 tokens: 4
+    // tiles 11.5 us, one 14.5 us).
+    const uint32_t least = max(__float2uint_rn(sqrtf(0.09f * static_cast<float>(longest))), 1u);
+    const int ctas = static_cast<int>(min(gridDim.x, (static_cast<uint32_t>(total) + least - 1) / least));
     const uint32_t each = ctas > 0 ? static_cast<uint32_t>(total) / static_cast<uint32_t>(ctas) : 0u;
     const uint32_t extra = static_cast<uint32_t>(total) - each * static_cast<uint32_t>(ctas);
     const int g0 = static_cast<int>(blockIdx.x * each + min(blockIdx.x, extra));
