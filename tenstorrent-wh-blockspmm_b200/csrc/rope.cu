@@ -36,7 +36,7 @@ __global__ void rope_table_kernel(float2* table, int64_t n_pos, int half, double
 
 // A thread turns unit u of kHeads heads of one token: (cos, sin) are loaded
 // once for them, and 2 kHeads loads are in flight.  Memory-bound: 8191 tokens of
-// 32 heads of 128 in f32 take 41.5 us, 6520 GB/s, a plain copy's rate.  16 tokens
+// 32 heads of 128 in f32 take 41.7 us, 6490 GB/s, a plain copy's rate.  16 tokens
 // take 1.8 us on the device, their launch more than that.
 template <typename T, int kHeads>
 __global__ void __launch_bounds__(256) rope_kernel(const RopeParams p) {
@@ -98,10 +98,11 @@ bsp_status launch_rope_table(bsp_device* dev, int64_t n_pos, int32_t rot, double
 bsp_status launch_rope(RopeParams& p, bsp_dtype type, int sm_count, cudaStream_t stream) {
   // One head a thread for up to about 512 threads an SM, two above: 16 tokens of
   // 32 heads of 128 in bf16 take 1.8 and 2.2 us, 300 tokens 3.0 either way, 1000
-  // 4.5 and 4.2, 3000 10.1 and 8.7 (four heads: 3.1, 3.5, 3.8 and 9.1).
+  // 4.5 and 4.2, 3000 10.1 and 8.7 (four heads: 3.1, 3.5, 3.8 and 9.1).  In f32
+  // four: 2000 tokens 6.9 us (two 7.1), 8191 half rotated 41.7 (two 42.4).
   const bool few = p.tokens * p.heads * (p.d / 16) < static_cast<int64_t>(sm_count) * 512;
   if (type == BSP_BF16) return few ? run_rope<uint16_t, 1>(p, stream) : run_rope<uint16_t, 2>(p, stream);
-  return few ? run_rope<float, 1>(p, stream) : run_rope<float, 2>(p, stream);
+  return few ? run_rope<float, 1>(p, stream) : run_rope<float, 4>(p, stream);
 }
 
 }  // namespace bsp
