@@ -430,7 +430,7 @@ bsp_status bsp_decode_execute(const bsp_decode_plan* plan, const bsp_kv_cache* c
   p.lens = lens;
   p.page_table = page_table;
   p.table_stride = table_stride;
-  p.table_width = table_width;
+  p.max_len = static_cast<int32_t>(std::min<int64_t>(table_width * plan->page, 0x7FFFFF00));
   p.n_seqs = n_seqs;
   p.heads = plan->heads;
   p.group = plan->heads / plan->kv_heads;

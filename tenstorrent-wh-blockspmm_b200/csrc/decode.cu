@@ -150,7 +150,7 @@ __device__ __forceinline__ void tma_load_4d_pred(uint32_t smem_dst, const void* 
 // table holds.
 __device__ __forceinline__ int dc_len(const DecodeParams& p, int s) {
   const int len = __ldg(p.lens + s);
-  return len < 0 || len > p.table_width * p.cache.page ? 0 : len;
+  return len < 0 || len > p.max_len ? 0 : len;
 }
 __device__ __forceinline__ int dc_tiles(const DecodeParams& p, int s) { return (dc_len(p, s) + kDcTile - 1) / kDcTile; }
 

@@ -56,7 +56,8 @@ struct DecodeParams {
   bsp_kv_cache cache;
   const int32_t* lens;
   const int32_t* page_table;
-  int64_t table_stride, table_width;
+  int64_t table_stride;
+  int32_t max_len;            // tokens that a row of the page table holds, a tile below 2^31
   int32_t n_seqs, heads;
   int32_t group;              // query heads of one key/value head
   int32_t chunks;             // rows of up to 16 query heads per key/value head

@@ -762,6 +762,28 @@ def test_graph_capture(bsp):
     bsp.device().synchronize()
 
 
+def test_graph_capture_of_cut_prompt(bsp):
+    """A plan that is cut, captured with its joining kernel and replayed on other inputs."""
+    torch = torch_()
+    q, k, v = (torch.zeros((n, h, 64), device="cuda", dtype=torch.bfloat16) for n, h in ((9, 4), (4000, 2), (4000, 2)))
+    plan = bsp.PromptPlan(bsp.device(), [9], [4000], 4, 2, 64)
+    assert plan.info()["workspace_bytes"] > 0
+    o = [torch.zeros_like(q) for _ in range(2)]
+    plan.execute(q, k, v, o[0])
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        plan.execute(q, k, v, o[0])
+    for _ in range(3):
+        for t in (q, k, v):
+            t.normal_()
+        graph.replay()
+        plan.execute(q, k, v, o[1])
+        torch.cuda.synchronize()
+        assert torch.equal(o[0], o[1]) and bool(o[0].any())
+    bsp.device().synchronize()
+
+
 # ---------------------------------------------------------------- refusals --
 def test_refusals(bsp):
     torch = torch_()
