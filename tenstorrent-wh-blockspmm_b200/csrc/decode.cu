@@ -72,10 +72,12 @@ static_assert(sizeof(DcHeader) <= 1024, "header must fit its 1 KiB slot");
 
 // Shared memory from the 1 KiB-aligned base: header, slots (K and V of a tile
 // in turn), then the warps' results: O [4][heads][d], m [4][heads], l [4][heads].
-// CTAs on an SM: one with rows of 16 heads (registers), two for d = 128, four
-// for d = 64, whose tiles are half the bytes for the same work on scores (16
-// heads of 64 in pages of 16: 39 us with two, 32 with three, 29.5 with four).
-__host__ __device__ constexpr int dc_per_sm(int d, int heads) { return heads > 8 ? 1 : d == 64 ? 4 : 2; }
+// CTAs on an SM: two; four for rows of up to 8 heads of 64, whose tiles are half
+// the bytes for the same work on scores (16 heads of 64 in pages of 16: 39 us
+// with two, 32 with three, 29.5 with four).  Rows of 16 heads with one CTA, which
+// leaves them more registers: 64 contexts of 4000 tokens, 4 key/value heads of
+// 128 73 us, with two 60; heads of 64 55 and 40.
+__host__ __device__ constexpr int dc_per_sm(int d, int heads) { return heads <= 8 && d == 64 ? 4 : 2; }
 // As many slots as fit the SM's 228 KB then (1 KB of each CTA is the system's).
 __host__ __device__ constexpr int dc_slot_bytes(int d) { return kDcTile * d; }
 __host__ __device__ constexpr int dc_result_bytes(int d, int heads) { return 16 * heads * (d + 2); }
