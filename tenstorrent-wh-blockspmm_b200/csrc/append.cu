@@ -7,10 +7,10 @@
 // page's earlier codes again.
 //
 // A job is one head of the keys, the values or the queries of a chunk (the new
-// tokens of one sequence on one page); a team does several of a chunk's jobs.  A
-// team has one warp per 16 tokens of the page when sequences bring pages of
-// tokens, and a single warp when they bring one token each: a warp with nothing
-// to do still costs its start.  Memory-bound, so the loads of the next job are
+// tokens of one sequence on one page); a team does several of a chunk's jobs.  It
+// has one warp per 16 tokens of its chunk, so a long prompt and many single tokens
+// go together (90 tokens with one each of 63 other sequences: 14.1 us, 37 us with
+// one warp a team).  Memory-bound, so the loads of the next job are
 // always in flight: asynchronous copies bring its 16-bit values to shared
 // memory (each lane its own, two buffers), while (cos, sin) of the warp's 16
 // tokens stay in registers for all its jobs.  Keys are rotated twice, for their
@@ -31,11 +31,15 @@ using namespace dev;
 namespace {
 
 constexpr int kApWarps = 8;
-constexpr int kApTokens = 16;  // of one head that a warp takes at once
+// Tokens of one head that a warp takes at once: side by side (a head of 128 is 8
+// lanes, of 64 4) and one after the other, 16 in all where sequences bring many.
+constexpr int kApTokens = 16;
+constexpr int ap_across(int d) { return 512 / d; }
 
 // New tokens [t0, t0 + n) of one sequence, at slots [slot, slot + n) of page.
 struct Chunk {
   int32_t page, slot, n;
+  int32_t warps;  // of a team, a power of two
   int64_t t0, pos0;
 };
 
@@ -145,11 +149,11 @@ __device__ __forceinline__ Target settle(const AppendParams& p, const Chunk& ck,
   float* sp = (is_v ? p.cache.v_scale : p.cache.k_scale) + static_cast<int64_t>(ck.page) * p.cache.kv_heads + h;
   const uint32_t old_bits = ck.slot > 0 ? __float_as_uint(*sp) : 0;
   for (int k = 16; k; k >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, k));
-  if (p.team_warps > 1) {
-    team_sync(team, p.team_warps);  // the last job's maxima have been read
-    if (lane == 0) s_max[team * p.team_warps + in_team] = m;
-    team_sync(team, p.team_warps);
-    for (int k = 0; k < p.team_warps; ++k) m = fmaxf(m, s_max[team * p.team_warps + k]);
+  if (ck.warps > 1) {
+    team_sync(team, ck.warps);  // the last job's maxima have been read
+    if (lane == 0) s_max[team * ck.warps + in_team] = m;
+    team_sync(team, ck.warps);
+    for (int k = 0; k < ck.warps; ++k) m = fmaxf(m, s_max[team * ck.warps + k]);
   } else {
     __syncwarp();
   }
@@ -161,7 +165,7 @@ __device__ __forceinline__ Target settle(const AppendParams& p, const Chunk& ck,
     } else {
       const float f = two_to(max(was - e, -126));
       uint32_t* w = reinterpret_cast<uint32_t*>(codes);
-      for (int i = 32 * in_team + lane; i < ck.slot * (kD / 4); i += 32 * p.team_warps) {
+      for (int i = 32 * in_team + lane; i < ck.slot * (kD / 4); i += 32 * ck.warps) {
         const uint32_t c = w[i];
         const float v[4] = {code_value(c & 0xFF), code_value((c >> 8) & 0xFF), code_value((c >> 16) & 0xFF),
                             code_value(c >> 24)};
@@ -219,7 +223,7 @@ __device__ __noinline__ void append_long(const AppendParams& p, const Chunk& ck,
   float m = 0.f;
   Target to{nullptr, 1.f};
   for (int pass = j.is_q ? 1 : 0; pass < 2; ++pass) {
-    for (int t = in_team * kAcross + lane / kUnits; t < ck.n; t += kAcross * p.team_warps) {
+    for (int t = in_team * kAcross + lane / kUnits; t < ck.n; t += kAcross * ck.warps) {
       float lo[8], hi[8];
       load_vec(j.x + t * j.x_token + un.lo, lo);
       load_vec(j.x + t * j.x_token + un.hi, hi);
@@ -242,30 +246,34 @@ __device__ __noinline__ void append_long(const AppendParams& p, const Chunk& ck,
   }
 }
 
-// kUnits: units of two vectors of 8 values in a head (d / 16).
-template <int kUnits, bool kInterleaved>
-__global__ void __launch_bounds__(32 * kApWarps, 2) append_kernel(const __grid_constant__ AppendParams p) {
+// kUnits: units of two vectors of 8 values in a head (d / 16); kDeep: tokens one
+// after the other.  With one, a block needs half the registers, and twice as many
+// are on an SM.
+template <int kUnits, bool kInterleaved, int kDeep>
+__global__ void __launch_bounds__(32 * kApWarps, kDeep == 1 ? 4 : 2) append_kernel(const __grid_constant__ AppendParams p) {
   constexpr int kAcross = 32 / kUnits;        // tokens side by side in a warp
-  constexpr int kDeep = kApTokens / kAcross;  // and one after the other
+  constexpr int kTokens = kAcross * kDeep;
   constexpr int kD = 16 * kUnits;
   __shared__ float s_max[kApWarps];
   extern __shared__ uint4 s_raw[];            // per warp 2 x [kDeep][2][32]
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int team = warp / p.team_warps, in_team = warp % p.team_warps;
-  const int teams = kApWarps / p.team_warps;
   const int jobs = 2 * p.cache.kv_heads + (p.q.p ? p.heads : 0);
-  const int first = blockIdx.y * teams + team, step = gridDim.y * teams;
   stream_release();
   stream_wait();
   Chunk ck;
   if (!find_chunk(p, blockIdx.x, lane, ck)) return;
-  if (ck.n > kApTokens * p.team_warps) {
+  // log2 of the team's warps: kTokens << shift holds the chunk, or it is the block
+  const int shift = min(32 - __clz((ck.n - 1) / kTokens), 31 - __clz(kApWarps));
+  ck.warps = 1 << shift;
+  const int team = warp >> shift, in_team = warp & (ck.warps - 1), teams = kApWarps >> shift;
+  const int first = blockIdx.y * teams + team, step = gridDim.y * teams;
+  if (ck.n > kTokens * ck.warps) {
     const bool bad = bad_page(p, ck, lane);
     for (int job = first; job < jobs && !bad; job += step)
       append_long<kUnits, kInterleaved>(p, ck, job, team, in_team, lane, s_max);
     return;
   }
-  const int u = lane % kUnits, t0 = in_team * kApTokens + lane / kUnits;  // this lane's tokens: t0 + kAcross k
+  const int u = lane % kUnits, t0 = in_team * kTokens + lane / kUnits;  // this lane's tokens: t0 + kAcross k
   const RopeUnit<8> turned(u, p.table ? p.rot : 0, kD), plain(u, 0, kD);
   uint4* raw = s_raw + warp * (2 * kDeep * 2 * 32) + lane;
   auto fetch = [&](int job, int buf) {
@@ -334,11 +342,15 @@ __global__ void __launch_bounds__(32 * kApWarps, 2) append_kernel(const __grid_c
 }
 
 using AppendKernel = void (*)(AppendParams);
-AppendKernel pick(int d, bool interleaved) {
-  return d == 64 ? (interleaved ? append_kernel<4, true> : append_kernel<4, false>)
-                 : (interleaved ? append_kernel<8, true> : append_kernel<8, false>);
+template <int kUnits, bool kInterleaved>
+AppendKernel pick(bool few) {
+  return few ? append_kernel<kUnits, kInterleaved, 1> : append_kernel<kUnits, kInterleaved, kApTokens * kUnits / 32>;
 }
-constexpr int raw_bytes(int d) { return kApWarps * 2 * kApTokens * d * 2; }
+AppendKernel pick(int d, bool interleaved, bool few) {
+  return d == 64 ? (interleaved ? pick<4, true>(few) : pick<4, false>(few))
+                 : (interleaved ? pick<8, true>(few) : pick<8, false>(few));
+}
+constexpr int raw_bytes(int d, bool few) { return kApWarps * 2 * (few ? ap_across(d) : kApTokens) * d * 2; }
 
 }  // namespace
 
@@ -346,9 +358,9 @@ bsp_status launch_append(AppendParams& p, bsp_device* dev, cudaStream_t stream) 
   if (!dev->append_ready) {
     for (int d : {64, 128})
       for (bool i : {false, true}) {
-        const bsp_status s =
-            cuda_check(cudaFuncSetAttribute(pick(d, i), cudaFuncAttributeMaxDynamicSharedMemorySize, raw_bytes(d)),
-                       "cudaFuncSetAttribute(append)");
+        const bsp_status s = cuda_check(
+            cudaFuncSetAttribute(pick(d, i, false), cudaFuncAttributeMaxDynamicSharedMemorySize, raw_bytes(d, false)),
+            "cudaFuncSetAttribute(append)");
         if (s != BSP_OK) return s;
       }
     dev->append_ready = true;
@@ -356,25 +368,26 @@ bsp_status launch_append(AppendParams& p, bsp_device* dev, cudaStream_t stream) 
   const int page = p.cache.page;
   p.page_shift = __builtin_ctz(static_cast<unsigned>(page));
   const int64_t per_seq = p.tokens / p.n_seqs;
-  // A warp to 16 tokens of a page, at the calls' average (pages of 64: 14278
-  // tokens of six sequences 69 us, with single warps 166; a token each of 64
-  // sequences 4.9 us with single warps, 7.9 with four).
-  p.team_warps = 1;
-  while (p.team_warps * 2 * kApTokens <= std::min<int64_t>(per_seq, page)) p.team_warps *= 2;
+  // A step of decoding (no more tokens than sequences) whose chunks do not fit the
+  // GPU's blocks at once: a warp takes fewer tokens, so that twice as many blocks do
+  // (a token each of 512 sequences 14.1 us, 17.6 us with 16 tokens a warp; of 64
+  // sequences 5.0 us either way).
+  const bool few = p.tokens <= p.n_seqs && p.n_seqs > 2 * dev->sm_count;
   const int64_t by_page = p.tokens / page + 2 * static_cast<int64_t>(p.n_seqs);
   p.by_token = p.tokens < by_page;
   const int64_t chunks = std::min(p.tokens, by_page);
   if (chunks > 0x7FFFFFFF) return set_error(BSP_ERR_UNSUPPORTED, "too many sequences");
   const int jobs = 2 * p.cache.kv_heads + (p.q.p ? p.heads : 0);
-  const int teams = kApWarps / p.team_warps;
+  int64_t teams = kApWarps;  // that a block has for a chunk of average length
+  while (teams > 1 && kApTokens * kApWarps <= teams * std::min<int64_t>(per_seq, page) / 2) teams /= 2;
   // A job to a team while that does not need more blocks than the GPU holds at
   // once (two an SM), else several: 14278 tokens in pages of 16 take 68 us with
   // one block to a chunk (of 904), 74 us with three and 96 us with six; a token
   // each of 64 sequences 4.9 us with four blocks to a chunk, 5.1 us with six.
   const int64_t most = (jobs + teams - 1) / teams;
-  const int64_t enough = std::max<int64_t>(2 * static_cast<int64_t>(dev->sm_count) / (p.tokens / page + p.n_seqs), 1);
+  const int64_t enough = std::max<int64_t>((few ? 4 : 2) * static_cast<int64_t>(dev->sm_count) / (p.tokens / page + p.n_seqs), 1);
   const dim3 grid(static_cast<unsigned>(chunks), static_cast<unsigned>(std::min(most, enough)));
-  return launch_overlapped(pick(p.cache.d, p.interleaved), grid, 32 * kApWarps, raw_bytes(p.cache.d), stream, p,
+  return launch_overlapped(pick(p.cache.d, p.interleaved, few), grid, 32 * kApWarps, raw_bytes(p.cache.d, few), stream, p,
                            "cache append launch");
 }
 

@@ -43,7 +43,7 @@ struct AppendParams {
   int64_t n_pos;
   int64_t tokens;
   int32_t n_seqs, heads, rot, interleaved;
-  int32_t team_warps, page_shift;
+  int32_t page_shift;
   int32_t by_token;           // blocks are counted by tokens, not by pages
   unsigned int* status;
 };

@@ -181,6 +181,10 @@ APPEND = [
     ([1] * 40, list(range(40)), 8, 32, 64, 128, 128),
     ([1] * 30 + [150], [5] * 30 + [37], 2, 6, 64, 128, 64),   # a prompt among single tokens
     ([1] * 20 + [200, 17], [100] * 20 + [90, 0], 1, 3, 128, 64, 64),
+    # more sequences than blocks fit at once, no more tokens than sequences
+    ([1] * 310, [7 * i % 70 for i in range(310)], 1, 2, 16, 128, 128),
+    ([0] * 220 + [70, 0, 40, 3] + [1] * 170, [3] * 394, 2, 3, 128, 128, 64),
+    ([0] * 200 + [100] + [1] * 190, [30] * 391, 1, 1, 128, 64, 64),
 ]
 
 
