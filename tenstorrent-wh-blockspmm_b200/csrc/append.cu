@@ -50,7 +50,7 @@ struct Chunk {
 // blocks, half of them without a chunk).  So the sequence is found by a search in
 // steps of 32 and no host copy of the lengths is needed.
 __device__ __forceinline__ int64_t first_chunk(const AppendParams& p, int s) {
-  const int64_t start = __ldg(p.starts + s);
+  const int64_t start = p.starts[s];
   return p.by_token ? start : (start >> p.page_shift) + 2 * static_cast<int64_t>(s);
 }
 __device__ __forceinline__ bool find_chunk(const AppendParams& p, int64_t c, int lane, Chunk& out) {
@@ -63,7 +63,7 @@ __device__ __forceinline__ bool find_chunk(const AppendParams& p, int64_t c, int
     lo += k * step;
     n_left = min(step, n_left - k * step);
   }
-  const int64_t t0 = __ldg(p.starts + lo), n = __ldg(p.starts + lo + 1) - t0, b = __ldg(p.before + lo);
+  const int64_t t0 = p.starts[lo], n = p.starts[lo + 1] - t0, b = p.before[lo];
   if (t0 < 0 || n < 0 || t0 + n > p.tokens || b < 0) {
     if (lane == 0) atomicOr(p.status, ST_BAD_INDEX);
     return false;
@@ -77,7 +77,7 @@ __device__ __forceinline__ bool find_chunk(const AppendParams& p, int64_t c, int
   out.pos0 = b + (out.t0 - t0);
   const int64_t left = t0 + n - out.t0;
   out.n = static_cast<int32_t>(left < page - out.slot ? left : page - out.slot);
-  out.page = index < p.table_width ? __ldg(p.page_table + lo * p.table_stride + index) : -1;
+  out.page = index < p.table_width ? p.page_table[lo * p.table_stride + index] : -1;
   if (p.table && out.pos0 + out.n > p.n_pos) {
     if (lane == 0) atomicOr(p.status, ST_BAD_INDEX);
     return false;

@@ -109,7 +109,10 @@ __device__ __forceinline__ bool mbar_wait_bounded(uint32_t bar, uint32_t parity,
 
 // ---- overlap with the kernels before and after in the stream ----------------
 // Wait until the kernel before this one has finished and its writes are seen
-// (at once where the launch did not allow an early start).
+// (at once where the launch did not allow an early start).  Seen by ordinary
+// loads and TMA: ld.global.nc (__ldg) asks for memory that nobody writes while
+// this kernel is resident, and it is resident before this wait, so what a kernel
+// before may have written (lengths, pages, scales, tables) is not read with it.
 __device__ __forceinline__ void stream_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 // The kernel behind this one may start (it waits in its own stream_wait).
 __device__ __forceinline__ void stream_release() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }

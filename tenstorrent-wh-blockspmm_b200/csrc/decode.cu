@@ -151,7 +151,7 @@ __device__ __forceinline__ void tma_load_4d_pred(uint32_t smem_dst, const void* 
 // Tokens of sequence s that count: 0 where the length is not one that the page
 // table holds.
 __device__ __forceinline__ int dc_len(const DecodeParams& p, int s) {
-  const int len = __ldg(p.lens + s);
+  const int len = p.lens[s];
   return len < 0 || len > p.max_len ? 0 : len;
 }
 __device__ __forceinline__ int dc_tiles(const DecodeParams& p, int s) { return (dc_len(p, s) + kDcTile - 1) / kDcTile; }
@@ -211,7 +211,7 @@ __device__ __forceinline__ void dc_produce(const DecodeParams& p, DcHeader* hdr,
     // lane's box of the batch that starts at tile b: its page and scale
     auto page_of = [&](int b) -> int32_t {
       const int64_t token = static_cast<int64_t>(pc.tile0 + b + at) * kDcTile + sub * box;
-      return b + at < pc.n && token < len ? __ldg(pages + (token >> shift)) : -2;  // -2: no box
+      return b + at < pc.n && token < len ? pages[token >> shift] : -2;  // -2: no box
     };
     auto checked = [&](int32_t id) -> int32_t {
       if (id == -2 || (id >= 0 && id < p.cache.n_pages)) return id;
@@ -219,7 +219,7 @@ __device__ __forceinline__ void dc_produce(const DecodeParams& p, DcHeader* hdr,
       return -1;  // read as zeros
     };
     auto scale_of = [&](int32_t id) {
-      return id >= 0 ? __ldg(scale + static_cast<int64_t>(id) * p.cache.kv_heads + kvh) : 1.f;
+      return id >= 0 ? scale[static_cast<int64_t>(id) * p.cache.kv_heads + kvh] : 1.f;
     };
     int32_t id = checked(page_of(0)), id_next = page_of(per_batch);
     float sc = scale_of(id);
@@ -659,7 +659,7 @@ __global__ void __launch_bounds__(kDcThreads, dc_per_sm(kD, 8 * kNt)) decode_ker
   // sequences without a token: O = 0, lse = -inf
   for (int s = blockIdx.x; s < p.n_seqs; s += gridDim.x) {
     if (dc_len(p, s) > 0) continue;
-    if (threadIdx.x == 0 && __ldg(p.lens + s) != 0) atomicOr(p.status, ST_BAD_INDEX);
+    if (threadIdx.x == 0 && p.lens[s] != 0) atomicOr(p.status, ST_BAD_INDEX);
     for (int i = threadIdx.x; i < p.heads * (kD / 8); i += kDcThreads) {
       const int head = i / (kD / 8), col = i % (kD / 8);
       uint16_t* dst = static_cast<uint16_t*>(p.o.p) + s * p.o.token + head * p.o.head;

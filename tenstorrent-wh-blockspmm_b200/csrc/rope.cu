@@ -51,7 +51,7 @@ __global__ void __launch_bounds__(256) rope_kernel(const RopeParams p) {
   const RopeUnit<kN> un(u, p.rot, p.d);
   const T* x = static_cast<const T*>(p.x.p) + token * p.x.token + head0 * p.x.head;
   T* out = static_cast<T*>(p.y.p) + token * p.y.token + head0 * p.y.head;
-  const int32_t pos = __ldg(p.positions + token);
+  const int32_t pos = p.positions[token];
   float lo[kHeads][kN], hi[kHeads][kN];
 #pragma unroll
   for (int h = 0; h < kHeads; ++h)

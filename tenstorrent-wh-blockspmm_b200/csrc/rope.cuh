@@ -81,11 +81,11 @@ __device__ __forceinline__ void turn_unit(float (&lo)[kN], float (&hi)[kN], cons
     for (int i = 0; i < kN; ++i) turn(lo[i], hi[i], cs[i], sign);
   }
 }
-// A read-only load that stays where it is written: the compiler would keep the
-// values of two passes over the same positions in registers between them.
+// A load that stays where it is written: the compiler would keep the values of
+// two passes over the same positions in registers between them.
 __device__ __forceinline__ float4 load_once(const float2* p) {
   float4 v;
-  asm volatile("ld.global.nc.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "l"(p));
+  asm volatile("ld.global.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "l"(p));
   return v;
 }
 // (cos, sin) of unit u's pairs from a position's row of the table.
