@@ -826,6 +826,9 @@ class KvCache:
         for x, name in ((k_scale, "k_scale"), (v_scale, "v_scale")):
             if not x.is_cuda or x.dtype is not torch.float32 or x.shape != k.shape[:2] or not x.is_contiguous():
                 _refuse(f"cache {name} must be a contiguous f32 cuda tensor [pages, kv_heads]")
+        for x, name in ((v, "v"), (k_scale, "k_scale"), (v_scale, "v_scale")):
+            if x.device != k.device:
+                _refuse(f"cache {name} is on {x.device}, k on {k.device}")
         self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
         n, h, page, d = k.shape
         # strides of single-entry dimensions are never stepped over: give them a valid value
@@ -835,13 +838,14 @@ class KvCache:
                                 page, d)
         self.address = ctypes.addressof(self.desc)
         self.kv_heads, self.page, self.d = h, page, d
+        self.ordinal = k.device.index
 
     @staticmethod
-    def empty(n_pages, kv_heads, page, d, device_index=0):
-        """A cache of n_pages zeroed pages."""
+    def empty(n_pages, kv_heads, page, d, device_index=None):
+        """A cache of n_pages zeroed pages (on the current GPU, or device_index)."""
         import torch
 
-        dv = torch.device("cuda", device_index)
+        dv = torch.device("cuda", torch.cuda.current_device() if device_index is None else device_index)
         k, v = (torch.zeros((n_pages, kv_heads, page, d), dtype=torch.uint8, device=dv) for _ in range(2))
         ks, vs = (torch.ones((n_pages, kv_heads), dtype=torch.float32, device=dv) for _ in range(2))
         return KvCache(k, v, ks, vs)

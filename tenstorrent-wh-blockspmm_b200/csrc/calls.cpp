@@ -110,6 +110,23 @@ const at::Tensor& tensor(PyObject* x, const char* name, at::ScalarType type, int
   return t;
 }
 
+// A cache: its description (bsp.KvCache keeps it) and the GPU that its tensors are on.
+struct Cache {
+  const bsp_kv_cache* desc;
+  long ordinal;
+};
+Cache cache_of(PyObject* x) {
+  const Ref address(PyObject_GetAttr(x, s_address));
+  const auto* desc = static_cast<const bsp_kv_cache*>(PyLong_AsVoidPtr(address.p));
+  if (PyErr_Occurred()) throw PyFailed{};
+  if (!desc) refuse("null cache");
+  return {desc, number(x, s_ordinal)};
+}
+const bsp_kv_cache* cache_on(const Cache& c, int at) {
+  if (c.ordinal != at) refuse("the cache is on cuda:" + std::to_string(c.ordinal) + ", not on GPU " + std::to_string(at));
+  return c.desc;
+}
+
 // A [tokens, heads, d] operand, d contiguous.  A dimension of one entry is never
 // stepped over: its stride counts as 0.
 struct Heads {
@@ -243,13 +260,13 @@ PyObject* py_rope(PyObject*, PyObject* const* a, Py_ssize_t n) {
 // kv_append(cache, k, v, starts, before, pages, table, layout, q, q_out, k_out, dev, stream)
 PyObject* py_kv_append(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return guarded(n, 13, [&] {
-    const Ref address(PyObject_GetAttr(a[0], s_address));
-    const auto* cache = static_cast<const bsp_kv_cache*>(PyLong_AsVoidPtr(address.p));
-    if (!cache) throw PyFailed{};
+    const Cache held = cache_of(a[0]);
     const at::Tensor& kt = with_dims(a[1], "k", 3);
     const at::Tensor& bt = with_dims(a[4], "before", 1);
     const int64_t tokens = kt.size(0), seqs = bt.size(0);
-    const int at = kt.device().index(), hk = cache->kv_heads, d = cache->d;
+    const int at = kt.device().index();
+    const bsp_kv_cache* cache = cache_on(held, at);
+    const int hk = cache->kv_heads, d = cache->d;
     const Heads k = heads_of(a[1], "k", tokens, hk, d, at), v = heads_of(a[2], "v", tokens, hk, d, at);
     const int32_t* starts = index_of(a[3], "starts", seqs + 1, at);
     const int32_t* before = index_of(a[4], "before", seqs, at);
@@ -317,9 +334,7 @@ PyObject* py_decode(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (s != BSP_OK) return s;
     const int at = static_cast<int>(PyLong_AsLong(a[1]));
     if (PyErr_Occurred()) throw PyFailed{};
-    const Ref address(PyObject_GetAttr(a[2], s_address));
-    const auto* cache = static_cast<const bsp_kv_cache*>(PyLong_AsVoidPtr(address.p));
-    if (!cache) throw PyFailed{};
+    const bsp_kv_cache* cache = cache_on(cache_of(a[2]), at);
     const int64_t seqs = with_dims(a[3], "q", 3).size(0), heads = info[2], d = info[4];
     const Heads q = heads_of(a[3], "q", seqs, heads, d, at), o = heads_of(a[6], "o", seqs, heads, d, at);
     const int32_t* lens = index_of(a[4], "lens", seqs, at);

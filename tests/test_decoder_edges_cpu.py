@@ -21,3 +21,30 @@ def test_early_kernels_read_no_memory_as_constant(name):
     nothing they read is constant for as long as they live: no ld.global.nc."""
     assert not re.search(r"__ldg\s*\(|ld\.global\.nc|__restrict__", _code(name))
     assert name == "rope.cuh" or "stream_wait()" in _code(name)
+
+
+# ------------------------------------------------------------------ devices --
+torch = pytest.importorskip("torch")
+import bsp  # noqa: E402
+
+
+class OnGpu:
+    """Looks like a CUDA tensor on GPU `index`; has no memory there."""
+
+    def __init__(self, shape, dtype, index):
+        self._t = torch.zeros(shape, dtype=dtype)
+        self.shape, self.dtype, self.device = self._t.shape, dtype, torch.device("cuda", index)
+        self.is_cuda = True
+
+    def __getattr__(self, name):
+        return getattr(self._t, name)
+
+
+def test_cache_on_one_gpu():
+    """All four tensors of a cache are on one GPU, which the cache knows."""
+    parts = [((3, 2, 16, 64), torch.uint8), ((3, 2, 16, 64), torch.uint8), ((3, 2), torch.float32), ((3, 2), torch.float32)]
+    assert bsp.KvCache(*(OnGpu(*p, 1) for p in parts)).ordinal == 1
+    for other in range(4):
+        with pytest.raises(bsp.BspError) as e:
+            bsp.KvCache(*(OnGpu(*p, int(i == other)) for i, p in enumerate(parts)))
+        assert e.value.status == bsp.BSP_ERR_INVALID_ARG and "cuda:1" in str(e.value)

@@ -55,3 +55,28 @@ def test_calls_see_what_the_call_before_wrote(bsp, page, d):  # noqa: F811
     assert bool(torch.isfinite(gold[0]).all())
     for _ in range(5):
         assert all(torch.equal(a, b) for a, b in zip(run(False), gold))
+
+
+# ------------------------------------------------------------------ devices --
+def test_cache_of_another_gpu_is_refused(bsp):  # noqa: F811
+    """A cache says on which GPU it is; the calls compare that with their tensors
+    before anything is launched.  (The stand-in's memory is this GPU's, so that the
+    call could do no harm if it went on.)"""
+    torch = torch_()
+    cache = bsp.KvCache.empty(2, 1, 16, 64)
+    assert cache.ordinal == torch.cuda.current_device() and cache.k.device.index == cache.ordinal
+
+    class Elsewhere:
+        address, ordinal = cache.address, cache.ordinal + 1
+
+    x = torch.ones((1, 1, 64), device="cuda", dtype=torch.bfloat16)
+    o = torch.zeros_like(x)
+    plan = bsp.DecodePlan(bsp.device(), 1, 1, 1, 64, 16)
+    for call in (lambda c: bsp.kv_append(c, x, x, i32([0, 1]), i32([0]), i32([[0]])),
+                 lambda c: plan.execute(c, x, i32([1]), i32([[0]]), o)):
+        with pytest.raises(bsp.BspError, match="cache is on cuda:1, not on GPU 0") as e:
+            call(Elsewhere)
+        assert e.value.status == bsp.BSP_ERR_INVALID_ARG
+        call(cache)
+    bsp.device().synchronize()
+    assert bool((o == 1).all()) and bool(cache.k.any())
