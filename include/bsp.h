@@ -549,7 +549,12 @@ bsp_status bsp_prompt_plan_info(const bsp_prompt_plan* plan, int64_t info[16]);
  * [n_seqs][heads].  A sequence of length 0 gets O = 0 and lse = -inf.  What the
  * pages hold behind lens[s] is never used.  The plan is a workspace for up to
  * max_seqs sequences (any lengths) that one launch uses at a time: run a
- * plan's launches on one stream.  Options: max_ctas, timeout_ms. */
+ * plan's launches on one stream.  Options: max_ctas, timeout_ms.
+ * Scores, softmax and sums in fp32; for the product with the codes of V the
+ * weights are rounded to fp16, relative to their page's scale and the largest
+ * weight: 2^-11 of a weight, at most 2^-25 of the largest for those far below
+ * it.  O is rounded once.  Value scales of a row's pages may be 2^100 apart;
+ * beyond that what the smaller ones add to O may be dropped (not their weights). */
 typedef struct bsp_decode_plan bsp_decode_plan;
 
 bsp_status bsp_decode_plan_create(bsp_device* dev, int32_t max_seqs, int32_t heads, int32_t kv_heads, int32_t d,

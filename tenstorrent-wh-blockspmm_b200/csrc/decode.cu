@@ -16,15 +16,19 @@
 // tokens of it) and operand, swizzled so that ldmatrix reads without bank
 // conflicts.  Each of four warps takes 32 tokens with its own running maximum:
 //   S^T [16 tokens x 8 heads]  = K Q^T    m16n8k16, A = K, B = Q
-//   P'  = 2^(S c + b - m)                 c = scale log2 e 2^a: the value scale
-//                                         2^b goes into the exponent, so codes
-//                                         of V enter the product as they are;
-//                                         l sums P' 2^-b
+//   P'  = 2^(S c - m + 7 + b - r)         c = scale log2 e 2^a; m follows the
+//                                         largest S c; l sums P' 2^(r - b - 7)
 //   O^T [d x 8 heads]         += V^T P'   A = V (ldmatrix.trans), B = P'
+// V enters the product as its codes, so O is in units of 2^(r - 7), r the warp's
+// reference: b <= r <= b + 7 for the pages at hand, moved (and O with it, in
+// fp32) only when a page's b leaves that span.
 // e4m3 codes are exact in fp16.  Q is scaled to [1, 2) by a power of two per
 // head before it is rounded to fp16 (bf16's 8 bits fit; what falls below
 // 2^-14 of the head's largest value loses bits that the sum cannot show).
-// P' <= 2^8 is rounded to fp16 (2^-11); sums are in fp32.
+// P' <= 2^15 is rounded to fp16: 2^-11 of a weight, or, far below, 2^-25 of the
+// largest weight (2^-32 where the pages' scales are alike).  Were b part of m, one
+// page of large scale would take all other pages' weights below what fp16 holds,
+// whether its values count or not (a page of zeros has scale 1).  Sums are in fp32.
 //
 // Warps (192 threads): 0-3 as above, 4 issues the copies of K, 5 those of V;
 // they hold the page numbers and scales of the next tiles in their lanes, so
@@ -57,6 +61,8 @@ constexpr int kDcTmaWarp = 4;  // K; the next one V
 constexpr int kDcMaxSlots = 12;
 constexpr int kDcJoin = 8;
 constexpr float kDcRescale = 8.f;    // log2 of the growth that moves the maximum
+constexpr float kDcSpan = 7.f;       // how far a page's exponent may be below the reference: 2^(8 + 7) fits fp16
+constexpr float kDcNoRef = -128.f;   // below any exponent
 
 struct DcHeader {
   uint64_t full[kDcMaxSlots], empty[kDcMaxSlots];
@@ -66,7 +72,7 @@ struct DcHeader {
   uint32_t each, extra;
   int32_t last;         // this CTA joins the row
   int abort_flag;
-  float scales[kDcMaxSlots][kDcTile / 16];  // 2^a or 2^b of each 16 tokens of a slot
+  float scales[kDcMaxSlots][kDcTile / 16];  // 2^a, or b, of each 16 tokens of a slot
 };
 static_assert(sizeof(DcHeader) <= 1024, "header must fit its 1 KiB slot");
 
@@ -221,6 +227,9 @@ __device__ __forceinline__ void dc_produce(const DecodeParams& p, DcHeader* hdr,
     auto scale_of = [&](int32_t id) {
       return id >= 0 ? scale[static_cast<int64_t>(id) * p.cache.kv_heads + kvh] : 1.f;
     };
+    auto held = [&](float s) {  // what the slot holds of a scale: a V slot its exponent
+      return kind ? static_cast<float>(static_cast<int>((__float_as_uint(s) >> 23) & 0xFFu) - 127) : s;
+    };
     int32_t id = checked(page_of(0)), id_next = page_of(per_batch);
     float sc = scale_of(id);
 #pragma unroll 1
@@ -239,7 +248,7 @@ __device__ __forceinline__ void dc_produce(const DecodeParams& p, DcHeader* hdr,
         tma_load_4d_pred(ring + slot * dc_slot_bytes(kD) + sub * box * kD, tm, 0, 0, kvh,
                          id >= 0 ? id : static_cast<int32_t>(p.cache.n_pages), bar, mine);
         if (at == k)
-          for (int i = 0; i < box / 16; ++i) hdr->scales[slot][sub * (box / 16) + i] = sc;
+          for (int i = 0; i < box / 16; ++i) hdr->scales[slot][sub * (box / 16) + i] = held(sc);
         const uint32_t bytes = static_cast<uint32_t>(__popc(__ballot_sync(0xffffffffu, mine))) * box * kD;
         __syncwarp();  // the scales are written before lane 0 arrives
         mbar_arrive_expect_tx_pred(bar, bytes, lane == 0);
@@ -265,12 +274,26 @@ __device__ __forceinline__ void dc_produce(const DecodeParams& p, DcHeader* hdr,
   __syncwarp();
 }
 
-// A warp's (m, l, O) to shared memory, slot of four.
+// A warp's (m, l, O) to shared memory, slot of four, as what the results of warps
+// and parts are joined by: O = 2^m O', sum of weights = 2^m l'.  The reference goes
+// into m and l as far as 2^+-50, so that a factor 2^(m - m') never takes another's
+// sum of weights below fp32's range; what is left of it into O.
 template <int kD, int kNt>
 __device__ __forceinline__ void put_result(float* red_o, float* red_m, float* red_l, int slot, int g, int t,
-                                          const float (&o)[kNt][kD / 16][4], const float (&m)[kNt][2],
-                                          const float (&l)[kNt][2], int nh) {
+                                          float (&o)[kNt][kD / 16][4], const float (&m)[kNt][2],
+                                          const float (&l)[kNt][2], float ref, int nh) {
   constexpr int kHeads = 8 * kNt;
+  const float fit = fminf(fmaxf(ref, -50.f), 50.f);
+  if (ref != fit) {
+    const float f = ex2(ref - fit);
+#pragma unroll
+    for (int n = 0; n < kNt; ++n)
+#pragma unroll
+      for (int c = 0; c < kD / 16; ++c)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[n][c][i] *= f;
+  }
+  const float shift = fit - kDcSpan, unit = ex2(-shift);
 #pragma unroll
   for (int n = 0; n < kNt; ++n) {
 #pragma unroll
@@ -281,8 +304,8 @@ __device__ __forceinline__ void put_result(float* red_o, float* red_m, float* re
       x += __shfl_xor_sync(0xffffffffu, x, 16);
       const int head = 8 * n + 2 * t + h;
       if (g == 0) {
-        red_m[slot * kHeads + head] = m[n][h];
-        red_l[slot * kHeads + head] = x;
+        red_m[slot * kHeads + head] = m[n][h] + shift;
+        red_l[slot * kHeads + head] = x * unit;
       }
       float* dst = red_o + (slot * kHeads + head) * kD + 2 * g;
       if (head < nh)
@@ -346,6 +369,7 @@ __device__ __forceinline__ void dc_consume(const DecodeParams& p, DcHeader* hdr,
       qs[n][1] = __shfl_sync(0xffffffffu, up, 8 * t + 4) * p.scale_log2;
     }
     float o[kNt][kChunks][4], m[kNt][2], l[kNt][2];
+    float ref = kDcNoRef;
 #pragma unroll
     for (int n = 0; n < kNt; ++n) {
       m[n][0] = m[n][1] = -INFINITY;
@@ -373,7 +397,7 @@ __device__ __forceinline__ void dc_consume(const DecodeParams& p, DcHeader* hdr,
       } else {
         const uint32_t kb = ring + slot * dc_slot_bytes(kD) + first;
         const float* k_scales = hdr->scales[slot] + kDcSlices * warp;
-        float s[kDcSlices][kNt][4], vs_inv[kDcSlices];
+        float s[kDcSlices][kNt][4];
         bool grow = false;
         float mx[kNt][2];
 #pragma unroll
@@ -405,20 +429,17 @@ __device__ __forceinline__ void dc_consume(const DecodeParams& p, DcHeader* hdr,
         free_slot();
         ok = wait_slot();
         if (!ok) break;
-        const uint32_t vb = ring + slot * dc_slot_bytes(kD) + first;
+        const uint32_t vb_at = ring + slot * dc_slot_bytes(kD) + first;
         const float* v_scales = hdr->scales[slot] + kDcSlices * warp;
 #pragma unroll
         for (int sl = 0; sl < kDcSlices; ++sl) {
-          const float vs = v_scales[sl];
-          const float eb = static_cast<float>(static_cast<int>(__float_as_uint(vs) >> 23) - 127);
-          vs_inv[sl] = __uint_as_float((254u << 23) - __float_as_uint(vs));  // 2^-b of vs = 2^b
           const bool in0 = 16 * sl + g < left, in1 = 16 * sl + g + 8 < left;
 #pragma unroll
           for (int n = 0; n < kNt; ++n) {
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-              s[sl][n][h] = in0 ? s[sl][n][h] + eb : -INFINITY;
-              s[sl][n][2 + h] = in1 ? s[sl][n][2 + h] + eb : -INFINITY;
+              s[sl][n][h] = in0 ? s[sl][n][h] : -INFINITY;
+              s[sl][n][2 + h] = in1 ? s[sl][n][2 + h] : -INFINITY;
               mx[n][h] = fmaxf(mx[n][h], fmaxf(s[sl][n][h], s[sl][n][2 + h]));
             }
           }
@@ -435,37 +456,29 @@ __device__ __forceinline__ void dc_consume(const DecodeParams& p, DcHeader* hdr,
             grow |= x > m[n][h] + kDcRescale;
           }
         }
-        if (__any_sync(0xffffffffu, grow)) {
+        // log2 of the factor in a slice's P', and its inverse
+        float up[kDcSlices], down[kDcSlices], vb[kDcSlices];
+        bool move = grow;
 #pragma unroll
-          for (int n = 0; n < kNt; ++n) {
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              const float mn = fmaxf(m[n][h], mx[n][h]);
-              const float f = m[n][h] == -INFINITY ? 0.f : ex2(m[n][h] - mn);
-              m[n][h] = mn;
-              l[n][h] *= f;
-#pragma unroll
-              for (int c = 0; c < kChunks; ++c) {
-                o[n][c][h] *= f;
-                o[n][c][2 + h] *= f;
-              }
-            }
-          }
+        for (int sl = 0; sl < kDcSlices; ++sl) {
+          vb[sl] = 16 * sl < left ? v_scales[sl] : vb[0];
+          up[sl] = kDcSpan + vb[sl] - ref;
+          down[sl] = ex2(-up[sl]);
+          move |= !(fabsf(2.f * up[sl] - kDcSpan) <= kDcSpan);
         }
         // Codes behind the last token are whatever the page held: clear them
         // (0 times a NaN code would not be 0).
         const bool tail = left < 16 * kDcSlices;
-#pragma unroll
-        for (int sl = 0; sl < kDcSlices; ++sl) {
+        auto add_slice = [&](int sl) {
           uint32_t pb[kNt][2];
 #pragma unroll
           for (int n = 0; n < kNt; ++n) {
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-              const float mm = m[n][h] == -INFINITY ? 0.f : m[n][h];
+              const float mm = (m[n][h] == -INFINITY ? 0.f : m[n][h]) - up[sl];
               s[sl][n][h] = ex2(s[sl][n][h] - mm);
               s[sl][n][2 + h] = ex2(s[sl][n][2 + h] - mm);
-              l[n][h] += (s[sl][n][h] + s[sl][n][2 + h]) * vs_inv[sl];
+              l[n][h] += (s[sl][n][h] + s[sl][n][2 + h]) * down[sl];
             }
             pb[n][0] = transpose8(half_pair(s[sl][n][0], s[sl][n][1]));  // B: tokens 2 t, 2 t + 1 of head g
             pb[n][1] = transpose8(half_pair(s[sl][n][2], s[sl][n][3]));  // tokens 2 t + 8, 2 t + 9
@@ -479,7 +492,7 @@ __device__ __forceinline__ void dc_consume(const DecodeParams& p, DcHeader* hdr,
 #pragma unroll
           for (int c = 0; c < kChunks; c += 2) {
             uint32_t r[4];
-            ldmatrix4t((vb ^ (c << 4)) + sl * 16 * kD, r);
+            ldmatrix4t((vb_at ^ (c << 4)) + sl * 16 * kD, r);
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
               // register: codes (token 2 t, d 2 g), (2 t, 2 g + 1), (2 t + 1, 2 g), (2 t + 1, 2 g + 1)
@@ -491,13 +504,80 @@ __device__ __forceinline__ void dc_consume(const DecodeParams& p, DcHeader* hdr,
               for (int n = 0; n < kNt; ++n) mma16816(o[n][c + i], a0, a1, a2, a3, pb[n][0], pb[n][1]);
             }
           }
+        };
+        if (__any_sync(0xffffffffu, move)) {
+#pragma unroll 1
+          for (bool last = false; !last;) {
+            // The reference nearest to the present one that holds both slices, or,
+            // where none does, the first slice (which is added here then) and after
+            // it the second.  Downwards O's numbers grow: they stay below 2^100, and
+            // what a page that the reference cannot come down to would add is less
+            // than 2^-60 of O's largest: it only counts in l.
+            last = fabsf(vb[0] - vb[1]) <= kDcSpan;
+            float to = fminf(fmaxf(ref, last ? fmaxf(vb[0], vb[1]) : vb[0]), (last ? fminf(vb[0], vb[1]) : vb[0]) + kDcSpan);
+            if (to < ref) {
+              float top = 0.f;
+#pragma unroll
+              for (int n = 0; n < kNt; ++n)
+#pragma unroll
+                for (int c = 0; c < kChunks; ++c)
+#pragma unroll
+                  for (int i = 0; i < 4; ++i) top = fmaxf(top, fabsf(o[n][c][i]));
+              const uint32_t bits = __reduce_max_sync(0xffffffffu, __float_as_uint(top));
+              const int room = min(max(227 - static_cast<int>(bits >> 23), 0), 120);
+              if (bits != 0) to = fmaxf(to, ref - static_cast<float>(room));
+            }
+            const float unit = ex2(fminf(ref - to, 120.f));
+            ref = to;
+#pragma unroll
+            for (int n = 0; n < kNt; ++n) {
+#pragma unroll
+              for (int h = 0; h < 2; ++h) {
+                const float mn = fmaxf(m[n][h], mx[n][h]);
+                const float f = m[n][h] == -INFINITY ? 0.f : ex2(m[n][h] - mn);
+                m[n][h] = mn;
+                l[n][h] *= f;
+#pragma unroll
+                for (int c = 0; c < kChunks; ++c) {
+                  o[n][c][h] *= f * unit;
+                  o[n][c][2 + h] *= f * unit;
+                }
+              }
+            }
+#pragma unroll
+            for (int sl = 0; sl < kDcSlices; ++sl) {
+              up[sl] = kDcSpan + vb[sl] - ref;
+              down[sl] = ex2(-up[sl]);
+              if (up[sl] < 0.f && (sl == 0 || last)) {
+#pragma unroll
+                for (int n = 0; n < kNt; ++n)
+#pragma unroll
+                  for (int h = 0; h < 2; ++h) {
+                    const float mm = m[n][h] == -INFINITY ? 0.f : m[n][h];
+                    l[n][h] += ex2(s[sl][n][h] - mm) + ex2(s[sl][n][2 + h] - mm);
+                  }
+                up[sl] = -INFINITY;
+                down[sl] = 0.f;
+              }
+            }
+            if (!last) {
+              add_slice(0);
+#pragma unroll
+              for (int n = 0; n < kNt; ++n)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) s[0][n][i] = -INFINITY;  // it has been added
+              vb[0] = vb[1];
+            }
+          }
         }
+#pragma unroll
+        for (int sl = 0; sl < kDcSlices; ++sl) add_slice(sl);
       }
       free_slot();
     }
     // ---- the four warps' results of this piece
     consumers_sync();  // the last piece's have been read
-    put_result<kD, kNt>(red_o, red_m, red_l, warp, g, t, o, m, l, nh);
+    put_result<kD, kNt>(red_o, red_m, red_l, warp, g, t, o, m, l, ref, nh);
     consumers_sync();
     const int tid = 32 * warp + lane;
     const bool whole = pc.n == pc.tiles;

@@ -80,3 +80,127 @@ def test_cache_of_another_gpu_is_refused(bsp):  # noqa: F811
         call(cache)
     bsp.device().synchronize()
     assert bool((o == 1).all()) and bool(cache.k.any())
+
+
+# ------------------------------------------------------- value scales far apart --
+def _pages_of(kind, size, n, page, hk, d, rng):
+    """Values [n, hk, d] whose pages have scales far apart."""
+    v = rng.normal(0, 1, (n, hk, d)) * size
+    at = np.arange(n)[:, None, None]
+    if kind == "zeros":           # the first page holds zeros: scale 1
+        v[: min(page, n)] = 0
+    elif kind == "zeros_last":
+        v[-(n % page or page):] = 0
+    elif kind == "outlier":       # one token far larger than all others
+        v[n // 3] = 1e3
+    elif kind == "turns":         # three sizes in turn
+        v = v * np.choose(at // page % 3, [1.0, 2.0 ** 20, 2.0 ** -20])
+    elif kind == "falling":
+        v = v * 2.0 ** (-2.0 * (at // page))
+    elif kind == "rising":
+        v = v * 2.0 ** (2.0 * (at // page))
+    return v
+
+
+FAR = [("zeros", 1e-3), ("zeros", 1e-4), ("zeros", 1e-5), ("zeros", 1e-12), ("zeros", 1e-25), ("zeros_last", 1e-5),
+       ("outlier", 1e-4), ("outlier", 1e-20), ("turns", 1.0), ("falling", 1e6), ("rising", 1e-6), ("plain", 1.0)]
+
+
+@pytest.mark.parametrize("kind,size", FAR, ids=[f"{k}_{s:g}" for k, s in FAR])
+@pytest.mark.parametrize("hq,hk,d,page", [(8, 2, 64, 16), (16, 1, 128, 16), (4, 1, 128, 64), (20, 1, 64, 32)])
+def test_decode_value_scales(bsp, kind, size, hq, hk, d, page):  # noqa: F811
+    """The output's error is that of the weights (2^-11, rounded to fp16) times
+    sum p |v|, whatever the scales of the pages; weights below 2^-14 of the largest
+    are off by up to 2^-25 of it."""
+    torch = torch_()
+    rng = np.random.default_rng(11)
+    lens = [640, 100, 17]
+    per = [-(-n // page) for n in lens]
+    pages = page_table(rng, lens, page, sum(per))
+    cache = bsp.KvCache.empty(sum(per), hk, page, d)
+    k = rng.normal(0, 1, (sum(lens), hk, d))
+    v = np.concatenate([_pages_of(kind, size, n, page, hk, d, rng) for n in lens])
+    bsp.kv_append(cache, *(cuda(ref.bf16(x), torch.bfloat16) for x in (k, v)), i32(np.concatenate([[0], np.cumsum(lens)])),
+                  i32([0] * 3), cuda(pages))
+    q = ref.bf16(rng.normal(0, 1, (3, hq, d)))
+    codes, scales = [cache.k.cpu().numpy(), cache.v.cpu().numpy()], [host(cache.k_scale), host(cache.v_scale)]
+    keys, values = ([(ref.VALUES[c[pages[s][: per[s]]]] * x[pages[s][: per[s]]][:, :, None, None])
+                     .transpose(1, 0, 2, 3).reshape(hk, -1, d)[:, :n] for s, n in enumerate(lens)]
+                    for c, x in zip(codes, scales))
+    gold, lse = np.zeros(q.shape), np.zeros(q.shape[:2])
+    weight, size_, most = np.zeros(q.shape), np.zeros(q.shape[:2] + (1,)), np.zeros(q.shape)
+    for s in range(3):
+        for h in range(hq):
+            qq, kk, vv = q[s, h][None].astype(float), keys[s][h // (hq // hk)], values[s][h // (hq // hk)]
+            gold[s, h], lse[s, h], weight[s, h] = (x[0] for x in ref.attention(qq, kk, vv, d ** -0.5, [lens[s]]))
+            size_[s, h, 0] = d ** -0.5 * (np.abs(qq) @ np.abs(kk).T).max()
+            top = np.exp(d ** -0.5 * (qq @ kk.T).max() - lse[s, h])  # the largest weight
+            most[s, h] = 2.0 ** -25 * top * np.abs(vv).sum(0)
+    weight = weight + most / (2 * ref.UH)
+    for ctas in (0, 1, 5):
+        plan = bsp.DecodePlan(bsp.device(), 3, hq, hk, d, page, opts=bsp.make_opts(max_ctas=ctas))
+        o, l = torch.full(q.shape, float("nan"), device="cuda").bfloat16(), torch.full(q.shape[:2], float("nan"), device="cuda")
+        plan.execute(cache, cuda(q, torch.bfloat16), i32(lens), cuda(pages), o, lse=l)
+        bsp.device().synchronize()
+        # (the 1e-30 of the check is far below every value here but those of 1e-25)
+        check_attention(o, l, gold, lse, weight, size_, 2 * ref.UH)
+
+
+@pytest.mark.parametrize("d,hq", [(64, 4), (128, 16)])
+def test_decode_scales_at_the_ends(bsp, d, hq):  # noqa: F811
+    """Pages at the two ends of the scales' range, 2^-100 and 2^119: the large
+    values are the output, and the sum of the weights is not touched by them."""
+    torch = torch_()
+    rng = np.random.default_rng(2)
+    page, n = 16, 96
+    cache = bsp.KvCache.empty(n // page, 1, page, d)
+    v = np.ones((n, 1, d)) * np.where(np.arange(n) // page % 2, 3e38, 1e-30)[:, None, None]
+    k = rng.normal(0, 1, (n, 1, d))
+    pages = i32(np.arange(n // page)[None])
+    bsp.kv_append(cache, cuda(ref.bf16(k), torch.bfloat16), cuda(ref.bf16(v), torch.bfloat16), i32([0, n]), i32([0]), pages)
+    assert {float(x) for x in cache.v_scale.flatten()} == {2.0 ** -100, 2.0 ** 119}
+    q = ref.bf16(rng.normal(0, 1, (1, hq, d)))
+    o, l = torch.empty((1, hq, d), device="cuda").bfloat16(), torch.empty((1, hq), device="cuda")
+    kk, vv = (ref.VALUES[c.cpu().numpy()[:, 0]].reshape(n, d) * host(s)[:, 0].repeat(page)[:, None]
+              for c, s in ((cache.k, cache.k_scale), (cache.v, cache.v_scale)))
+    gold, lse, weight = ref.attention(q[0].astype(float), kk, vv, d ** -0.5, [n] * hq)
+    size = d ** -0.5 * (np.abs(q[0].astype(float)) @ np.abs(kk).T).max(1, keepdims=True)
+    for ctas in (1, 0):
+        plan = bsp.DecodePlan(bsp.device(), 1, hq, 1, d, page, opts=bsp.make_opts(max_ctas=ctas))
+        plan.execute(cache, cuda(q, torch.bfloat16), i32([n]), pages, o, lse=l)
+        bsp.device().synchronize()
+        check_attention(o[0], l[0], gold, lse, weight, size, 2 * ref.UH)
+
+
+@pytest.mark.parametrize("d,page", [(64, 16), (128, 64)])
+def test_decode_many_small_weights_beside_a_large_one(bsp, d, page):  # noqa: F811
+    """One token takes nearly all the weight and its value is zero; 20000 tokens of
+    2^-22 each, of one key, are the output."""
+    torch = torch_()
+    n, hq = 20001, 4
+    per = -(-n // page)
+    cache = bsp.KvCache.empty(per, 1, page, d)
+    rng = np.random.default_rng(3)
+    k = np.zeros((n, 1, d))
+    k[0, 0, 0] = 2.0
+    v = rng.normal(0.5, 1, (n, 1, d))
+    v[0] = 0
+    v[:: page, 0, :: 7] = 4.0  # the pages have one scale
+    v[0] = 0
+    v[1, 0, 3] = 4.0
+    pages = i32(np.arange(per)[None])
+    bsp.kv_append(cache, cuda(ref.bf16(k), torch.bfloat16), cuda(ref.bf16(v), torch.bfloat16), i32([0, n]), i32([0]), pages)
+    q = np.zeros((1, hq, d), np.float32)
+    q[0, :, 0] = ref.bf16([7.5, 7.6, 7.7, 7.8])  # scores of 15 to 15.6 at scale 1: weights of 2^-22 beside it
+    o, l = torch.empty((1, hq, d), device="cuda").bfloat16(), torch.empty((1, hq), device="cuda")
+    kk, vv = (ref.VALUES[c.cpu().numpy()[:, 0]].reshape(-1, d)[:n] * host(s)[:, 0].repeat(page)[:n, None]
+              for c, s in ((cache.k, cache.k_scale), (cache.v, cache.v_scale)))
+    gold, lse, weight = ref.attention(q[0].astype(float), kk, vv, 1.0, [n] * hq)
+    size = (np.abs(q[0].astype(float)) @ np.abs(kk).T).max(1, keepdims=True)
+    top = np.exp((q[0].astype(float) @ kk.T).max(1) - lse)
+    weight = weight + 2.0 ** -32 * top[:, None] * np.abs(vv).sum(0) / (2 * ref.UH)
+    for ctas in (0, 1):  # one: a quarter of the tokens is in the warp of the large one
+        plan = bsp.DecodePlan(bsp.device(), 1, hq, 1, d, page, opts=bsp.make_opts(max_ctas=ctas))
+        plan.execute(cache, cuda(q, torch.bfloat16), i32([n]), pages, o, scale=1.0, lse=l)
+        bsp.device().synchronize()
+        check_attention(o[0], l[0], gold, lse, weight, size, 2 * ref.UH)
