@@ -523,9 +523,11 @@ bsp_status bsp_kv_append(bsp_device* dev, const bsp_kv_cache* cache, const void*
  * which the parts' results meet, so run its launches one after the other (on
  * one stream); any other plan may run on several streams at once.
  * Scores, softmax and sums in fp32; probabilities are rounded to bf16 for the
- * product with V; O is rounded once.  A hidden key may hold anything, but V is
- * multiplied in steps of 128 keys with weights that are 0 for hidden ones: a NaN
- * or infinity in V reaches the rows that see any key of its step.
+ * product with V; O is rounded once.  A hidden key may hold anything and its
+ * weight is exactly 0, but V is multiplied in steps of 128 keys for tiles of 128
+ * rows (128 / P queries of P heads, info[11]), and 0 times a NaN or infinity is
+ * NaN: one in V reaches its column of every row of a tile in which some row sees a
+ * key of its step, earlier queries among them; not the rows that see no key at all.
  * Options: max_ctas, timeout_ms, group_rows = -1 (nothing is cut). */
 typedef struct bsp_prompt_plan bsp_prompt_plan;
 

@@ -131,14 +131,15 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
 // 2^x of two values without the exponential unit: x = n + f with n the nearest
 // whole number (adding 1.5 * 2^23 leaves it in the low bits), 2^f by a
 // polynomial of degree 4 on [-1/2, 1/2] with p(0) = 1, fitted for the least
-// relative error (2.9e-6), and n added to the exponent.  x <= 127; below -126
-// (a masked score) the result is 2^-126, which vanishes beside the maximum's
-// 2^-8 or more.
+// relative error (2.9e-6), and n added to the exponent.  x <= 127; from -127
+// down (a masked score) the result is 0: p(0) = 1, and its exponent less 127 is an
+// empty field.  (So a hidden key weighs nothing, whatever its value.  Between -127
+// and -126 the result is somewhere below 2^-126.)
 __device__ __forceinline__ uint64_t exp2_pair(uint64_t x) {
   const uint64_t magic = pair_of(12582912.f, 12582912.f), back = pair_of(-12582912.f, -12582912.f);
   float a, b;
   unpair(x, a, b);
-  x = pair_of(fmaxf(a, -126.f), fmaxf(b, -126.f));
+  x = pair_of(fmaxf(a, -127.f), fmaxf(b, -127.f));
   const uint64_t t = add2(x, magic);
   const uint64_t f = fma2(add2(t, back), pair_of(-1.f, -1.f), x);
   uint64_t p = fma2(f, pair_of(0.009582852944731712f, 0.009582852944731712f),
@@ -309,12 +310,12 @@ __device__ __forceinline__ void pr_mma(const PromptParams& p, PrHeader* hdr, uin
   __syncwarp();
 }
 
-// Store 32 bytes of a row.
-__device__ __forceinline__ void store32(uint16_t* dst, const uint32_t (&o)[32], int at, float f) {
+// Store 32 bytes of a row; keep: all bits, or none (zeros).
+__device__ __forceinline__ void store32(uint16_t* dst, const uint32_t (&o)[32], int at, float f, uint32_t keep) {
   uint32_t w[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i)
-    w[i] = pack2(__uint_as_float(o[at + 2 * i]) * f, __uint_as_float(o[at + 2 * i + 1]) * f);
+    w[i] = pack2(__uint_as_float(o[at + 2 * i]) * f, __uint_as_float(o[at + 2 * i + 1]) * f) & keep;
   *reinterpret_cast<uint4*>(dst) = make_uint4(w[0], w[1], w[2], w[3]);
   *reinterpret_cast<uint4*>(dst + 8) = make_uint4(w[4], w[5], w[6], w[7]);
 }
@@ -516,9 +517,9 @@ __device__ __forceinline__ void pr_softmax(const PromptParams& p, PrHeader* hdr,
     if (!wait_all(&hdr->o_full[t], outs & 1, ctl, ST_TIMEOUT_EPILOGUE)) return;
     ++outs;
     tc_fence_after();
-    if (m == -INFINITY && l < 1.f) l = 0.f;  // no key: exp2_pair gave 2^-126 for each masked one
     const bool whole = un.parts == 1;
     const float inv = whole ? share_of(m, l) : 1.f;
+    const uint32_t keep = l == 0.f ? 0u : ~0u;  // no key: O is 0 but for a NaN or infinity in V
 #pragma unroll 1
     for (int c = 0; c < kD / 32; ++c) {
       uint32_t o[32];
@@ -530,8 +531,8 @@ __device__ __forceinline__ void pr_softmax(const PromptParams& p, PrHeader* hdr,
           reinterpret_cast<uint4*>(work)[(8 * c + i) * 128 + row] =
               make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
       } else if (valid) {
-        store32(orow + 32 * c, o, 0, inv);
-        store32(orow + 32 * c + 16, o, 16, inv);
+        store32(orow + 32 * c, o, 0, inv, keep);
+        store32(orow + 32 * c + 16, o, 16, inv, keep);
       }
     }
     if (valid && !whole) {

@@ -5,7 +5,7 @@ import numpy as np
 import pytest
 
 import decoder_ref as ref
-from test_decoder_gpu import bsp, check_attention, cuda, host, i32, page_table, torch_  # noqa: F401
+from test_decoder_gpu import bsp, check_attention, cuda, host, i32, page_table, prompt_gold, torch_  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 
@@ -204,3 +204,75 @@ def test_decode_many_small_weights_beside_a_large_one(bsp, d, page):  # noqa: F8
         plan.execute(cache, cuda(q, torch.bfloat16), i32([n]), pages, o, scale=1.0, lse=l)
         bsp.device().synchronize()
         check_attention(o[0], l[0], gold, lse, weight, size, 2 * ref.UH)
+
+
+# ------------------------------------------------------------ masked values --
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("hq,hk", [(1, 1), (4, 1)])
+def test_prompt_hidden_values_weigh_nothing(bsp, d, hq, hk):  # noqa: F811
+    """Values near the type's largest and lowest at keys that the causal mask hides,
+    at each place of a step: exactly nothing of them in the rows before."""
+    torch = torch_()
+    n = 300
+    rng = np.random.default_rng(12)
+    q = ref.bf16(rng.normal(0, 1, (n, hq, d)))
+    k, v = (ref.bf16(rng.normal(0, 1, (n, hk, d))) for _ in range(2))
+    qt, kt, vt = (cuda(x, torch.bfloat16) for x in (q, k, v))
+    gold = prompt_gold(q.astype(float), k.astype(float), v.astype(float), [n], [n], hk, d ** -0.5, True)
+    plan = bsp.PromptPlan(bsp.device(), [n], [n], hq, hk, d)
+    o, lse = torch.empty_like(qt), torch.empty((n, hq), device="cuda")
+    for at in (1, 30, 64, 127, 130, 200, 290):
+        v2 = vt.clone()
+        v2[at:, :, ::2] = 3.3e38
+        v2[at:, :, 1::2] = -3.3e38
+        plan.execute(qt, kt, v2, o, lse=lse)
+        bsp.device().synchronize()
+        check_attention(o[:at], lse[:at], *(x[:at] for x in gold), ref.U16)
+
+
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), 3.3e38])
+@pytest.mark.parametrize("cut", [False, True])
+@pytest.mark.parametrize("d", [64, 128])
+def test_prompt_rows_without_a_key_are_zero(bsp, bad, cut, d):  # noqa: F811
+    """Queries that see no key get O = 0 and lse = -inf, whatever V holds."""
+    torch = torch_()
+    n, m = (2100, 1500) if cut else (257, 200)
+    q, k, v = (torch.randn((x, h, d), device="cuda").bfloat16() for x, h in ((n, 2), (m, 1), (m, 1)))
+    v[:] = bad
+    plan = bsp.PromptPlan(bsp.device(), [n], [m], 2, 1, d)
+    assert (plan.info()["workspace_bytes"] > 0) == cut
+    o, lse = torch.full_like(q, float("nan")), torch.full((n, 2), float("nan"), device="cuda")
+    plan.execute(q, k, v, o, lse=lse)
+    bsp.device().synchronize()
+    assert bool((o[: n - m] == 0).all()) and bool(torch.isneginf(lse[: n - m]).all())
+    assert not bool((o[n - m:] == 0).any()) and bool(torch.isfinite(lse[n - m:]).all())
+
+
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+@pytest.mark.parametrize("hq,hk,d", [(1, 1, 128), (4, 1, 64), (3, 3, 128)])
+def test_prompt_value_that_is_not_finite(bsp, bad, hq, hk, d):  # noqa: F811
+    """A NaN or infinity in V: not finite where it is seen, in its column alone;
+    rows of tiles that do not run its step of 128 keys, and other columns, keep
+    their bits."""
+    torch = torch_()
+    n, more = 500, 60
+    q, k, v = (torch.randn((x, h, d), device="cuda").bfloat16() for x, h in ((n, hq), (n + more, hk), (n + more, hk)))
+    plan = bsp.PromptPlan(bsp.device(), [n], [n + more], hq, hk, d)
+    tokens = 128 // plan.info()["packed_heads"]
+    o, o2 = torch.empty_like(q), torch.empty_like(q)
+    lse, lse2 = (torch.empty((n, hq), device="cuda") for _ in range(2))
+    plan.execute(q, k, v, o, lse=lse)
+    for at in (0, 59, 128, 187, 300, n + more - 1):
+        v2 = v.clone()
+        v2[at, 0, 3] = bad
+        plan.execute(q, k, v2, o2, lse=lse2)
+        bsp.device().synchronize()
+        seen = torch.arange(n, device="cuda") + more >= at
+        heads = slice(0, hq // hk)
+        assert not bool(torch.isfinite(o2[seen][:, heads, 3]).any())
+        # the last query of a row's tile, and the keys that the tile's steps cover
+        last = (torch.arange(n, device="cuda") // tokens * tokens + tokens - 1).clamp(max=n - 1)
+        runs = (last + more + 1 + 127) // 128 * 128 > at // 128 * 128
+        same = torch.ones_like(o, dtype=torch.bool)
+        same[runs.nonzero()[:, 0], heads, 3] = False
+        assert torch.equal(o2[same], o[same]) and torch.equal(lse2, lse)
