@@ -499,10 +499,11 @@ typedef struct bsp_kv_cache {
  * position before they are stored (table NULL: stored as they are).
  * Optional: q [tokens][heads][d] rotated to q_out, rotated keys to k_out
  * (NULL skips them; q_out may be q, k_out may be k).
- * A (page, head) keeps the smallest power of two e that holds its largest
- * magnitude in e4m3's range (448); when later tokens need a larger one, the
- * page's earlier codes are rounded to it again (exact but for values that
- * fall below e4m3's normal range).  Pages of different sequences must differ.
+ * A (page, head) keeps the smallest power of two that holds its largest
+ * magnitude in e4m3's range (448), within [2^-100, 2^119], 1 while it holds only
+ * zeros; when later tokens need a larger one, the page's earlier codes are
+ * rounded to it again (exact but for values that fall below e4m3's normal range).
+ * Pages of different sequences must differ.
  * starts: int32 [n_seqs + 1]; before: int32 [n_seqs]; tokens = starts[n_seqs]. */
 bsp_status bsp_kv_append(bsp_device* dev, const bsp_kv_cache* cache, const void* k, int64_t k_token, int64_t k_head,
                          const void* v, int64_t v_token, int64_t v_head, int64_t tokens, int32_t n_seqs,

@@ -139,6 +139,16 @@ struct Target {
   float scale;     // 2^-e
 };
 
+// The warp looks whether `bytes` codes (a multiple of 16) are all zeros.
+__device__ __forceinline__ bool only_zeros(const uint8_t* codes, int bytes, int lane) {
+  uint32_t some = 0;
+  for (int i = lane; i < bytes / 16; i += 32) {
+    const uint4 c = reinterpret_cast<const uint4*>(codes)[i];
+    some |= c.x | c.y | c.z | c.w;
+  }
+  return !__any_sync(0xFFFFFFFFu, (some & 0x7F7F7F7Fu) != 0);
+}
+
 // The page's exponent from the lanes' maxima and what the page holds; earlier
 // codes are rounded again where it grew.
 template <int kD>
@@ -159,7 +169,10 @@ __device__ __forceinline__ Target settle(const AppendParams& p, const Chunk& ck,
   }
   int e = scale_exponent(m);
   if (ck.slot > 0) {
-    const int was = min(max(static_cast<int>((old_bits >> 23) & 0xFFu) - 127, -100), 119);
+    int was = min(max(static_cast<int>((old_bits >> 23) & 0xFFu) - 127, -100), 119);
+    // Zeros have no size: a page that holds nothing else has scale 1, which smaller
+    // values behind them would be rounded away with.  Any scale is theirs.
+    if (was == 0 && e < 0 && only_zeros(codes, ck.slot * kD, lane)) was = e;
     if (was >= e) {
       e = was;
     } else {

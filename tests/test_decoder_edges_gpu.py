@@ -276,3 +276,40 @@ def test_prompt_value_that_is_not_finite(bsp, bad, hq, hk, d):  # noqa: F811
         same = torch.ones_like(o, dtype=torch.bool)
         same[runs.nonzero()[:, 0], heads, 3] = False
         assert torch.equal(o2[same], o[same]) and torch.equal(lse2, lse)
+
+
+# ------------------------------------------------------------------- zeros --
+@pytest.mark.parametrize("page,d,hk,zeros,after", [(16, 64, 1, 1, 1), (16, 128, 2, 15, 1), (64, 128, 3, 7, 40),
+                                                   (128, 64, 2, 100, 28), (128, 128, 1, 127, 1)])
+@pytest.mark.parametrize("size", [1e-2, 1e-4, 1e-12])
+def test_append_small_values_behind_zeros(bsp, page, d, hk, zeros, after, size):  # noqa: F811
+    """A page that begins with zeros takes the scale of the values that follow, as
+    if they stood alone; a page that holds one code at scale 1 keeps it."""
+    torch = torch_()
+    rng = np.random.default_rng(page + zeros)
+    x = ref.bf16(rng.normal(0, size, (after, hk, d)))
+    xt = cuda(x, torch.bfloat16)
+    nothing = torch.zeros((zeros, hk, d), device="cuda", dtype=torch.bfloat16)
+    nothing[:, :, 1] = -0.0
+    cache = bsp.KvCache.empty(2, hk, page, d)
+    pages = i32([[1]])
+    bsp.kv_append(cache, nothing, nothing, i32([0, zeros]), i32([0]), pages)
+    assert bool((cache.k_scale[1] == 1).all()) and not bool((cache.k[1] & 127).any())
+    bsp.kv_append(cache, xt, xt, i32([0, after]), i32([zeros]), pages)
+    bsp.device().synchronize()
+    e = np.array([ref.exponent(np.abs(x[:, h]).max()) for h in range(hk)])
+    for codes, scale in ((cache.k, cache.k_scale), (cache.v, cache.v_scale)):
+        assert np.array_equal(host(scale)[1], 2.0 ** e)
+        got = codes.cpu().numpy()[1]
+        for h in range(hk):
+            assert np.array_equal(got[h, zeros: zeros + after], ref.e4m3(x[:, h].astype(float) * 2.0 ** -e[h]))
+        assert not (got[:, :zeros] & 127).any()
+    # the smallest code of one earlier token is a value that has to stay
+    cache = bsp.KvCache.empty(2, hk, page, d)
+    bsp.kv_append(cache, nothing, nothing, i32([0, zeros]), i32([0]), pages)
+    cache.k[1, hk - 1, zeros // 2, d - 1] = 129
+    bsp.kv_append(cache, xt, xt, i32([0, after]), i32([zeros]), pages)
+    bsp.device().synchronize()
+    assert float(cache.k_scale[1, hk - 1]) == 1.0 and int(cache.k[1, hk - 1, zeros // 2, d - 1]) == 129
+    assert np.array_equal(cache.k.cpu().numpy()[1, hk - 1, zeros: zeros + after], ref.e4m3(x[:, hk - 1].astype(float)))
+    assert np.array_equal(host(cache.v_scale)[1], 2.0 ** e)
