@@ -769,6 +769,19 @@ def _stream_of(stream, dev: Device):
     return stream.cuda_stream if hasattr(stream, "cuda_stream") else int(stream)
 
 
+def _empty(shape, dtype, device, stream):
+    """An output that a call on `stream` makes: it belongs to that stream, so its
+    memory is none that kernels still running on the current one may use."""
+    import torch
+
+    if stream is None:
+        return torch.empty(shape, dtype=dtype, device=device)
+    if not isinstance(stream, torch.cuda.Stream):
+        stream = torch.cuda.ExternalStream(_stream_of(stream, None), device=device)
+    with torch.cuda.stream(stream):
+        return torch.empty(shape, dtype=dtype, device=device)
+
+
 def _refuse(msg):
     raise BspError(BSP_ERR_INVALID_ARG, msg)
 
@@ -791,7 +804,7 @@ def rope_table(n_pos, rot, base=10000.0, kind="none", factor=1.0, context=0.0, s
         _refuse(f"scaling {kind!r}: one of {sorted(ROPE_KINDS)}")
     if n_pos < 1 or rot < 2:
         _refuse("n_pos and rot must be positive")
-    table = torch.empty((n_pos, rot // 2, 2), dtype=torch.float32, device=torch.device("cuda", dev.ordinal))
+    table = _empty((n_pos, rot // 2, 2), torch.float32, torch.device("cuda", dev.ordinal), stream)
     sc = RopeScaling(ROPE_KINDS[kind], factor, context, slow, fast, magnitude)
     _check(lib().bsp_rope_table(dev.handle, n_pos, rot, base, ctypes.byref(sc), _ptr(table), _stream_of(stream, dev)))
     return table
@@ -803,9 +816,7 @@ def rope(x, positions, table, layout="half", transpose=False, out=None, dev: Dev
     head is copied.  transpose=True gives the gradient of x from that of the
     result.  out may be x."""
     if out is None:
-        import torch
-
-        out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        out = _empty(x.shape, x.dtype, x.device, stream)
     (_calls or _load_calls()).rope(x, positions, table, _rope_layout(layout), bool(transpose), out, dev, stream)
     return out
 

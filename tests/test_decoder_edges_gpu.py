@@ -313,3 +313,31 @@ def test_append_small_values_behind_zeros(bsp, page, d, hk, zeros, after, size):
     assert float(cache.k_scale[1, hk - 1]) == 1.0 and int(cache.k[1, hk - 1, zeros // 2, d - 1]) == 129
     assert np.array_equal(cache.k.cpu().numpy()[1, hk - 1, zeros: zeros + after], ref.e4m3(x[:, hk - 1].astype(float)))
     assert np.array_equal(host(cache.v_scale)[1], 2.0 ** e)
+
+
+# ----------------------------------------------------------------- streams --
+@pytest.mark.parametrize("as_number", [False, True])
+def test_outputs_belong_to_the_calls_stream(bsp, as_number):  # noqa: F811
+    """What rope and rope_table allocate comes from the memory of the stream that
+    they run on, and goes back to it: the current stream's kernels never had it."""
+    torch = torch_()
+    s = torch.cuda.Stream()
+    given = s.cuda_stream if as_number else s
+    x, pos = torch.randn((4099, 3, 64), device="cuda"), i32(np.arange(4099))
+    turned = bsp.rope_table(4099, 64)
+    torch.cuda.synchronize()
+    table = bsp.rope_table(4099, 64, stream=given)
+    y = bsp.rope(x, pos, table, stream=given)
+    s.synchronize()
+    assert torch.equal(y, bsp.rope(x, pos, table)) and torch.equal(table, bsp.rope_table(4099, 64))
+    del table, y
+    for make in (lambda: bsp.rope_table(4099, 64, stream=given), lambda: bsp.rope(x, pos, turned, stream=given)):
+        made = make()
+        s.synchronize()
+        at, shape = made.data_ptr(), made.shape
+        del made
+        here = torch.empty(shape, device="cuda")
+        with torch.cuda.stream(torch.cuda.ExternalStream(s.cuda_stream)):
+            there = torch.empty(shape, device="cuda")
+        assert here.data_ptr() != at and there.data_ptr() == at
+    bsp.device().synchronize()
