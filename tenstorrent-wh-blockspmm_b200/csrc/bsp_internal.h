@@ -4,6 +4,7 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
 #include <string>
 #include <vector>
 
@@ -324,7 +325,7 @@ struct bsp_device {
   // area + pinned staging, grow-only) and copy / compute streams
   void* plan_ws = nullptr;
   size_t plan_ws_bytes = 0;
-  bool append_ready = false;  // kernel attributes of bsp_kv_append are set
+  std::atomic<bool> append_ready{false};  // kernel attributes of bsp_kv_append are set (calls come from any thread)
   void* aux_ws = nullptr;   // attention merge workspace of host-buffer plans
   size_t aux_ws_bytes = 0;
   cudaStream_t s_h2d = nullptr, s_comp = nullptr, s_d2h = nullptr;

@@ -341,3 +341,39 @@ def test_outputs_belong_to_the_calls_stream(bsp, as_number):  # noqa: F811
             there = torch.empty(shape, device="cuda")
         assert here.data_ptr() != at and there.data_ptr() == at
     bsp.device().synchronize()
+
+
+def test_first_appends_of_a_device_from_several_threads(bsp):  # noqa: F811
+    """The first append on a device sets the kernels up, whichever thread makes it:
+    eight at once (each has its stream, cache and tensors) give what one gives."""
+    import threading
+
+    torch = torch_()
+    x = torch.randn((300, 2, 128), device="cuda").bfloat16()
+    pages, starts, before = i32(np.arange(19)[None]), i32([0, 300]), i32([0])
+    one = bsp.KvCache.empty(19, 2, 16, 128)
+    bsp.kv_append(one, x, x, starts, before, pages)
+    torch.cuda.synchronize()
+    for _ in range(5):
+        dev = bsp.Device(0)
+        caches, streams = [bsp.KvCache.empty(19, 2, 16, 128) for _ in range(8)], [torch.cuda.Stream() for _ in range(8)]
+        torch.cuda.synchronize()
+        together, failed = threading.Barrier(8), []
+
+        def call(i):
+            try:
+                together.wait(30)
+                bsp.kv_append(caches[i], x, x, starts, before, pages, dev=dev, stream=streams[i])
+            except Exception as e:
+                failed.append(e)
+
+        threads = [threading.Thread(target=call, args=(i,)) for i in range(8)]
+        for t in threads:
+            t.start()
+        for t in threads:
+            t.join()
+        dev.synchronize()
+        torch.cuda.synchronize()
+        assert not failed
+        assert all(torch.equal(c.k, one.k) and torch.equal(c.v_scale, one.v_scale) for c in caches)
+        dev.close()
