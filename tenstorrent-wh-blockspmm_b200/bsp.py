@@ -880,8 +880,9 @@ PROMPT_INFO_KEYS = ["units", "ctas", "q_tokens", "kv_tokens", "heads", "kv_heads
 
 class PromptPlan:
     """Attention over whole prompts packed one after the other: q_lens[s]
-    queries and kv_lens[s] keys of sequence s (host lists); causal: query i
-    sees the keys up to i + (kv_len - q_len).  A plan with a workspace
+    queries and kv_lens[s] keys of sequence s (host lists; the earlier tokens'
+    keys too where a prompt's later part is given, in bf16: no KvCache is read);
+    causal: query i sees the keys up to i + (kv_len - q_len).  A plan with a workspace
     (info()["workspace_bytes"]: few rows of many keys are cut along the keys)
     runs on one stream at a time."""
 

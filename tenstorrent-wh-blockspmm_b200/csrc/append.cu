@@ -9,7 +9,7 @@
 // A job is one head of the keys, the values or the queries of a chunk (the new
 // tokens of one sequence on one page); a team does several of a chunk's jobs.  It
 // has one warp per 16 tokens of its chunk, so a long prompt and many single tokens
-// go together (90 tokens with one each of 63 other sequences: 14.1 us, 37 us with
+// go together (90 tokens with one each of 63 other sequences: 13.3 us, 37 us with
 // one warp a team).  Memory-bound, so the loads of the next job are
 // always in flight: asynchronous copies bring its 16-bit values to shared
 // memory (each lane its own, two buffers), while (cos, sin) of the warp's 16
@@ -18,8 +18,8 @@
 // the passes spilled: 140 us against 91 then).
 //
 // 14278 tokens, 32 + 2 x 8 heads of 128, pages of 16: 66 us, 5400 GB/s, 83 % of a
-// plain copy's rate (56 % of the issue slots, 23 % of the warps: registers allow
-// two blocks an SM).  A token each of 64 sequences: 4.9 us, latency.
+// plain copy's rate (58 % of the issue slots, 23 % of the warps: registers allow
+// two blocks an SM).  A token each of 64 sequences: 5.0 us, latency.
 #include <cuda_fp8.h>
 
 #include "bsp_ptx.cuh"
@@ -383,7 +383,7 @@ bsp_status launch_append(AppendParams& p, bsp_device* dev, cudaStream_t stream) 
   const int64_t per_seq = p.tokens / p.n_seqs;
   // A step of decoding (no more tokens than sequences) whose chunks do not fit the
   // GPU's blocks at once: a warp takes fewer tokens, so that twice as many blocks do
-  // (a token each of 512 sequences 14.1 us, 17.6 us with 16 tokens a warp; of 64
+  // (a token each of 512 sequences 13.4 us, 17.0 us with 16 tokens a warp; of 64
   // sequences 5.0 us either way).
   const bool few = p.tokens <= p.n_seqs && p.n_seqs > 2 * dev->sm_count;
   const int64_t by_page = p.tokens / page + 2 * static_cast<int64_t>(p.n_seqs);

@@ -36,13 +36,14 @@
 // still counts its parts, so the counters stay right for the next launch.
 //
 // Measured: two contexts of 100003 and 131072 tokens, 8 key/value heads of 128
-// for 40 query heads, 86 us (5490 GB/s, 84 % of a plain copy's rate); 64 of 500
-// to 8000 tokens 65 us (5210 GB/s).  Its steady state runs at the copy's rate (a
+// for 40 query heads, 85 us (5580 GB/s, 85 % of a plain copy's rate); 64 of 500
+// to 8000 tokens 65 us (5180 GB/s).  Its steady state runs at the copy's rate (a
 // copy of the kernel that only loads takes 80 and 61 us); the rest, about 10 us,
 // is the launch, the first loads of a CTA and the joining.  24 sequences in
-// pages of 16, 16 heads of 64: 28 us (2980 GB/s), where a box is 1 KB.  One
-// sequence of 1000 tokens: 7.0 us, of which 0.8 are an empty launch, 0.7 finding
-// the tiles, 3.4 a tile from its page number to its result and 2.1 the joining.
+// pages of 16, 16 heads of 64: 29 us (2890 GB/s), where a box is 1 KB.  One
+// sequence of 1000 tokens: 7.2 us (taken apart when it was 7.0: 0.8 an empty
+// launch, 0.7 finding the tiles, 3.4 a tile from its page number to its result and
+// 2.1 the joining).  With b in the running maximum these were 85, 64, 27 and 6.9 us.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -79,10 +80,10 @@ static_assert(sizeof(DcHeader) <= 1024, "header must fit its 1 KiB slot");
 // Shared memory from the 1 KiB-aligned base: header, slots (K and V of a tile
 // in turn), then the warps' results: O [4][heads][d], m [4][heads], l [4][heads].
 // CTAs on an SM: two; four for rows of up to 8 heads of 64, whose tiles are half
-// the bytes for the same work on scores (16 heads of 64 in pages of 16: 39 us
-// with two, 32 with three, 29.5 with four).  Rows of 16 heads with one CTA, which
-// leaves them more registers: 64 contexts of 4000 tokens, 4 key/value heads of
-// 128 73 us, with two 60; heads of 64 55 and 40.
+// the bytes for the same work on scores (16 heads of 64 in pages of 16, the same
+// inputs again and again: 31.8 us with two, 26.8 with three, 25.6 with four).  Rows
+// of 16 heads with one CTA, which leaves them more registers: 64 contexts of 4000
+// tokens, 4 key/value heads of 128 72 us, with two 57; heads of 64 54 and 39.
 __host__ __device__ constexpr int dc_per_sm(int d, int heads) { return heads <= 8 && d == 64 ? 4 : 2; }
 // As many slots as fit the SM's 228 KB then (1 KB of each CTA is the system's).
 __host__ __device__ constexpr int dc_slot_bytes(int d) { return kDcTile * d; }
@@ -196,6 +197,12 @@ __device__ __forceinline__ bool next_piece(const DecodeParams& p, Walk& w, Piece
   return true;
 }
 
+// Copy x of a CTA (K of its first tile 0, V 1, K of the next 2, ...) goes to slot
+// x % kSlots, which with an odd number of slots passes between the two warps.  A
+// parity names a phase only while the others of that parity are over: before copy x
+// its warp waits for the reading of copy x - kSlots, and when it gets there copy
+// x - 2 - kSlots has been read (its last wait), so copy x - 2 kSlots too, since the
+// consumers go in order.
 template <int kD, int kSlots>
 __device__ __forceinline__ void dc_produce(const DecodeParams& p, DcHeader* hdr, uint32_t ring, Walk w,
                                           const WaitCtl& ctl, int kind, int lane) {
@@ -704,8 +711,8 @@ __global__ void __launch_bounds__(kDcThreads, dc_per_sm(kD, 8 * kNt)) decode_ker
     // A tile takes a CTA 1 us, and each part of a row 0.1 us more where they are
     // joined: a row of n tiles in parts of t takes t + 0.1 n / t, least at t =
     // sqrt(0.1 n).  Fewer tiles to a CTA only lengthen the joining (131072 tokens,
-    // one key/value head: 16 tiles a CTA 30 us, 8 32 us, 4 51 us; 8000 tokens: 4
-    // tiles 11.5 us, one 14.5 us).
+    // one key/value head: this rule 29.9 us, 16 tiles a CTA 30.5, 8 31.3, 4 45, one
+    // 51; 8000 tokens: 11.8 us, 16 18.1, 8 13.9, 4 11.7, one 14.8).
     const uint32_t least = max(__float2uint_rn(sqrtf(0.09f * static_cast<float>(longest))), 1u);
     const int ctas = static_cast<int>(min(gridDim.x, (static_cast<uint32_t>(total) + least - 1) / least));
     const uint32_t each = ctas > 0 ? static_cast<uint32_t>(total) / static_cast<uint32_t>(ctas) : 0u;

@@ -3,8 +3,8 @@
 //   O_i = sum_j softmax_j(scale q_i k_j) v_j,  j <= i + (kv_len - q_len).
 //
 // Rows.  A tile is 128 rows = 128 / P queries x P query heads of one key/value
-// head (P: the largest power of two that divides heads / kv_heads), so that a
-// short sequence still fills a tile and a causal tile wastes little on its
+// head (P: the largest power of two up to 32 that divides heads / kv_heads), so
+// that a short sequence still fills a tile and a causal tile wastes little on its
 // diagonal.  One TMA box {64 values, P heads, 128 / P queries} brings it in
 // that order.  A unit is one or two such tiles of consecutive queries; both
 // read the same keys.
