@@ -554,7 +554,8 @@ bsp_status bsp_prompt_plan_info(const bsp_prompt_plan* plan, int64_t info[16]);
  * pages hold behind lens[s] is never used.  The plan is a workspace for up to
  * max_seqs sequences (any lengths) that one launch uses at a time: run a
  * plan's launches on one stream.  Options: max_ctas, timeout_ms.
- * Scores, softmax and sums in fp32; for the product with the codes of V the
+ * Scores, softmax and sums in fp32; q is held in fp16 relative to its head's
+ * largest value (exact down to 2^-17 of it); for the product with the codes of V the
  * weights are rounded to fp16, relative to their page's scale and the largest
  * weight: 2^-11 of a weight, at most 2^-25 of the largest for those far below
  * it.  O is rounded once.  Value scales of a row's pages may be 2^100 apart;

@@ -23,8 +23,8 @@
 // reference: b <= r <= b + 7 for the pages at hand, moved (and O with it, in
 // fp32) only when a page's b leaves that span.
 // e4m3 codes are exact in fp16.  Q is scaled to [1, 2) by a power of two per
-// head before it is rounded to fp16 (bf16's 8 bits fit; what falls below
-// 2^-14 of the head's largest value loses bits that the sum cannot show).
+// head before it is rounded to fp16: bf16's 8 bits fit down to 2^-17 of the head's
+// largest value, below that a value is off by up to 2^-25 of the largest.
 // P' <= 2^15 is rounded to fp16: 2^-11 of a weight, or, far below, 2^-25 of the
 // largest weight (2^-32 where the pages' scales are alike).  Were b part of m, one
 // page of large scale would take all other pages' weights below what fp16 holds,
